@@ -8,7 +8,8 @@
 import sys as _sys
 
 from torchopt_amd import accelerated_op
-from torchopt_amd.accelerated_op import AdamOp, MultiAdamOp
+from torchopt_amd.accelerated_op import (AdamOp, MultiAdamOp, dequantize_blocks, orthogonalize,
+                                         quantize_blocks)
 from torchopt_amd.accelerated_op import is_available as accelerated_op_available
 from torchopt_amd.alias import adam, adamw, apply_updates, chain
 from torchopt_amd.func import FuncOptimizer
@@ -21,9 +22,10 @@ from torchopt_amd.placement import (placed_like_tree, state_empty_like, state_ze
 from torchopt_amd import _C  # noqa: E402
 
 _sys.modules.setdefault('torchopt_amd._C.adam_op', _C.adam_op)
+_sys.modules.setdefault('torchopt_amd._C.muon_op', _C.muon_op)
 
 __version__ = '0.1.0'
 
 __all__ = ['Adam', 'AdamOp', 'AdamW', 'FuncOptimizer', 'FusedAdam', 'FusedAdamW', 'MetaAdam', 'MetaAdamW', 'MultiAdamOp', 'accelerated_op',
-           'accelerated_op_available', 'adam', 'adamw', 'apply_updates', 'chain', 'placed_like_tree',
-           'state_empty_like', 'state_zeros_like', 'state_zeros_like_tree', 'unshared']
+           'accelerated_op_available', 'adam', 'adamw', 'apply_updates', 'chain', 'dequantize_blocks',
+           'orthogonalize', 'placed_like_tree', 'quantize_blocks', 'state_empty_like', 'state_zeros_like', 'state_zeros_like_tree', 'unshared']

@@ -9,8 +9,11 @@ from typing import Iterable, Union
 import torch
 
 from torchopt_amd.accelerated_op.adam_op import AdamOp, MultiAdamOp
+from torchopt_amd.accelerated_op.muon_op import (dequantize_blocks, orthogonalize,
+                                                 quantize_blocks)
 
-__all__ = ['AdamOp', 'MultiAdamOp', 'is_available']
+__all__ = ['AdamOp', 'MultiAdamOp', 'dequantize_blocks', 'is_available', 'orthogonalize',
+           'quantize_blocks']
 
 Device = Union[torch.device, str, int]
 

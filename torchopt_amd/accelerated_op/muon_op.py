@@ -1,0 +1,157 @@
+"""`orthogonalize`: Newton-Schulz orthogonalisation of matrices, differentiable, and the 8-bit
+blocks an optimizer can keep its momentum in.
+
+The reference has no counterpart; the manners are those of `AdamOp`: `torchopt_amd._C.muon_op`
+(hand-written gfx950 kernels) and nothing else behind it, GPU tensors only, work on the current
+stream, whole lists in one call.
+
+For a matrix ``G`` with ``X = G / (|G|_F + eps)``, each of `steps` times
+
+    ``X <- a X + b (X X^T) X + c (X X^T)^2 X``
+
+takes the singular values of ``X`` through the polynomial ``a t + b t^3 + c t^5`` and leaves its
+singular vectors: with the default coefficients every singular value that is not tiny ends between
+0.7 and 1.2, so the result is close to the nearest matrix with orthonormal rows (or columns).
+
+The gradient is the formula's own (through every step and the norm), not that of an ideal
+orthogonalisation.  It is computed from the input, whose iterates are made again on the way: what
+autograd keeps between the passes is the input alone.  It is not differentiable a second time.
+"""
+
+from __future__ import annotations
+
+from typing import Any, Sequence
+
+import torch
+
+try:
+    from torchopt_amd._C import muon_op
+except ImportError as exc:  # no fallback module: the op is the compiled extension or nothing
+    raise ImportError(
+        'torchopt_amd._C, the compiled extension in front of libtoa_muon.so, cannot be '
+        f'imported ({exc}); build it with `python torchopt_amd/build.py`. There is no '
+        'pure-Python or CPU fallback.') from exc
+
+from torch.autograd.function import once_differentiable
+
+
+__all__ = ['COEFFICIENTS', 'dequantize_blocks', 'orthogonalize', 'quantize_blocks']
+
+# the quintic whose slope at zero is steep (small singular values grow 3.4-fold a step) at the
+# price of ending near one instead of at it
+COEFFICIENTS = (3.4445, -4.7750, 2.0315)
+
+
+class _Orthogonalize(torch.autograd.Function):
+    """All matrices of a list as one node."""
+
+    @staticmethod
+    def forward(ctx: Any, series: tuple, *inputs: torch.Tensor):
+        ctx.series = series
+        ctx.save_for_backward(*inputs)
+        ctx.set_materialize_grads(False)
+        return tuple(muon_op.orthogonalize_multi(inputs, *series))
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx: Any, *grads: torch.Tensor | None):
+        inputs = ctx.saved_tensors
+        live = [k for k, g in enumerate(grads) if g is not None and ctx.needs_input_grad[1 + k]]
+        out: list[torch.Tensor | None] = [None] * len(inputs)
+        if live:
+            fresh = muon_op.orthogonalize_backward_multi(
+                [grads[k] for k in live], [inputs[k] for k in live], *ctx.series)
+            for k, g in zip(live, fresh):
+                out[k] = g
+        return (None, *out)
+
+
+def _by_kind(tensors: Sequence[torch.Tensor]) -> list[list[int]]:
+    """Positions of the tensors of each device and dtype."""
+    if _one_kind(tensors):
+        return [list(range(len(tensors)))]
+    kinds: dict[tuple, list[int]] = {}
+    for k, t in enumerate(tensors):
+        kinds.setdefault((t.device, t.dtype), []).append(k)
+    return list(kinds.values())
+
+
+def _one_kind(tensors: Sequence[torch.Tensor]) -> bool:
+    first = tensors[0]
+    return all(t.dtype is first.dtype and t.device == first.device for t in tensors)
+
+
+def orthogonalize(
+    matrices: torch.Tensor | Sequence[torch.Tensor],
+    *,
+    steps: int = 5,
+    coefficients: tuple[float, float, float] = COEFFICIENTS,
+    eps: float = 1e-7,
+):
+    """Orthogonalise a tensor of matrices (its last two dimensions), or every tensor of a list or
+    tuple, whose shapes, dtypes and devices may differ.
+
+    Args:
+        matrices: GPU tensors of float32, float16 or bfloat16, any strides.
+        steps: how often the polynomial is applied, 1 to 32.
+        coefficients: ``(a, b, c)``.  Coefficients under which the iterates could grow beyond
+            2^20 are refused.
+        eps: added to the Frobenius norm.
+
+    Returns:
+        A tensor like `matrices` (a list or tuple of them for a list or tuple), differentiable
+        with respect to it.  Float32 and float16 results come from products with 22-bit operands
+        and float32 sums; for bfloat16 the operands of the last two steps carry 11 bits.
+    """
+    single = isinstance(matrices, torch.Tensor)
+    tensors = [matrices] if single else list(matrices)
+    for t in tensors:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError(f'orthogonalize: expected tensors, got {type(t).__name__}')
+    series = (int(steps), tuple(float(c) for c in coefficients), float(eps))
+    out: list[torch.Tensor | None] = [None] * len(tensors)
+    grad = torch.is_grad_enabled()
+    for ks in _by_kind(tensors) if tensors else []:
+        group = [tensors[k] for k in ks]
+        if grad and any(t.requires_grad for t in group):
+            fresh = _Orthogonalize.apply(series, *group)
+        else:
+            fresh = muon_op.orthogonalize_multi(group, *series)
+        for k, y in zip(ks, fresh):
+            out[k] = y
+    if single:
+        return out[0]
+    return out if isinstance(matrices, list) else type(matrices)(out)
+
+
+def quantize_blocks(tensors: torch.Tensor | Sequence[torch.Tensor]):
+    """8-bit blocks of a dense tensor, or of every tensor of a list: ``(codes, scales)``.
+
+    Each 128 consecutive elements in memory order (the last ones may be fewer) share one float32
+    scale, the largest magnitude among them over 127; the int8 code of an element is its multiple
+    of the scale, rounded half to even.  So an element is off by half a scale at most, and a block
+    of zeros stays one.  A block with a NaN or an infinity stands for NaN throughout."""
+    if isinstance(tensors, torch.Tensor):
+        codes, scales = muon_op.quantize_multi([tensors])
+        return codes[0], scales[0]
+    codes: list = [None] * len(tensors)
+    scales: list = [None] * len(tensors)
+    for ks in _by_kind(tensors) if len(tensors) else []:
+        for k, c, s in zip(ks, *muon_op.quantize_multi([tensors[k] for k in ks])):
+            codes[k], scales[k] = c, s
+    return codes, scales
+
+
+def dequantize_blocks(codes, scales, dtype: torch.dtype = torch.float32):
+    """What `quantize_blocks` made, as a tensor (or list of tensors) of `dtype`."""
+    if isinstance(codes, torch.Tensor):
+        out = torch.empty_like(codes, dtype=dtype)
+        return muon_op.dequantize_multi_([out], [codes], [scales])[0]
+    out = [torch.empty_like(c, dtype=dtype) for c in codes]
+    by_device: dict[torch.device, list[int]] = {}
+    for k, c in enumerate(codes):
+        by_device.setdefault(c.device, []).append(k)
+    for ks in by_device.values():
+        muon_op.dequantize_multi_([out[k] for k in ks], [codes[k] for k in ks],
+                                  [scales[k] for k in ks])
+    return out

@@ -1,0 +1,872 @@
+// Device code of libtoa_muon.so: see include/toa_muon.h for what the operators compute.
+//
+// Every matrix is worked on in its wide orientation (s rows, w columns, s <= w; a tall one is
+// read and written turned).  Per step k of the series, with X = X_k:
+//     S = X X^T            (s x s, symmetric: lower tiles only, mirrored when stored)
+//     P = b S + c S S      (symmetric too)
+//     X' = a X + P X
+// and for the gradient, with the cotangent Y of X' (all from the formulas, S and P symmetric):
+//     M = Y X^T + X Y^T,   N = b M + c (M S + S M),   Y_prev = a Y + P Y + N X.
+// All of them are sums of products A B^T of row-major operands, so ONE kernel computes them: a
+// tile of up to two products with a common sum, plus a multiple of a third matrix, stored in both
+// orientations (X and X^T; for the symmetric ones the mirror image).
+//
+// Operands.  The matrix cores multiply halves; an operand element is kept as hi + lo, two halves
+// that together carry 22 bits, and a product is hi hi + hi lo + lo hi with float32 sums (what is
+// dropped, lo lo, is 2^-22 of it).  Halves have few exponents, so every matrix is stored times a
+// power of two that takes its bound to 2^13..2^14: |X_k| <= max of the polynomial on the previous
+// interval (from the start's norm, 1 or less), and products of such bounds for the others.  An
+// element is at most the spectral norm, so nothing overflows, and what lies 2^-24 below the bound
+// still has all its bits.  ("half" operands keep hi alone: 11 bits.)
+//
+// Layout.  A row of an operand is a run of 128-byte pieces: [32 hi | 32 lo] of 32 columns, or 64
+// halves of 64 columns.  Either way one piece of each row is what a tile step consumes.  Columns
+// beyond the matrix are zero up to a multiple of 64.
+#pragma once
+
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+namespace toa_muon {
+
+typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+constexpr int kMaxGroups = 16;   // distinct shapes in one launch
+constexpr int kMaxSteps = 32;
+constexpr int kMaxParts = 256;   // partial sums per matrix
+constexpr int kBlock = 128;      // elements of an 8-bit block
+constexpr int kPiece = 128;      // bytes of a row that one tile step consumes
+constexpr int kPad = 64;         // columns are padded to a multiple of this
+
+// What a kernel needs to know of the caller's tensors, in the wide orientation.
+struct MatRec {
+    const void *g;     // the matrix (orthogonalize), or its gradient (step)
+    const void *aux;   // the momentum (step), or the cotangent (gradient)
+    void *out;
+    float *scales;     // of an 8-bit momentum
+    int64_t g_rs, g_cs, aux_rs, aux_cs, out_rs, out_cs;
+    float rate, keep;  // out <- keep * out - rate * result (step), or rate * result
+};
+
+// Sums over a matrix and what follows from them.
+struct MatNorm {
+    double x_scale;    // 2^e / (|G| + eps): what G is multiplied with on its way to X_0
+    double y_scale;    // 2^e for the cotangent
+    double size;       // |G|_F
+    double plus;       // |G|_F + eps
+};
+
+struct Group {         // matrices of one shape
+    int64_t base;      // bytes from the workspace to the first one's region
+    int64_t stride;    // bytes from one region to the next
+    int s, w, mat0, tile0, tiles;  // tiles: per matrix, of this launch
+};
+
+struct Shapes {
+    int n;
+    Group g[kMaxGroups];
+};
+
+__device__ inline float toFloat(float v) { return v; }
+__device__ inline float toFloat(_Float16 v) { return (float)v; }
+__device__ inline float toFloat(__bf16 v) { return (float)v; }
+template <typename T> __device__ inline T fromFloat(float v) { return (T)v; }
+
+// The group and the matrix a workgroup belongs to; `tile` becomes the tile's number in it.
+__device__ inline int findGroup(const Shapes &sh, int &tile, int &mat) {
+    int k = 0;
+    while (k + 1 < sh.n && tile >= sh.g[k + 1].tile0) ++k;
+    tile -= sh.g[k].tile0;
+    mat = tile / sh.g[k].tiles;
+    tile -= mat * sh.g[k].tiles;
+    return k;
+}
+
+__device__ inline double blockSum(double v, double *lds) {
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    double s = 0.0;
+    for (unsigned i = 0; i < blockDim.x / 64; ++i) s += lds[i];
+    __syncthreads();
+    return s;
+}
+
+// ---- the records -----------------------------------------------------------------------------
+
+constexpr int kFill = 32;
+struct FillArgs {
+    MatRec r[kFill];
+};
+// Records travel in the launch's own arguments: no host buffer has to outlive the call, and a
+// captured graph holds them by value.
+__global__ void fill_kernel(FillArgs a, MatRec *dst, int n) {
+    const int i = threadIdx.x;
+    if (i < n) dst[i] = a.r[i];
+}
+
+// ---- the momentum and the norms --------------------------------------------------------------
+//
+// One pass over G (or g and M), in memory order where the matrix is dense: sums of squares in
+// double (no overflow, no dependence on how many there are), a partial sum per workgroup, added
+// up in a fixed order by factors_kernel.
+
+enum { kSumG = 0, kSumAux = 1, kMomentum = 2, kMomentumF32 = 3, kMomentumI8 = 4 };
+
+struct SumArgs {
+    Shapes sh;
+    const MatRec *recs;
+    double *parts;     // [matrix][kMaxParts]
+    float momentum, sign;
+    double momentum64;
+    int nesterov;
+    int64_t per[kMaxGroups];  // elements per workgroup, a multiple of 2048
+};
+
+template <typename T> __device__ inline void load8(const T *p, int valid, float (&v)[8]) {
+    if (valid >= 8 && ((uintptr_t)p & 15) == 0) {
+        typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+        for (unsigned q = 0; q < 8 / (16 / sizeof(T)); ++q) {
+            const vec t = ((const vec *)p)[q];
+#pragma unroll
+            for (unsigned i = 0; i < 16 / sizeof(T); ++i) v[q * (16 / sizeof(T)) + i] = toFloat((T)t[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < valid ? toFloat(p[i]) : 0.f;
+    }
+}
+
+template <typename T> __device__ inline void store8(T *p, int valid, const float (&v)[8]) {
+    if (valid >= 8 && ((uintptr_t)p & 15) == 0) {
+        typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
+#pragma unroll
+        for (unsigned q = 0; q < 8 / (16 / sizeof(T)); ++q) {
+            vec t;
+#pragma unroll
+            for (unsigned i = 0; i < 16 / sizeof(T); ++i) t[i] = fromFloat<T>(v[q * (16 / sizeof(T)) + i]);
+            ((vec *)p)[q] = t;
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < valid) p[i] = fromFloat<T>(v[i]);
+    }
+}
+
+// Largest magnitude of the 16 lanes that share an 8-bit block, as bits (a NaN is the largest).
+__device__ inline unsigned long long blockPeak(unsigned long long m) {
+#pragma unroll
+    for (int o = 8; o; o >>= 1) {
+        const unsigned long long t = __shfl_xor(m, o);
+        m = t > m ? t : m;
+    }
+    return m;
+}
+
+// The scale of a block whose largest magnitude has the bits `peak`: NaN where that is not finite,
+// so that the whole block stands for NaN.
+__device__ inline float scaleOf(unsigned long long peak) {
+    if (peak >= 0x7ff0000000000000ull) return __int_as_float(0x7fc00000);
+    return (float)(__longlong_as_double((long long)peak) / 127.0);
+}
+
+__device__ inline int codeOf(double v, float scale) {
+    if (!(scale > 0.f)) return 0;
+    // (a scale too small for float32's normal range may be rounded to half of peak / 127)
+    const double q = __builtin_rint(v / (double)scale);
+    return (int)(q > 127.0 ? 127.0 : q < -127.0 ? -127.0 : q);
+}
+
+template <typename T, int KIND>
+__global__ __launch_bounds__(256) void sum_kernel(SumArgs a) {
+    __shared__ double lds[4];
+    int part = blockIdx.x, mat;
+    const int gi = findGroup(a.sh, part, mat);
+    const Group &g = a.sh.g[gi];
+    mat += g.mat0;
+    const MatRec &r = a.recs[mat];
+    const int64_t n = (int64_t)g.s * g.w;
+    const int64_t from = part * a.per[gi];
+    const int64_t to = from + a.per[gi] < n ? from + a.per[gi] : n;
+    const T *src = (const T *)(KIND == kSumAux ? r.aux : r.g);
+    const int64_t rs = KIND == kSumAux ? r.aux_rs : r.g_rs;
+    const int64_t cs = KIND == kSumAux ? r.aux_cs : r.g_cs;
+    // the steps' tensors are dense by contract
+    const bool flat = KIND >= kMomentum || (cs == 1 && rs == g.w) || (rs == 1 && cs == g.s);
+    double sum = 0.0;
+    // In double: values next to a border (decay rates are short decimals, 16-bit values short
+    // binary fractions, so ties are common) round as the exact sum does, whatever the type.
+    auto next = [&](double m, float grad) { return a.momentum64 * m + (double)grad; };
+    for (int64_t e = from + (int64_t)threadIdx.x * 8; (e & ~(int64_t)127) < to; e += 2048) {
+        // (the bound keeps the 16 lanes of an 8-bit block together)
+        const int valid = e >= to ? 0 : to - e < 8 ? (int)(to - e) : 8;
+        float v[8];
+        if (KIND == kSumG || KIND == kSumAux) {
+            if (flat) {
+                load8(src + e, valid, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int64_t x = e + i, row = x / g.w, col = x - row * g.w;
+                    v[i] = i < valid ? toFloat(src[row * rs + col * cs]) : 0.f;
+                }
+            }
+        } else {
+            float grad[8], m[8];
+            load8(src + e, valid, grad);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) grad[i] *= a.sign;
+            if (KIND == kMomentumI8) {
+                int8_t *codes = (int8_t *)const_cast<void *>(r.aux) + e;
+                const float old = valid ? r.scales[e >> 7] : 0.f;
+                double d[8];
+                unsigned long long peak = 0;
+                int8_t c[8];
+                if (valid == 8 && ((uintptr_t)codes & 7) == 0) {
+                    *(int2 *)c = *(const int2 *)codes;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) c[i] = i < valid ? codes[i] : (int8_t)0;
+                }
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    d[i] = i < valid ? next((double)c[i] * (double)old, grad[i]) : 0.0;
+                    const unsigned long long mag =
+                        (unsigned long long)__double_as_longlong(d[i]) & 0x7fffffffffffffffull;
+                    peak = mag > peak ? mag : peak;
+                }
+                const float scale = scaleOf(blockPeak(peak));
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    c[i] = (int8_t)codeOf(d[i], scale);
+                    m[i] = (float)c[i] * scale;
+                }
+                if (valid == 8 && ((uintptr_t)codes & 7) == 0) {
+                    *(int2 *)codes = *(const int2 *)c;
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; ++i)
+                        if (i < valid) codes[i] = c[i];
+                }
+                if (valid && (e & 127) == 0) r.scales[e >> 7] = scale;
+            } else if (KIND == kMomentumF32) {
+                float *buf = (float *)const_cast<void *>(r.aux) + e;
+                load8(buf, valid, m);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) m[i] = (float)next(m[i], grad[i]);
+                store8(buf, valid, m);
+            } else {
+                T *buf = (T *)const_cast<void *>(r.aux) + e;
+                load8(buf, valid, m);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    m[i] = toFloat(fromFloat<T>((float)next(m[i], grad[i])));
+                store8(buf, valid, m);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                v[i] = a.nesterov ? __builtin_fmaf(a.momentum, m[i], grad[i]) : m[i];
+                if (i >= valid) v[i] = 0.f;  // (0 * NaN of a block that stands for NaN)
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += (double)v[i] * (double)v[i];
+    }
+    sum = blockSum(sum, lds);
+    if (threadIdx.x == 0) a.parts[(int64_t)mat * kMaxParts + part] = sum;
+}
+
+// ---- scales and factors ----------------------------------------------------------------------
+
+struct Factor {
+    float acc, add, turn, pad;  // result = acc * sum + add * E; turn: the sum between the products
+};
+
+struct FactorArgs {
+    const double *parts, *parts_y;  // parts_y: of the cotangent, or null
+    MatNorm *norms;
+    Factor *factors;                // [matrix][stages]
+    int steps, stages, nparts_pad;
+    float a, b, c;
+    double eps, rho;                // rho: max |p(t) / t| over every interval
+    double x[kMaxSteps + 1];        // bound of |X_k| from a start of norm 1
+    double d[kMaxSteps];            // bound of |p'| on [0, x_k]
+    int nparts[kMaxGroups], mat_end[kMaxGroups], ngroups;
+};
+
+// The power of two that takes a bound to at most 2^14.
+__device__ inline int expOf(double bound) {
+    if (!(bound > 1e-36)) bound = 1e-36;
+    const int e = 13 - ilogb(bound);
+    return e > 120 ? 120 : e < -110 ? -110 : e;
+}
+
+__device__ inline double startOf(double size, double eps) {
+    const double s0 = size / (size + eps);
+    return s0 > 1e-30 && s0 <= 1.0 ? s0 : s0 <= 1e-30 ? 1e-30 : 1.0;  // NaN: as if 1
+}
+
+// One workgroup per matrix: norm, then a thread per step for the factors of its stages.
+__global__ __launch_bounds__(256) void factors_kernel(FactorArgs a) {
+    __shared__ double lds[4];
+    const int mat = blockIdx.x, t = threadIdx.x;
+    int k = 0;
+    while (k + 1 < a.ngroups && mat >= a.mat_end[k]) ++k;
+    const int np = a.nparts[k];
+    const double size = sqrt(blockSum(t < np ? a.parts[(int64_t)mat * kMaxParts + t] : 0.0, lds));
+    const double ysize =
+        a.parts_y ? sqrt(blockSum(t < np ? a.parts_y[(int64_t)mat * kMaxParts + t] : 0.0, lds)) : 0.0;
+    const double s0 = startOf(size, a.eps), plus = size + a.eps;
+    auto bound = [&](int i) {
+        double grown = s0;
+        for (int j = 0; j < i; ++j) grown *= a.rho;
+        return grown < a.x[i] ? grown : a.x[i];
+    };
+    auto ybound = [&](int i) {  // of the cotangent of X_i
+        double v = ysize == ysize && ysize < 1e300 ? ysize : 1.0;
+        for (int j = a.steps - 1; j >= i; --j) v *= a.d[j];
+        return v;
+    };
+    if (t == 0) {
+        MatNorm n;
+        n.x_scale = ldexp(1.0 / plus, expOf(bound(0)));
+        n.y_scale = ldexp(1.0, expOf(ybound(a.steps)));
+        n.size = size;
+        n.plus = plus;
+        a.norms[mat] = n;
+    }
+    if (t >= a.steps) return;
+    const double x = bound(t), ab = fabs((double)a.b), ac = fabs((double)a.c);
+    const int ex = expOf(x), es = expOf(x * x), ep = expOf(ab * x * x + ac * x * x * x * x);
+    const bool last = t + 1 == a.steps;
+    const int ex1 = last && !a.parts_y ? 0 : expOf(bound(t + 1));
+    Factor *f = a.factors + (int64_t)mat * a.stages + 3 * t;
+    f[0] = {ldexpf(1.f, es - 2 * ex), 0.f, 1.f, 0.f};
+    f[1] = {ldexpf(a.c, ep - 2 * es), ldexpf(a.b, ep - es), 1.f, 0.f};
+    f[2] = {ldexpf(1.f, ex1 - ep - ex), ldexpf(a.a, ex1 - ex), 1.f, 0.f};
+    if (!a.parts_y) return;
+    const double y1 = ybound(t + 1);
+    const int ey1 = expOf(y1), ey = t ? expOf(ybound(t)) : 0;
+    const int em = expOf(2.0 * x * y1), en = expOf((ab + 2.0 * ac * x * x) * 2.0 * x * y1);
+    f = a.factors + (int64_t)mat * a.stages + 3 * a.steps + 3 * t;
+    f[0] = {ldexpf(1.f, em - ey1 - ex), 0.f, 1.f, 0.f};
+    f[1] = {ldexpf(a.c, en - em - es), ldexpf(a.b, en - em), 1.f, 0.f};
+    f[2] = {ldexpf(1.f, ey - en - ex), ldexpf(a.a, ey - ey1), ldexpf(1.f, (en + ex) - (ep + ey1)), 0.f};
+}
+
+// ---- operands ----------------------------------------------------------------------------------
+
+// Eight consecutive columns (a multiple of 8) of an operand row.
+__device__ inline void storeOperand(char *row, int col, const float (&v)[8], bool split) {
+    half8 hi, lo;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        hi[i] = (_Float16)v[i];
+        lo[i] = (_Float16)(v[i] - (float)hi[i]);
+    }
+    if (split) {
+        char *p = row + (col >> 5) * kPiece + (col & 31) * 2;
+        *(half8 *)p = hi;
+        *(half8 *)(p + 64) = lo;
+    } else {
+        *(half8 *)(row + col * 2) = hi;
+    }
+}
+
+__device__ inline void loadOperand(const char *row, int col, float (&v)[8], bool split) {
+    if (split) {
+        const char *p = row + (col >> 5) * kPiece + (col & 31) * 2;
+        const half8 hi = *(const half8 *)p, lo = *(const half8 *)(p + 64);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)hi[i] + (float)lo[i];
+    } else {
+        const half8 hi = *(const half8 *)(row + col * 2);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = (float)hi[i];
+    }
+}
+
+// Bytes of an operand row of `cols` padded columns.
+__host__ __device__ inline int64_t rowBytes(int64_t padded, bool split) {
+    return padded * (split ? 4 : 2);
+}
+
+__host__ __device__ inline int64_t padded(int64_t n) { return (n + kPad - 1) / kPad * kPad; }
+
+enum { kPackG = 0, kPackAux = 1, kPackM = 2, kPackMF32 = 3, kPackMI8 = 4 };
+
+struct PackArgs {
+    Shapes sh;
+    const MatRec *recs;
+    const MatNorm *norms;
+    char *ws;
+    int64_t off[kMaxGroups], off_t[kMaxGroups];  // of the operand and of its transpose
+    float momentum, sign;
+    int nesterov, split;
+};
+
+// G (or the step's U, or the cotangent) -> the operand and its transpose, by tiles of 64 x 64.
+template <typename T, int KIND>
+__global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
+    __shared__ float tile[64][65];
+    int t = blockIdx.x, mat;
+    const int gi = findGroup(a.sh, t, mat);
+    const Group &g = a.sh.g[gi];
+    char *region = a.ws + g.base + mat * g.stride;
+    mat += g.mat0;
+    const MatRec &r = a.recs[mat];
+    const int across = (int)(padded(g.w) / 64);
+    const int i0 = t / across * 64, j0 = t % across * 64;
+    const double scale = KIND == kPackAux ? a.norms[mat].y_scale : a.norms[mat].x_scale;
+    const T *src = (const T *)(KIND == kPackAux ? r.aux : r.g);
+    const int64_t rs = KIND == kPackAux ? r.aux_rs : r.g_rs, cs = KIND == kPackAux ? r.aux_cs : r.g_cs;
+    const bool by_rows = cs <= rs;  // lanes run along the smaller stride
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll 4
+    for (int q = wave; q < 64; q += 4) {
+        const int di = by_rows ? q : lane, dj = by_rows ? lane : q;
+        const int i = i0 + di, j = j0 + dj;
+        float v = 0.f;
+        if (i < g.s && j < g.w) {
+            const int64_t at = i * rs + j * cs;
+            v = toFloat(src[at]);
+            if (KIND >= kPackM) {
+                float m;
+                if (KIND == kPackMI8)
+                    m = (float)((const int8_t *)r.aux)[at] * r.scales[at >> 7];
+                else if (KIND == kPackMF32)
+                    m = ((const float *)r.aux)[at];
+                else
+                    m = toFloat(((const T *)r.aux)[at]);
+                v = a.nesterov ? __builtin_fmaf(a.momentum, m, a.sign * v) : m;
+            }
+            v = (float)((double)v * scale);
+        }
+        tile[di][dj] = v;
+    }
+    __syncthreads();
+    const int64_t sp = padded(g.s), wp = padded(g.w);
+    const int64_t ld = rowBytes(wp, a.split), ld_t = rowBytes(sp, a.split);
+    for (int q = threadIdx.x; q < 512; q += 256) {
+        const int d = q >> 3, c = (q & 7) * 8;
+        float v[8];
+        if (i0 + d < g.s) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = tile[d][c + i];
+            storeOperand(region + a.off[gi] + (i0 + d) * ld, j0 + c, v, a.split);
+        }
+        if (j0 + d < g.w) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = tile[c + i][d];
+            storeOperand(region + a.off_t[gi] + (j0 + d) * ld_t, i0 + c, v, a.split);
+        }
+    }
+}
+
+// ---- the product -------------------------------------------------------------------------------
+
+enum { kToOperand = 0, kToTensor = 1, kToParam = 2, kToFloat = 3 };
+
+struct Product {             // one matrix's operands, as byte offsets into its region
+    int64_t a0, b0, a1, b1;  // rows of A and of B: sum over both pairs of A B^T
+    int64_t e;               // the third matrix (same shape as the result), or -1
+    int64_t d, dt;           // the result and its transpose, or -1
+    int lda0, ldb0, lda1, ldb1, lde, ldd, lddt;
+    int steps0, steps1;      // pieces of 128 bytes along each pair's rows
+    int rows, cols;
+};
+
+struct GemmArgs {
+    char *ws;
+    const MatRec *recs;
+    const Factor *factors;
+    int stages, stage, symmetric, mode, split_out, tiles_total;
+    Shapes sh;
+    Product p[kMaxGroups];
+};
+
+__device__ inline f32x16 mfma(half8 a, half8 b, f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// Row and column of tile number t: row-major, or the lower triangle of a symmetric result.
+__device__ inline void tileOf(int t, int across, bool symmetric, int &ti, int &tj) {
+    if (symmetric) {
+        ti = (int)((__builtin_sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
+        while (ti * (ti + 1) / 2 > t) --ti;
+        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
+        tj = t - ti * (ti + 1) / 2;
+    } else {
+        ti = t / across;
+        tj = t - ti * across;
+    }
+}
+
+// Tile BM x BN by WM x WN waves.  LDS holds one 128-byte piece of every row of both operands; 16
+// byte chunks of a row are permuted (chunk ^ row % 8) so that the 16-byte reads of a wave, which
+// go down the rows, spread over the banks.
+template <typename T, int BM, int BN, int WM, int WN, bool SPLIT>
+__global__ __launch_bounds__(WM *WN * 64) void gemm_kernel(GemmArgs a) {
+    constexpr int NT = WM * WN * 64;
+    constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 results per wave
+    constexpr int kStage = (BM + BN) * kPiece;
+    constexpr int kScratch = 32 * 36 * 4;                // per wave, for the stores
+    constexpr int kLds = kStage > WM * WN * kScratch ? kStage : WM * WN * kScratch;
+    __shared__ __attribute__((aligned(16))) char lds[kLds];
+
+    int t = blockIdx.x, mat;
+    const int gi = findGroup(a.sh, t, mat);
+    const Product &p = a.p[gi];
+    char *region = a.ws + a.sh.g[gi].base + mat * a.sh.g[gi].stride;
+    mat += a.sh.g[gi].mat0;
+    int ti, tj;
+    tileOf(t, (p.cols + BN - 1) / BN, a.symmetric, ti, tj);
+    const int i0 = ti * BM, j0 = tj * BN;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wi = wave / WN * (BM / WM), wj = wave % WN * (BN / WN);
+    const Factor f = a.factors[(int64_t)mat * a.stages + a.stage];
+
+    f32x16 acc[TM][TN];
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+#pragma unroll
+            for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
+
+    for (int pair = 0; pair < 2; ++pair) {
+        const int steps = pair ? p.steps1 : p.steps0;
+        if (pair && steps) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] *= f.turn;
+        }
+        const char *A = region + (pair ? p.a1 : p.a0), *B = region + (pair ? p.b1 : p.b0);
+        const int64_t lda = pair ? p.lda1 : p.lda0, ldb = pair ? p.ldb1 : p.ldb0;
+        for (int k = 0; k < steps; ++k) {
+            __syncthreads();
+            for (int q = threadIdx.x; q < (BM + BN) * 8; q += NT) {
+                const int row = q >> 3, chunk = q & 7;
+                // rows beyond the matrix repeat its last one; what comes of them is not stored
+                const char *src;
+                if (row < BM) {
+                    const int i = i0 + row < p.rows ? i0 + row : p.rows - 1;
+                    src = A + i * lda;
+                } else {
+                    const int j = j0 + row - BM < p.cols ? j0 + row - BM : p.cols - 1;
+                    src = B + j * ldb;
+                }
+                *(int4 *)(lds + row * kPiece + ((chunk ^ (row & 7)) << 4)) =
+                    *(const int4 *)(src + (int64_t)k * kPiece + (chunk << 4));
+            }
+            __syncthreads();
+            auto frag = [&](int row, int chunk) {
+                row += lane & 31;
+                chunk += lane >> 5;
+                return *(const half8 *)(lds + row * kPiece + ((chunk ^ (row & 7)) << 4));
+            };
+            if (SPLIT) {
+#pragma unroll
+                for (int slab = 0; slab < 2; ++slab) {
+                    half8 ah[TM], al[TM], bh[TN], bl[TN];
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) {
+                        ah[i] = frag(wi + 32 * i, 2 * slab);
+                        al[i] = frag(wi + 32 * i, 4 + 2 * slab);
+                    }
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) {
+                        bh[j] = frag(BM + wj + 32 * j, 2 * slab);
+                        bl[j] = frag(BM + wj + 32 * j, 4 + 2 * slab);
+                    }
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) {
+                            acc[i][j] = mfma(al[i], bh[j], acc[i][j]);
+                            acc[i][j] = mfma(ah[i], bl[j], acc[i][j]);
+                            acc[i][j] = mfma(ah[i], bh[j], acc[i][j]);
+                        }
+                }
+            } else {
+#pragma unroll
+                for (int slab = 0; slab < 4; ++slab) {
+                    half8 ah[TM], bh[TN];
+#pragma unroll
+                    for (int i = 0; i < TM; ++i) ah[i] = frag(wi + 32 * i, 2 * slab);
+#pragma unroll
+                    for (int j = 0; j < TN; ++j) bh[j] = frag(BM + wj + 32 * j, 2 * slab);
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int j = 0; j < TN; ++j) acc[i][j] = mfma(ah[i], bh[j], acc[i][j]);
+                }
+            }
+        }
+    }
+
+    // Results leave by 32 x 32 blocks through LDS, eight to a lane: along rows for the result,
+    // along columns for its transpose.
+    __syncthreads();
+    float *box = (float *)(lds + wave * kScratch);
+    const MatRec &r = a.recs[mat];
+    const bool tensor = a.mode == kToTensor || a.mode == kToParam;
+    const bool turned = tensor && r.out_rs < r.out_cs;
+#pragma unroll
+    for (int i = 0; i < TM; ++i)
+#pragma unroll
+        for (int j = 0; j < TN; ++j) {
+            const int bi = i0 + wi + 32 * i, bj = j0 + wj + 32 * j;
+            if (bi >= p.rows && !(p.dt >= 0 && bi < padded(p.rows))) continue;
+            if (bj >= p.cols && !(p.d >= 0 && bj < padded(p.cols))) continue;
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+                box[((q >> 2) * 8 + (lane >> 5) * 4 + (q & 3)) * 36 + (lane & 31)] = acc[i][j][q];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int row = half * 16 + (lane >> 2), col = (lane & 3) * 8;
+                float v[8], e[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[q] = box[row * 36 + col + q] * f.acc;
+                if (p.e >= 0 && bi + row < p.rows && bj + col < p.cols) {
+                    loadOperand(region + p.e + (int64_t)(bi + row) * p.lde, bj + col, e, SPLIT);
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) v[q] += f.add * e[q];
+                }
+#pragma unroll
+                for (int q = 0; q < 8; ++q)
+                    if (bi + row >= p.rows || bj + col + q >= p.cols) v[q] = 0.f;
+                if (a.mode == kToOperand) {
+                    if (p.d >= 0 && bi + row < p.rows)
+                        storeOperand(region + p.d + (int64_t)(bi + row) * p.ldd, bj + col, v,
+                                     a.split_out);
+                } else if (a.mode == kToFloat) {
+                    if (bi + row < p.rows && bj + col < p.cols) {
+                        float *o = (float *)(region + p.d + (int64_t)(bi + row) * p.ldd) + bj + col;
+                        store8(o, p.cols - bj - col, v);
+                    }
+                } else if (!turned && bi + row < p.rows && bj + col < p.cols) {
+                    T *o = (T *)r.out + (bi + row) * r.out_rs + (bj + col) * r.out_cs;
+                    const int valid = p.cols - bj - col;
+                    if (r.out_cs == 1) {
+                        if (a.mode == kToParam) {
+                            load8(o, valid, e);
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) v[q] = r.keep * e[q] - r.rate * v[q];
+                        } else {
+#pragma unroll
+                            for (int q = 0; q < 8; ++q) v[q] *= r.rate;
+                        }
+                        store8(o, valid, v);
+                    } else {
+                        for (int q = 0; q < 8 && q < valid; ++q) {
+                            T *x = o + q * r.out_cs;
+                            *x = fromFloat<T>(a.mode == kToParam ? r.keep * toFloat(*x) - r.rate * v[q]
+                                                                 : r.rate * v[q]);
+                        }
+                    }
+                }
+                if (p.dt >= 0 || turned) {
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) box[row * 36 + col + q] = v[q];
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            if ((p.dt >= 0 && !(a.symmetric && ti == tj)) || turned) {
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    const int col = half * 16 + (lane >> 2), row = (lane & 3) * 8;
+                    if (bj + col >= p.cols) continue;
+                    float v[8], e[8];
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) v[q] = box[(row + q) * 36 + col];
+                    if (a.mode == kToOperand) {
+                        storeOperand(region + p.dt + (int64_t)(bj + col) * p.lddt, bi + row, v,
+                                     a.split_out);
+                    } else if (turned && bi + row < p.rows) {
+                        T *o = (T *)r.out + (bi + row) * r.out_rs + (bj + col) * r.out_cs;
+                        const int valid = p.rows - bi - row;
+                        if (r.out_rs == 1) {
+                            if (a.mode == kToParam) {
+                                load8(o, valid, e);
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) v[q] = r.keep * e[q] - r.rate * v[q];
+                            } else {
+#pragma unroll
+                                for (int q = 0; q < 8; ++q) v[q] *= r.rate;
+                            }
+                            store8(o, valid, v);
+                        } else {
+                            for (int q = 0; q < 8 && q < valid; ++q) {
+                                T *x = o + q * r.out_rs;
+                                *x = fromFloat<T>(a.mode == kToParam
+                                                      ? r.keep * toFloat(*x) - r.rate * v[q]
+                                                      : r.rate * v[q]);
+                            }
+                        }
+                    }
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+        }
+}
+
+// ---- the end of the gradient: through X_0 = G / (|G| + eps) ------------------------------------
+//
+//     dG = Y_0 / (|G| + eps) - X_0 <Y_0, X_0> / |G|
+
+struct TailArgs {
+    Shapes sh;
+    const MatRec *recs;
+    const MatNorm *norms;
+    char *ws;
+    double *parts;                              // <Y_0, X_0 * 2^e>
+    int64_t y[kMaxGroups], x[kMaxGroups];       // float rows of Y_0; operand rows of X_0
+    int64_t rows_per[kMaxGroups];               // dot: rows per workgroup
+    int nparts[kMaxGroups], split;
+};
+
+__global__ __launch_bounds__(256) void dot_kernel(TailArgs a) {
+    __shared__ double lds[4];
+    int part = blockIdx.x, mat;
+    const int gi = findGroup(a.sh, part, mat);
+    const Group &g = a.sh.g[gi];
+    const char *region = a.ws + g.base + mat * g.stride;
+    mat += g.mat0;
+    const int64_t wp = padded(g.w), ld = rowBytes(wp, a.split);
+    const int from = (int)(part * a.rows_per[gi]);
+    const int to = from + a.rows_per[gi] < g.s ? (int)(from + a.rows_per[gi]) : g.s;
+    double sum = 0.0;
+    const int across = (int)(wp / 8);
+    for (int64_t q = threadIdx.x; q < (int64_t)(to - from) * across; q += 256) {
+        const int i = from + (int)(q / across), j = (int)(q % across) * 8;
+        if (j >= g.w) continue;
+        float x[8], y[8];
+        loadOperand(region + a.x[gi] + i * ld, j, x, a.split);
+        load8((const float *)(region + a.y[gi]) + i * wp + j, g.w - j, y);
+#pragma unroll
+        for (int k = 0; k < 8; ++k) sum += (double)x[k] * (double)y[k];
+    }
+    sum = blockSum(sum, lds);
+    if (threadIdx.x == 0) a.parts[(int64_t)mat * kMaxParts + part] = sum;
+}
+
+template <typename T> __global__ __launch_bounds__(256) void tail_kernel(TailArgs a) {
+    __shared__ float tile[64][65];
+    __shared__ double lds[4];
+    int t = blockIdx.x, mat;
+    const int gi = findGroup(a.sh, t, mat);
+    const Group &g = a.sh.g[gi];
+    const char *region = a.ws + g.base + mat * g.stride;
+    mat += g.mat0;
+    const MatRec &r = a.recs[mat];
+    const MatNorm n = a.norms[mat];
+    const double dot = blockSum(
+        (int)threadIdx.x < a.nparts[gi] ? a.parts[(int64_t)mat * kMaxParts + threadIdx.x] : 0.0, lds);
+    const double back = 1.0 / (n.x_scale * n.plus);  // stored X_0 * back = X_0 (a power of two)
+    const double ky = 1.0 / n.plus;
+    const double kx = n.size > 0.0 ? dot * back / n.size * back : n.size;  // (NaN stays NaN)
+    const int64_t wp = padded(g.w), ld = rowBytes(wp, a.split);
+    const int across = (int)(wp / 64), i0 = t / across * 64, j0 = t % across * 64;
+    for (int q = threadIdx.x; q < 512; q += 256) {
+        const int i = i0 + (q >> 3), c = (q & 7) * 8, j = j0 + c;
+        float x[8], y[8];
+        if (i < g.s && j < g.w) {
+            loadOperand(region + a.x[gi] + i * ld, j, x, a.split);
+            load8((const float *)(region + a.y[gi]) + i * wp + j, g.w - j, y);
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+                tile[q >> 3][c + k] = (float)(ky * (double)y[k] - kx * (double)x[k]);
+        }
+    }
+    __syncthreads();
+    const bool by_rows = r.out_cs <= r.out_rs;
+    const int lane = threadIdx.x & 63;
+    for (int q = threadIdx.x >> 6; q < 64; q += 4) {
+        const int di = by_rows ? q : lane, dj = by_rows ? lane : q;
+        if (i0 + di < g.s && j0 + dj < g.w)
+            ((T *)r.out)[(i0 + di) * r.out_rs + (j0 + dj) * r.out_cs] = fromFloat<T>(tile[di][dj]);
+    }
+}
+
+// ---- 8-bit blocks ------------------------------------------------------------------------------
+
+constexpr int kListMax = 64;
+struct BlocksArgs {
+    int n;
+    const void *in[kListMax];
+    void *out[kListMax];
+    float *scales[kListMax];
+    size_t count[kListMax];
+    unsigned tile0[kListMax];  // a workgroup takes 2048 elements
+};
+
+__device__ inline int findArray(const BlocksArgs &a, unsigned b) {
+    int lo = 0, hi = a.n - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (b >= a.tile0[mid]) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+}
+
+template <typename T> __global__ __launch_bounds__(256) void quantize_kernel(BlocksArgs a) {
+    const int k = findArray(a, blockIdx.x);
+    const int64_t n = (int64_t)a.count[k];
+    const int64_t e = (int64_t)(blockIdx.x - a.tile0[k]) * 2048 + (int64_t)threadIdx.x * 8;
+    const int valid = e >= n ? 0 : n - e < 8 ? (int)(n - e) : 8;
+    float v[8];
+    unsigned long long peak = 0;
+    load8((const T *)a.in[k] + e, valid, v);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const unsigned long long m =
+            (unsigned long long)__double_as_longlong((double)v[i]) & 0x7fffffffffffffffull;
+        peak = m > peak ? m : peak;
+    }
+    const float scale = scaleOf(blockPeak(peak));
+    int8_t c[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = (int8_t)codeOf((double)v[i], scale);
+    int8_t *o = (int8_t *)a.out[k] + e;
+    if (valid == 8 && ((uintptr_t)o & 7) == 0) {
+        *(int2 *)o = *(const int2 *)c;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+            if (i < valid) o[i] = c[i];
+    }
+    if (valid && (e & 127) == 0) a.scales[k][e >> 7] = scale;
+}
+
+template <typename T> __global__ __launch_bounds__(256) void dequantize_kernel(BlocksArgs a) {
+    const int k = findArray(a, blockIdx.x);
+    const int64_t n = (int64_t)a.count[k];
+    const int64_t e = (int64_t)(blockIdx.x - a.tile0[k]) * 2048 + (int64_t)threadIdx.x * 8;
+    if (e >= n) return;
+    const int valid = n - e < 8 ? (int)(n - e) : 8;
+    const int8_t *p = (const int8_t *)a.in[k] + e;
+    const float scale = a.scales[k][e >> 7];
+    int8_t c[8];
+    if (valid == 8 && ((uintptr_t)p & 7) == 0) {
+        *(int2 *)c = *(const int2 *)p;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = i < valid ? p[i] : (int8_t)0;
+    }
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = (float)c[i] * scale;
+    store8((T *)a.out[k] + e, valid, v);
+}
+
+}  // namespace toa_muon

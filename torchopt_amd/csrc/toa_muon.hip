@@ -1,0 +1,686 @@
+// Host side of libtoa_muon.so (include/toa_muon.h): checks, the plan of a list (matrices sorted by
+// shape, in batches that a workspace of bounded size holds), and the launches.  Everything a kernel
+// reads beside the caller's tensors travels in launch arguments or is made on the device, so a call
+// allocates nothing and leaves nothing behind.
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <limits>
+#include <vector>
+
+#include "muon_kernels.hpp"
+#include "toa_muon.h"
+
+using namespace toa_muon;
+
+namespace {
+
+// A batch's regions stay below this (one matrix alone may be larger).
+constexpr int64_t kBatchBytes = (int64_t)1 << 30;
+constexpr int kBatchMats = 4096;
+constexpr int64_t kMaxDim = (int64_t)1 << 20;
+
+int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+
+// Where one matrix's buffers lie in its region.
+struct Layout {
+    int64_t x[kMaxSteps + 1], xt[kMaxSteps + 1], s[kMaxSteps], p[kMaxSteps];
+    int64_t y[2], yt[2], m, n, yf, bytes;
+};
+
+Layout layoutOf(int s, int w, int steps, bool backward) {
+    Layout l;
+    int64_t at = 0;
+    auto take = [&](int64_t rows, int64_t cols) {
+        const int64_t here = at;
+        at += align256(rows * rowBytes(padded(cols), true));
+        return here;
+    };
+    if (backward) {
+        // every iterate is kept: the way back needs them in reverse
+        for (int k = 0; k < steps; ++k) {
+            l.x[k] = take(s, w);
+            l.xt[k] = take(w, s);
+            l.s[k] = take(s, s);
+            l.p[k] = take(s, s);
+        }
+        for (int k = 0; k < 2; ++k) {
+            l.y[k] = take(s, w);
+            l.yt[k] = take(w, s);
+        }
+        l.m = take(s, s);
+        l.n = take(s, s);
+        l.yf = take(s, w);
+    } else {
+        const int64_t x0 = take(s, w), x0t = take(w, s);
+        const int64_t x1 = steps > 1 ? take(s, w) : 0, x1t = steps > 1 ? take(w, s) : 0;
+        const int64_t ss = take(s, s), pp = take(s, s);
+        for (int k = 0; k < steps; ++k) {
+            l.x[k] = k & 1 ? x1 : x0;
+            l.xt[k] = k & 1 ? x1t : x0t;
+            l.s[k] = ss;
+            l.p[k] = pp;
+        }
+    }
+    l.bytes = at;
+    return l;
+}
+
+struct Batch {
+    std::vector<size_t> mats;  // indices into the caller's list, shape by shape
+    struct Shape {
+        int s, w, mat0, count;
+        int64_t base;
+        Layout lay;
+    };
+    std::vector<Shape> shapes;
+    int64_t bytes = 0;  // of all regions
+};
+
+// Head of the workspace: records, norms, partial sums (two sets) and factors of a batch.
+struct Head {
+    int64_t recs, norms, parts, parts_y, factors, regions;
+};
+
+Head headOf(int64_t mats, int stages) {
+    Head h;
+    h.recs = 0;
+    h.norms = align256(mats * (int64_t)sizeof(MatRec));
+    h.parts = h.norms + align256(mats * (int64_t)sizeof(MatNorm));
+    h.parts_y = h.parts + align256(mats * kMaxParts * 8);
+    h.factors = h.parts_y + align256(mats * kMaxParts * 8);
+    h.regions = h.factors + align256(mats * stages * (int64_t)sizeof(Factor));
+    return h;
+}
+
+int plan(size_t num, const int64_t *rows, const int64_t *cols, int steps, bool backward,
+         std::vector<Batch> &batches, int64_t &bytes) {
+    bytes = 0;
+    std::vector<size_t> order;
+    order.reserve(num);
+    for (size_t i = 0; i < num; ++i) {
+        if (rows[i] < 0 || cols[i] < 0 || rows[i] > kMaxDim || cols[i] > kMaxDim) return TOA_ESIZE;
+        if (rows[i] && cols[i]) order.push_back(i);
+    }
+    auto key = [&](size_t i) {
+        return std::make_pair(std::min(rows[i], cols[i]), std::max(rows[i], cols[i]));
+    };
+    std::stable_sort(order.begin(), order.end(), [&](size_t i, size_t j) { return key(i) < key(j); });
+    Layout lay{};
+    for (size_t k = 0; k < order.size(); ++k) {
+        const auto shape = key(order[k]);
+        const bool same = k && shape == key(order[k - 1]);
+        if (!same) lay = layoutOf((int)shape.first, (int)shape.second, steps, backward);
+        Batch *b = batches.empty() ? nullptr : &batches.back();
+        if (!b || b->bytes + lay.bytes > kBatchBytes || (int)b->mats.size() == kBatchMats ||
+            (!same && (int)b->shapes.size() == kMaxGroups)) {
+            batches.emplace_back();
+            b = &batches.back();
+        }
+        if (b->shapes.empty() || !same)
+            b->shapes.push_back({(int)shape.first, (int)shape.second, (int)b->mats.size(), 0,
+                                 b->bytes, lay});
+        b->shapes.back().count++;
+        b->mats.push_back(order[k]);
+        b->bytes += lay.bytes;
+    }
+    const int stages = 3 * steps * (backward ? 2 : 1);
+    for (const Batch &b : batches)
+        bytes = std::max(bytes, headOf((int64_t)b.mats.size(), stages).regions + b.bytes);
+    return 0;
+}
+
+// The largest |f| on [0, top] of f(t) = k0 t^n0 + k1 t^(n0+2) + k2 t^(n0+4), n0 = 0 or 1.
+double largest(double k0, double k1, double k2, int n0, double top) {
+    auto at = [&](double t) {
+        const double q = t * t;
+        return std::fabs((k0 + q * (k1 + q * k2)) * (n0 ? t : 1.0));
+    };
+    double best = std::max(at(0.0), at(top));
+    // zeros of the derivative, a quadratic (n0 = 1) or linear (n0 = 0) equation in q = t^2
+    auto consider = [&](double q) {
+        if (q > 0.0 && q < top * top) best = std::max(best, at(std::sqrt(q)));
+    };
+    if (n0) {
+        const double qa = 5.0 * k2, qb = 3.0 * k1, qc = k0;
+        if (qa == 0.0) {
+            if (qb != 0.0) consider(-qc / qb);
+        } else {
+            const double disc = qb * qb - 4.0 * qa * qc;
+            if (disc >= 0.0) {
+                consider((-qb + std::sqrt(disc)) / (2.0 * qa));
+                consider((-qb - std::sqrt(disc)) / (2.0 * qa));
+            }
+        }
+    } else if (k2 != 0.0) {
+        consider(-k1 / (2.0 * k2));
+    }
+    return best;
+}
+
+int checkSeries(const toa_muon_series *q) {
+    if (!q) return TOA_ENULL;
+    if (q->steps < 1 || q->steps > kMaxSteps || !std::isfinite(q->a) || !std::isfinite(q->b) ||
+        !std::isfinite(q->c) || !(q->eps >= 0.0) || !std::isfinite(q->eps))
+        return TOA_EVALUE;
+    return 0;
+}
+
+// Bounds of the iterates from a start of norm 1 (with a hundredth of slack for rounding).
+int boundsOf(const toa_muon_series &q, FactorArgs &f) {
+    f.a = (float)q.a;
+    f.b = (float)q.b;
+    f.c = (float)q.c;
+    f.eps = q.eps;
+    f.steps = q.steps;
+    double x = 1.0, top = 1.0;
+    for (int k = 0; k <= q.steps; ++k) {
+        f.x[k] = 1.01 * x;
+        top = std::max(top, f.x[k]);
+        if (k == q.steps) break;
+        f.d[k] = std::max(1.01 * largest(q.a, 3.0 * q.b, 5.0 * q.c, 0, f.x[k]), 1e-3);
+        x = std::max(largest(q.a, q.b, q.c, 1, f.x[k]), 1e-6);
+        if (!(x <= 1048576.0)) return TOA_EVALUE;
+    }
+    f.rho = std::max(1.01 * largest(q.a, q.b, q.c, 0, top), 1e-3);
+    return 0;
+}
+
+template <typename... Args>
+int launch(void (*kernel)(Args...), int64_t grid, int block, hipStream_t stream, Args... args) {
+    if (grid <= 0) return 0;
+    if (grid > std::numeric_limits<int>::max()) return TOA_ESIZE;
+    void *ptrs[] = {(void *)&args...};
+    return (int)hipLaunchKernel((const void *)kernel, dim3((unsigned)grid), dim3(block), ptrs, 0,
+                                stream);
+}
+
+#define TRY(expr)                   \
+    do {                            \
+        const int rc_ = (expr);     \
+        if (rc_ != 0) return rc_;   \
+    } while (0)
+
+// fn(element type) for a dtype code.
+template <typename F> int withType(int dtype, F fn) {
+    switch (dtype) {
+        case TOA_F32: return fn(float());
+        case TOA_F16: return fn(_Float16());
+        case TOA_BF16: return fn(__bf16());
+        default: return TOA_EDTYPE;
+    }
+}
+
+enum What { kOrthogonalize, kStep, kBackward };
+
+struct Call {
+    What what;
+    int dtype, momentum_dtype;
+    const int64_t *rows, *cols;
+    const toa_muon_view *g, *aux, *out;  // aux: momentum or cotangent
+    float *const *scales;
+    const toa_muon_hyper *hyper;
+    toa_muon_series series;
+    char *ws;
+    hipStream_t stream;
+};
+
+double shapeRate(int adjust, int64_t rows, int64_t cols) {
+    if (adjust == TOA_MUON_ASPECT) return std::sqrt(std::max(1.0, (double)rows / (double)cols));
+    if (adjust == TOA_MUON_RMS) return 0.2 * std::sqrt((double)std::max(rows, cols));
+    return 1.0;
+}
+
+class Run {
+  public:
+    Run(const Call &c, const Batch &b, const FactorArgs &bounds)
+        : c_(c), b_(b), steps_(c.series.steps), back_(c.what == kBackward),
+          stages_(3 * steps_ * (back_ ? 2 : 1)), head_(headOf((int64_t)b.mats.size(), stages_)),
+          f_(bounds) {}
+
+    int go() {
+        TRY(fill());
+        TRY(sums());
+        TRY(factors());
+        TRY(pack(back_ ? 0 : -1));
+        for (int k = 0; k < steps_; ++k) TRY(forwardStep(k));
+        if (!back_) return 0;
+        for (int k = steps_ - 1; k >= 0; --k) TRY(backwardStep(k));
+        return tail();
+    }
+
+  private:
+    // whether step k's operands carry 22 bits (see the header)
+    bool split(int k) const { return back_ || c_.dtype != TOA_BF16 || k < steps_ - 2; }
+
+    const MatRec *recs() const { return (const MatRec *)(c_.ws + head_.recs); }
+
+    int fill() {
+        for (size_t from = 0; from < b_.mats.size(); from += kFill) {
+            FillArgs a{};
+            const int n = (int)std::min<size_t>(kFill, b_.mats.size() - from);
+            for (int k = 0; k < n; ++k) {
+                const size_t i = b_.mats[from + k];
+                const bool turned = c_.rows[i] > c_.cols[i];
+                MatRec &r = a.r[k];
+                auto put = [&](const toa_muon_view &v, int64_t &rs, int64_t &cs) {
+                    rs = turned ? v.col_stride : v.row_stride;
+                    cs = turned ? v.row_stride : v.col_stride;
+                    return v.data;
+                };
+                r.g = put(c_.g[i], r.g_rs, r.g_cs);
+                r.out = put(c_.out[i], r.out_rs, r.out_cs);
+                if (c_.aux) r.aux = put(c_.aux[i], r.aux_rs, r.aux_cs);
+                r.scales = c_.scales ? c_.scales[i] : nullptr;
+                r.rate = 1.f;
+                if (c_.hyper) {
+                    const double rate = shapeRate(c_.hyper->adjust, c_.rows[i], c_.cols[i]);
+                    r.rate = (float)(c_.hyper->apply ? c_.hyper->lr * rate : rate);
+                    r.keep = (float)(1.0 - c_.hyper->lr * c_.hyper->weight_decay);
+                }
+            }
+            TRY(launch(fill_kernel, 1, 64, c_.stream, a, (MatRec *)(c_.ws + head_.recs) + from, n));
+        }
+        return 0;
+    }
+
+    // Shapes of a launch with tilesOf(shape) workgroups for each matrix.
+    template <typename F> int64_t shapes(Shapes &sh, F tilesOf) const {
+        int64_t at = 0;
+        sh.n = (int)b_.shapes.size();
+        for (int k = 0; k < sh.n; ++k) {
+            const auto &s = b_.shapes[k];
+            const int64_t tiles = tilesOf(s, k);
+            sh.g[k] = {head_.regions + s.base, s.lay.bytes, s.s, s.w, s.mat0, (int)at, (int)tiles};
+            at += tiles * s.count;
+            if (at > std::numeric_limits<int>::max()) return at;
+        }
+        return at;
+    }
+
+    int sums() {
+        SumArgs a{};
+        a.recs = recs();
+        a.parts = (double *)(c_.ws + head_.parts);
+        if (c_.hyper) {
+            a.momentum = (float)c_.hyper->momentum;
+            a.momentum64 = c_.hyper->momentum;
+            a.sign = c_.hyper->maximize ? -1.f : 1.f;
+            a.nesterov = c_.hyper->nesterov;
+        }
+        const int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int k) {
+            const int64_t n = (int64_t)s.s * s.w;
+            int64_t per = std::max<int64_t>(8192, (n + kMaxParts - 1) / kMaxParts);
+            per = (per + 2047) / 2048 * 2048;
+            a.per[k] = per;
+            f_.nparts[k] = (int)((n + per - 1) / per);
+            f_.mat_end[k] = s.mat0 + s.count;
+            return (int64_t)f_.nparts[k];
+        });
+        f_.ngroups = a.sh.n;
+        return withType(c_.dtype, [&](auto t) {
+            using T = decltype(t);
+            if (c_.what != kStep) {
+                TRY(launch(sum_kernel<T, kSumG>, grid, 256, c_.stream, a));
+                if (!back_) return 0;
+                a.parts = (double *)(c_.ws + head_.parts_y);
+                return launch(sum_kernel<T, kSumAux>, grid, 256, c_.stream, a);
+            }
+            return launch(c_.momentum_dtype == TOA_I8      ? sum_kernel<T, kMomentumI8>
+                          : c_.momentum_dtype == c_.dtype ? sum_kernel<T, kMomentum>
+                                                           : sum_kernel<T, kMomentumF32>,
+                          grid, 256, c_.stream, a);
+        });
+    }
+
+    int factors() {
+        f_.parts = (const double *)(c_.ws + head_.parts);
+        f_.parts_y = back_ ? (const double *)(c_.ws + head_.parts_y) : nullptr;
+        f_.norms = (MatNorm *)(c_.ws + head_.norms);
+        f_.factors = (Factor *)(c_.ws + head_.factors);
+        f_.stages = stages_;
+        return launch(factors_kernel, (int64_t)b_.mats.size(), 256, c_.stream, f_);
+    }
+
+    int pack(int y) {
+        PackArgs a{};
+        a.recs = recs();
+        a.norms = (const MatNorm *)(c_.ws + head_.norms);
+        a.ws = c_.ws;
+        a.split = split(0);
+        if (c_.hyper) {
+            a.momentum = (float)c_.hyper->momentum;
+            a.sign = c_.hyper->maximize ? -1.f : 1.f;
+            a.nesterov = c_.hyper->nesterov;
+        }
+        const int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int k) {
+            a.off[k] = s.lay.x[0];
+            a.off_t[k] = s.lay.xt[0];
+            return padded(s.s) / 64 * (padded(s.w) / 64);
+        });
+        return withType(c_.dtype, [&](auto t) {
+            using T = decltype(t);
+            if (c_.what == kStep)
+                return launch(c_.momentum_dtype == TOA_I8      ? pack_kernel<T, kPackMI8>
+                              : c_.momentum_dtype == c_.dtype ? pack_kernel<T, kPackM>
+                                                               : pack_kernel<T, kPackMF32>,
+                              grid, 256, c_.stream, a);
+            TRY(launch(pack_kernel<T, kPackG>, grid, 256, c_.stream, a));
+            if (y < 0) return 0;
+            for (int k = 0; k < a.sh.n; ++k) {
+                a.off[k] = b_.shapes[k].lay.y[y];
+                a.off_t[k] = b_.shapes[k].lay.yt[y];
+            }
+            return launch(pack_kernel<T, kPackAux>, grid, 256, c_.stream, a);
+        });
+    }
+
+    // One launch of the product for every matrix of the batch.
+    template <typename F>
+    int product(int stage, int k, bool split_out, bool symmetric, int mode, F operands) {
+        GemmArgs a{};
+        a.ws = c_.ws;
+        a.recs = recs();
+        a.factors = (const Factor *)(c_.ws + head_.factors);
+        a.stages = stages_;
+        a.stage = stage;
+        a.symmetric = symmetric;
+        a.mode = mode;
+        a.split_out = split_out;
+        const bool sp = split(k);
+        constexpr int BM = 64, BN = 64;
+        const int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int g) {
+            Product &p = a.p[g];
+            p.e = p.d = p.dt = -1;
+            p.rows = s.s;
+            const int ld_s = (int)rowBytes(padded(s.s), sp), ld_w = (int)rowBytes(padded(s.w), sp);
+            operands(p, s.lay, ld_s, ld_w);
+            p.cols = symmetric ? s.s : s.w;
+            p.lde = symmetric ? ld_s : ld_w;
+            p.ldd = mode == kToFloat ? (int)padded(s.w) * 4
+                                     : (int)rowBytes(padded(symmetric ? s.s : s.w), split_out);
+            p.lddt = (int)rowBytes(padded(s.s), split_out);
+            p.steps0 = p.lda0 / kPiece;
+            p.steps1 = p.lda1 / kPiece;
+            const int64_t tm = (p.rows + BM - 1) / BM, tn = (p.cols + BN - 1) / BN;
+            return symmetric ? tm * (tm + 1) / 2 : tm * tn;
+        });
+        const bool tensor = mode == kToTensor || mode == kToParam;
+        return withType(tensor ? c_.dtype : TOA_F32, [&](auto t) {
+            using T = decltype(t);
+            return launch(sp ? gemm_kernel<T, BM, BN, 2, 2, true> : gemm_kernel<T, BM, BN, 2, 2, false>,
+                          grid, 256, c_.stream, a);
+        });
+    }
+
+    int forwardStep(int k) {
+        const bool sp = split(k), last = k + 1 == steps_;
+        TRY(product(3 * k, k, sp, true, kToOperand, [&](Product &p, const Layout &l, int, int ld_w) {
+            p.a0 = p.b0 = l.x[k];
+            p.lda0 = p.ldb0 = ld_w;
+            p.d = p.dt = l.s[k];
+        }));
+        TRY(product(3 * k + 1, k, sp, true, kToOperand, [&](Product &p, const Layout &l, int ld_s, int) {
+            p.a0 = p.b0 = p.e = l.s[k];
+            p.lda0 = p.ldb0 = ld_s;
+            p.d = p.dt = l.p[k];
+        }));
+        if (last && back_) return 0;  // the result itself is not needed
+        const int mode = !last ? kToOperand : c_.hyper && c_.hyper->apply ? kToParam : kToTensor;
+        return product(3 * k + 2, k, last || split(k + 1), false, mode,
+                       [&](Product &p, const Layout &l, int ld_s, int) {
+                           p.a0 = l.p[k];
+                           p.b0 = l.xt[k];
+                           p.lda0 = p.ldb0 = ld_s;
+                           p.e = l.x[k];
+                           if (!last) {
+                               p.d = l.x[k + 1];
+                               p.dt = l.xt[k + 1];
+                           }
+                       });
+    }
+
+    int backwardStep(int k) {
+        const int from = (steps_ - 1 - k) & 1, stage = 3 * steps_ + 3 * k;
+        TRY(product(stage, k, true, true, kToOperand, [&](Product &p, const Layout &l, int, int ld_w) {
+            p.a0 = p.b1 = l.y[from];
+            p.b0 = p.a1 = l.x[k];
+            p.lda0 = p.ldb0 = p.lda1 = p.ldb1 = ld_w;
+            p.d = p.dt = l.m;
+        }));
+        TRY(product(stage + 1, k, true, true, kToOperand, [&](Product &p, const Layout &l, int ld_s, int) {
+            p.a0 = p.b1 = p.e = l.m;
+            p.b0 = p.a1 = l.s[k];
+            p.lda0 = p.ldb0 = p.lda1 = p.ldb1 = ld_s;
+            p.d = p.dt = l.n;
+        }));
+        return product(stage + 2, k, true, false, k ? kToOperand : kToFloat,
+                       [&](Product &p, const Layout &l, int ld_s, int) {
+                           p.a0 = l.p[k];
+                           p.b0 = l.yt[from];
+                           p.a1 = l.n;
+                           p.b1 = l.xt[k];
+                           p.lda0 = p.ldb0 = p.lda1 = p.ldb1 = ld_s;
+                           p.e = l.y[from];
+                           p.d = k ? l.y[from ^ 1] : l.yf;
+                           if (k) p.dt = l.yt[from ^ 1];
+                       });
+    }
+
+    int tail() {
+        TailArgs a{};
+        a.recs = recs();
+        a.norms = (const MatNorm *)(c_.ws + head_.norms);
+        a.ws = c_.ws;
+        a.parts = (double *)(c_.ws + head_.parts);
+        a.split = split(0);
+        int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int k) {
+            a.y[k] = s.lay.yf;
+            a.x[k] = s.lay.x[0];
+            int64_t parts = std::min<int64_t>(kMaxParts, ((int64_t)s.s * s.w + 8191) / 8192);
+            a.rows_per[k] = (s.s + parts - 1) / parts;
+            a.nparts[k] = (int)((s.s + a.rows_per[k] - 1) / a.rows_per[k]);
+            return (int64_t)a.nparts[k];
+        });
+        TRY(launch(dot_kernel, grid, 256, c_.stream, a));
+        grid = shapes(a.sh, [&](const Batch::Shape &s, int) {
+            return padded(s.s) / 64 * (padded(s.w) / 64);
+        });
+        return withType(c_.dtype, [&](auto t) {
+            using T = decltype(t);
+            return launch(tail_kernel<T>, grid, 256, c_.stream, a);
+        });
+    }
+
+    const Call &c_;
+    const Batch &b_;
+    const int steps_;
+    const bool back_;
+    const int stages_;
+    const Head head_;
+    FactorArgs f_;
+};
+
+int run(const Call &call, size_t num, const void *workspace, size_t workspace_bytes) {
+    if (call.dtype != TOA_F32 && call.dtype != TOA_F16 && call.dtype != TOA_BF16) return TOA_EDTYPE;
+    FactorArgs bounds{};
+    TRY(boundsOf(call.series, bounds));
+    if (num == 0) return 0;
+    if (!call.rows || !call.cols) return TOA_ENULL;
+    std::vector<Batch> batches;
+    int64_t bytes;
+    TRY(plan(num, call.rows, call.cols, call.series.steps, call.what == kBackward, batches, bytes));
+    if (batches.empty()) return 0;
+    if (!call.g || !call.out || (call.what != kOrthogonalize && !call.aux)) return TOA_ENULL;
+    for (const Batch &b : batches)
+        for (size_t i : b.mats)
+            if (!call.g[i].data || !call.out[i].data || (call.aux && !call.aux[i].data) ||
+                (call.momentum_dtype == TOA_I8 && (!call.scales || !call.scales[i])))
+                return TOA_ENULL;
+    if (!workspace) return TOA_ENULL;
+    if (workspace_bytes < (size_t)bytes || ((uintptr_t)workspace & 255)) return TOA_EWORKSPACE;
+    // (every launch of every batch is checked against the grid's limits before the first goes out)
+    for (const Batch &b : batches)
+        for (const auto &s : b.shapes)
+            if (padded(s.s) / 64 * (padded(s.w) / 64) * (int64_t)b.mats.size() >
+                std::numeric_limits<int>::max())
+                return TOA_ESIZE;
+    for (const Batch &b : batches) TRY(Run(call, b, bounds).go());
+    return 0;
+}
+
+size_t workspaceOf(int dtype, size_t num, const int64_t *rows, const int64_t *cols, int steps,
+                   bool backward, int *status) {
+    int rc = 0;
+    int64_t bytes = 0;
+    try {
+        std::vector<Batch> batches;
+        rc = dtype != TOA_F32 && dtype != TOA_F16 && dtype != TOA_BF16 ? TOA_EDTYPE
+             : steps < 1 || steps > kMaxSteps                        ? TOA_EVALUE
+             : num && (!rows || !cols)                               ? TOA_ENULL
+                                       : plan(num, rows, cols, steps, backward, batches, bytes);
+    } catch (...) {
+        rc = (int)hipErrorOutOfMemory;
+    }
+    if (status) *status = rc;
+    return rc ? 0 : (size_t)bytes;
+}
+
+// Launches over lists of flat arrays, 64 to a launch.
+template <typename F>
+int blocks(size_t num, const void *const *in, void *const *out, const float *const *scales,
+           const size_t *n, F kernel, hipStream_t stream) {
+    if (num == 0) return 0;
+    if (!n) return TOA_ENULL;
+    for (size_t i = 0; i < num; ++i) {
+        if (!n[i]) continue;
+        if (!in || !out || !scales || !in[i] || !out[i] || !scales[i]) return TOA_ENULL;
+        if ((n[i] + 2047) / 2048 > (size_t)std::numeric_limits<int>::max() / 2) return TOA_ESIZE;
+    }
+    BlocksArgs a{};
+    int64_t tiles = 0;
+    for (size_t i = 0; i <= num; ++i) {
+        const int64_t more = i < num ? (int64_t)((n[i] + 2047) / 2048) : 0;
+        if (a.n && (i == num || a.n == kListMax || tiles + more > std::numeric_limits<int>::max())) {
+            TRY(launch(kernel, tiles, 256, stream, a));
+            a.n = 0;
+            tiles = 0;
+        }
+        if (!more) continue;
+        a.in[a.n] = in[i];
+        a.out[a.n] = out[i];
+        a.scales[a.n] = const_cast<float *>(scales[i]);
+        a.count[a.n] = n[i];
+        a.tile0[a.n] = (unsigned)tiles;
+        tiles += more;
+        ++a.n;
+    }
+    return 0;
+}
+
+// Nothing thrown in here may cross the C boundary.
+template <typename F> int guarded(F fn) {
+    try {
+        return fn();
+    } catch (...) {
+        return (int)hipErrorOutOfMemory;
+    }
+}
+
+}  // namespace
+
+extern "C" {
+
+int toa_muon_abi_version(void) { return 1; }
+
+const char *toa_muon_error_string(int code) {
+    switch (code) {
+        case 0: return "success";
+        case TOA_EDTYPE: return "toa_muon: unsupported dtype (float32, float16 and bfloat16 are served)";
+        case TOA_ENULL: return "toa_muon: a required pointer is NULL";
+        case TOA_ESIZE: return "toa_muon: a matrix is too large (a side beyond 2^20, or too many tiles)";
+        case TOA_EVALUE: return "toa_muon: a number is out of range (steps, coefficients, eps, or a "
+                                "hyper-parameter)";
+        case TOA_EWORKSPACE: return "toa_muon: workspace too small or not 256-byte aligned";
+        default: return code > 0 ? hipGetErrorString((hipError_t)code) : "toa_muon: unknown error";
+    }
+}
+
+size_t toa_muon_orthogonalize_workspace(int dtype, size_t num, const int64_t *rows,
+                                        const int64_t *cols, int steps, int *status) {
+    return workspaceOf(dtype, num, rows, cols, steps, false, status);
+}
+
+size_t toa_muon_backward_workspace(int dtype, size_t num, const int64_t *rows, const int64_t *cols,
+                                   int steps, int *status) {
+    return workspaceOf(dtype, num, rows, cols, steps, true, status);
+}
+
+int toa_muon_orthogonalize_multi(int dtype, size_t num, const int64_t *rows, const int64_t *cols,
+                                 const toa_muon_view *in, const toa_muon_view *out,
+                                 const toa_muon_series *series, void *workspace,
+                                 size_t workspace_bytes, void *stream) {
+    return guarded([&]() -> int {
+        TRY(checkSeries(series));
+        const Call c{kOrthogonalize, dtype, dtype, rows, cols, in, nullptr, out, nullptr, nullptr,
+                     *series, (char *)workspace, (hipStream_t)stream};
+        return run(c, num, workspace, workspace_bytes);
+    });
+}
+
+int toa_muon_orthogonalize_backward_multi(int dtype, size_t num, const int64_t *rows,
+                                          const int64_t *cols, const toa_muon_view *in,
+                                          const toa_muon_view *grad_out,
+                                          const toa_muon_view *grad_in,
+                                          const toa_muon_series *series, void *workspace,
+                                          size_t workspace_bytes, void *stream) {
+    return guarded([&]() -> int {
+        TRY(checkSeries(series));
+        const Call c{kBackward, dtype, dtype, rows, cols, in, grad_out, grad_in, nullptr, nullptr,
+                     *series, (char *)workspace, (hipStream_t)stream};
+        return run(c, num, workspace, workspace_bytes);
+    });
+}
+
+int toa_muon_step_multi(int dtype, int momentum_dtype, size_t num, const int64_t *rows,
+                        const int64_t *cols, const toa_muon_view *out, const toa_muon_view *grads,
+                        const toa_muon_view *momentum, float *const *scales,
+                        const toa_muon_hyper *hyper, const toa_muon_series *series,
+                        void *workspace, size_t workspace_bytes, void *stream) {
+    return guarded([&]() -> int {
+        TRY(checkSeries(series));
+        if (!hyper) return TOA_ENULL;
+        if (momentum_dtype != dtype && momentum_dtype != TOA_F32 && momentum_dtype != TOA_I8)
+            return TOA_EDTYPE;
+        if (!(hyper->momentum >= 0.0 && hyper->momentum < 1.0) ||
+            hyper->adjust < TOA_MUON_UNIT || hyper->adjust > TOA_MUON_RMS ||
+            (hyper->apply && !(std::isfinite(hyper->lr) && std::isfinite(hyper->weight_decay))))
+            return TOA_EVALUE;
+        const Call c{kStep, dtype, momentum_dtype, rows, cols, grads, momentum, out, scales, hyper,
+                     *series, (char *)workspace, (hipStream_t)stream};
+        return run(c, num, workspace, workspace_bytes);
+    });
+}
+
+int toa_muon_quantize_multi(int dtype, size_t num, const void *const *in, const size_t *n,
+                            int8_t *const *codes, float *const *scales, void *stream) {
+    return guarded([&]() -> int {
+        return withType(dtype, [&](auto t) {
+            return blocks(num, in, (void *const *)codes, (const float *const *)scales, n,
+                          quantize_kernel<decltype(t)>, (hipStream_t)stream);
+        });
+    });
+}
+
+int toa_muon_dequantize_multi(int dtype, size_t num, const int8_t *const *codes,
+                              const float *const *scales, const size_t *n, void *const *out,
+                              void *stream) {
+    return guarded([&]() -> int {
+        return withType(dtype, [&](auto t) {
+            return blocks(num, (const void *const *)codes, out, scales, n,
+                          dequantize_kernel<decltype(t)>, (hipStream_t)stream);
+        });
+    });
+}
+
+}  // extern "C"
