@@ -1,15 +1,18 @@
 // Device code of libtoa_muon.so: see include/toa_muon.h for what the operators compute.
 //
 // Every matrix is worked on in its wide orientation (s rows, w columns, s <= w; a tall one is
-// read and written turned).  Per step k of the series, with X = X_k:
-//     S = X X^T            (s x s, symmetric: lower tiles only, mirrored when stored)
-//     P = b S + c S S      (symmetric too)
-//     X' = a X + P X
-// and for the gradient, with the cotangent Y of X' (all from the formulas, S and P symmetric):
-//     M = Y X^T + X Y^T,   N = b M + c (M S + S M),   Y_prev = a Y + P Y + N X.
+// read and written turned).  Per step k of the series, with X = X_k, completing the square:
+//     S = X X^T + h I,               h = b / 2c          (symmetric: lower tiles only, mirrored)
+//     P = c S S + (a - b h / 2) I                        (symmetric too)
+//     X' = P X                       = a X + b (X X^T) X + c (X X^T)^2 X
+// and for the gradient, with the cotangent Y of X':
+//     M = Y X^T + X Y^T,   N = c (M S + S M),   Y_prev = P Y + N X.
 // All of them are sums of products A B^T of row-major operands, so ONE kernel computes them: a
-// tile of up to two products with a common sum, plus a multiple of a third matrix, stored in both
-// orientations (X and X^T; for the symmetric ones the mirror image).
+// tile of up to two products with a common sum, plus a multiple of the unit matrix, stored in both
+// orientations (X and X^T; for the symmetric ones the mirror image).  No stage reads a third
+// matrix; measured, the read of one at a tile's end cost as much as 15 % of its products.
+// (Where c is zero or tiny beside b: S = X X^T, P = c S S + b S + a I, N = c (M S + S M) + b M, with
+// that third matrix.)
 //
 // Operands.  The matrix cores multiply halves; an operand element is kept as hi + lo, two halves
 // that together carry 22 bits, and a product is hi hi + hi lo + lo hi with float32 sums (what is
@@ -283,17 +286,19 @@ __global__ __launch_bounds__(256) void sum_kernel(SumArgs a) {
 // ---- scales and factors ----------------------------------------------------------------------
 
 struct Factor {
-    float acc, add, turn, pad;  // result = acc * sum + add * E; turn: the sum between the products
+    float acc, add, turn, diag;  // result = acc * sum + add * E + diag * I;
+                                 // turn: the sum is multiplied with it between the products
 };
 
 struct FactorArgs {
     const double *parts, *parts_y;  // parts_y: of the cotangent, or null
     MatNorm *norms;
     Factor *factors;                // [matrix][stages]
-    int steps, stages, nparts_pad;
+    int steps, stages, square;      // square: S carries h
     float a, b, c;
-    double eps, rho;                // rho: max |p(t) / t| over every interval
+    double eps, h;
     double x[kMaxSteps + 1];        // bound of |X_k| from a start of norm 1
+    double r[kMaxSteps];            // bound of |p(t) / t| on [0, x_k], which is |P|'s
     double d[kMaxSteps];            // bound of |p'| on [0, x_k]
     int nparts[kMaxGroups], mat_end[kMaxGroups], ngroups;
 };
@@ -321,9 +326,9 @@ __global__ __launch_bounds__(256) void factors_kernel(FactorArgs a) {
     const double ysize =
         a.parts_y ? sqrt(blockSum(t < np ? a.parts_y[(int64_t)mat * kMaxParts + t] : 0.0, lds)) : 0.0;
     const double s0 = startOf(size, a.eps), plus = size + a.eps;
-    auto bound = [&](int i) {
+    auto bound = [&](int i) {  // of |X_i|
         double grown = s0;
-        for (int j = 0; j < i; ++j) grown *= a.rho;
+        for (int j = 0; j < i; ++j) grown *= a.r[j];
         return grown < a.x[i] ? grown : a.x[i];
     };
     auto ybound = [&](int i) {  // of the cotangent of X_i
@@ -340,22 +345,25 @@ __global__ __launch_bounds__(256) void factors_kernel(FactorArgs a) {
         a.norms[mat] = n;
     }
     if (t >= a.steps) return;
-    const double x = bound(t), ab = fabs((double)a.b), ac = fabs((double)a.c);
-    const int ex = expOf(x), es = expOf(x * x), ep = expOf(ab * x * x + ac * x * x * x * x);
+    const double x = bound(t), x2 = x * x, ab = fabs((double)a.b), ac = fabs((double)a.c);
+    const double sbound = a.square ? fmax(fabs(a.h), fabs(a.h + x2)) : x2;
+    const int ex = expOf(x), es = expOf(sbound), ep = expOf(a.r[t]);
     const bool last = t + 1 == a.steps;
     const int ex1 = last && !a.parts_y ? 0 : expOf(bound(t + 1));
+    const float add = a.square ? 0.f : a.b;
+    const double unit = a.square ? (double)a.a - (double)a.b * a.h * 0.5 : (double)a.a;
     Factor *f = a.factors + (int64_t)mat * a.stages + 3 * t;
-    f[0] = {ldexpf(1.f, es - 2 * ex), 0.f, 1.f, 0.f};
-    f[1] = {ldexpf(a.c, ep - 2 * es), ldexpf(a.b, ep - es), 1.f, 0.f};
-    f[2] = {ldexpf(1.f, ex1 - ep - ex), ldexpf(a.a, ex1 - ex), 1.f, 0.f};
+    f[0] = {ldexpf(1.f, es - 2 * ex), 0.f, 1.f, (float)(a.square ? ldexp(a.h, es) : 0.0)};
+    f[1] = {ldexpf(a.c, ep - 2 * es), ldexpf(add, ep - es), 1.f, (float)ldexp(unit, ep)};
+    f[2] = {ldexpf(1.f, ex1 - ep - ex), 0.f, 1.f, 0.f};
     if (!a.parts_y) return;
     const double y1 = ybound(t + 1);
     const int ey1 = expOf(y1), ey = t ? expOf(ybound(t)) : 0;
-    const int em = expOf(2.0 * x * y1), en = expOf((ab + 2.0 * ac * x * x) * 2.0 * x * y1);
+    const int em = expOf(2.0 * x * y1), en = expOf((ab + 2.0 * ac * x2) * 2.0 * x * y1);
     f = a.factors + (int64_t)mat * a.stages + 3 * a.steps + 3 * t;
     f[0] = {ldexpf(1.f, em - ey1 - ex), 0.f, 1.f, 0.f};
-    f[1] = {ldexpf(a.c, en - em - es), ldexpf(a.b, en - em), 1.f, 0.f};
-    f[2] = {ldexpf(1.f, ey - en - ex), ldexpf(a.a, ey - ey1), ldexpf(1.f, (en + ex) - (ep + ey1)), 0.f};
+    f[1] = {ldexpf(a.c, en - em - es), ldexpf(add, en - em), 1.f, 0.f};
+    f[2] = {ldexpf(1.f, ey - en - ex), 0.f, ldexpf(1.f, (en + ex) - (ep + ey1)), 0.f};
 }
 
 // ---- operands ----------------------------------------------------------------------------------
@@ -475,7 +483,8 @@ struct Product {             // one matrix's operands, as byte offsets into its 
     int64_t a0, b0, a1, b1;  // rows of A and of B: sum over both pairs of A B^T
     int64_t e;               // the third matrix (same shape as the result), or -1
     int64_t d, dt;           // the result and its transpose, or -1
-    int lda0, ldb0, lda1, ldb1, lde, ldd, lddt;
+    int lda, ldb;            // bytes of a row, the same for both pairs
+    int lde, ldd, lddt;
     int steps0, steps1;      // pieces of 128 bytes along each pair's rows
     int rows, cols;
 };
@@ -484,7 +493,7 @@ struct GemmArgs {
     char *ws;
     const MatRec *recs;
     const Factor *factors;
-    int stages, stage, symmetric, mode, split_out, tiles_total;
+    int stages, stage, symmetric, mode, split_out;
     Shapes sh;
     Product p[kMaxGroups];
 };
@@ -506,19 +515,50 @@ __device__ inline void tileOf(int t, int across, bool symmetric, int &ti, int &t
     }
 }
 
-// Tile BM x BN by WM x WN waves.  LDS holds one 128-byte piece of every row of both operands; 16
-// byte chunks of a row are permuted (chunk ^ row % 8) so that the 16-byte reads of a wave, which
-// go down the rows, spread over the banks.
-template <typename T, int BM, int BN, int WM, int WN, bool SPLIT>
-__global__ __launch_bounds__(WM *WN * 64) void gemm_kernel(GemmArgs a) {
-    constexpr int NT = WM * WN * 64;
+// Consecutive tiles go to one XCD (workgroups are dealt to the eight in turn), so that the tiles of
+// a matrix share an L2.
+__device__ inline int tileForWorkgroup(int b, int total) {
+    const int xcd = b & 7, q = total >> 3, r = total & 7;
+    return xcd * q + (xcd < r ? xcd : r) + (b >> 3);
+}
+
+// 16 bytes for each lane from global memory straight into LDS: the wave's 1 KiB from `lds` on.
+__device__ inline void loadToLds(const char *src, char *lds) {
+    __builtin_amdgcn_global_load_lds((const __attribute__((address_space(1))) void *)src,
+                                     (__attribute__((address_space(3))) void *)lds, 16, 0, 0);
+}
+
+// All but the wave's newest N loads have arrived, and (BARRIER) so have everybody else's.
+template <int N, bool BARRIER = true> __device__ inline void arrive() {
+    if (BARRIER)
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"n"(N) : "memory");
+    else
+        asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
+}
+
+// Tile BM x BN by WM x WN waves.  A stage of LDS holds one 128-byte piece of every row of both
+// operands; STAGES of them are in flight, filled by loads that bypass the registers.  The 16-byte
+// chunks of a row are permuted (chunk ^ row / 2 % 8): sixteen lanes of a 16-byte read, which go down
+// the rows, then touch each of the 64 banks once.
+//
+// KS > 1 (one wave to a tile) splits the sum instead: each of KS waves takes every KS-th piece
+// through stages of its own, without a barrier, and the partial sums are added through LDS, always
+// in the same order.
+template <typename T, int BM, int BN, int WM, int WN, int KS, int STAGES, bool SPLIT>
+__global__ __launch_bounds__(WM *WN *KS * 64) void gemm_kernel(GemmArgs a) {
+    constexpr int NW = WM * WN;                          // waves that share a stage
     constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 results per wave
+    constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;    // loads of 8 rows, per wave and stage
     constexpr int kStage = (BM + BN) * kPiece;
     constexpr int kScratch = 32 * 36 * 4;                // per wave, for the stores
-    constexpr int kLds = kStage > WM * WN * kScratch ? kStage : WM * WN * kScratch;
-    __shared__ __attribute__((aligned(16))) char lds[kLds];
+    constexpr bool kShared = NW > 1;
+    constexpr int kLds = STAGES * kStage * KS > NW * KS * kScratch ? STAGES * kStage * KS
+                                                                   : NW * KS * kScratch;
+    static_assert(KS == 1 || (NW == 1 && TM * TN == KS), "one block of the sum for each wave");
+    static_assert((NW == 1 || NW % 2 == 0) && BM % 32 == 0, "the permutation of a load's rows");
+    __shared__ __attribute__((aligned(16))) char lds_[kLds];
 
-    int t = blockIdx.x, mat;
+    int t = tileForWorkgroup(blockIdx.x, gridDim.x), mat;
     const int gi = findGroup(a.sh, t, mat);
     const Product &p = a.p[gi];
     char *region = a.ws + a.sh.g[gi].base + mat * a.sh.g[gi].stride;
@@ -526,7 +566,10 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_kernel(GemmArgs a) {
     int ti, tj;
     tileOf(t, (p.cols + BN - 1) / BN, a.symmetric, ti, tj);
     const int i0 = ti * BM, j0 = tj * BN;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63;
+    const int whole = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int wave = KS > 1 ? 0 : whole, part = KS > 1 ? whole : 0;
+    char *const lds = lds_ + part * STAGES * kStage;
     const int wi = wave / WN * (BM / WM), wj = wave % WN * (BN / WN);
     const Factor f = a.factors[(int64_t)mat * a.stages + a.stage];
 
@@ -538,124 +581,272 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_kernel(GemmArgs a) {
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
 
-    for (int pair = 0; pair < 2; ++pair) {
-        const int steps = pair ? p.steps1 : p.steps0;
-        if (pair && steps) {
+    // Where a lane's chunks come from, relative to the tile's first row (a row of both pairs has
+    // the same length).  Rows beyond the matrix repeat its last one; what comes of them is not
+    // stored.
+    auto chunk = [&](int group) { return ((lane & 7) ^ ((group & 1) * 4 + (lane >> 4))) << 4; };
+    unsigned from_a[LA], from_b[LB];
 #pragma unroll
-            for (int i = 0; i < TM; ++i)
+    for (int q = 0; q < LA; ++q) {
+        const int row = (q * NW + wave) * 8 + (lane >> 3);
+        from_a[q] = (unsigned)(i0 + row < p.rows ? row : p.rows - 1 - i0) * (unsigned)p.lda +
+                    chunk(q * NW + wave);
+    }
 #pragma unroll
-                for (int j = 0; j < TN; ++j) acc[i][j] *= f.turn;
+    for (int q = 0; q < LB; ++q) {
+        const int row = (q * NW + wave) * 8 + (lane >> 3);
+        from_b[q] = (unsigned)(j0 + row < p.cols ? row : p.cols - 1 - j0) * (unsigned)p.ldb +
+                    chunk(q * NW + wave);
+    }
+    const char *const a0 = region + p.a0 + (int64_t)i0 * p.lda;
+    const char *const b0 = region + p.b0 + (int64_t)j0 * p.ldb;
+    const char *const a1 = region + p.a1 + (int64_t)i0 * p.lda;
+    const char *const b1 = region + p.b1 + (int64_t)j0 * p.ldb;
+    // piece number k of this wave is number part + KS k of the tile
+    const int steps0 = p.steps0, all = p.steps0 + p.steps1;
+    const int steps = (all - part + KS - 1) / KS;
+    const char *A, *B;  // the piece that is being loaded
+    auto from_piece = [&](int k) {
+        k = part + KS * k;
+        const bool second = k >= steps0;
+        const int64_t at = (int64_t)(second ? k - steps0 : k) * kPiece;
+        A = (second ? a1 : a0) + at;
+        B = (second ? b1 : b0) + at;
+    };
+    auto load = [&](int q, int stage) {
+        char *to = lds + stage * kStage;
+        if (q < LA)
+            loadToLds(A + from_a[q < LA ? q : 0], to + (q * NW + wave) * 1024);
+        else
+            loadToLds(B + from_b[q < LA ? 0 : q - LA], to + BM * kPiece + ((q - LA) * NW + wave) * 1024);
+    };
+    // Phases of TM * TN matrix instructions.  The registers of a phase are read from LDS during the
+    // one before.  Before a step's last phase everybody has read the stage and the next one is
+    // waited for; the last phase's instructions cover the first reads from that one, and the loads
+    // that refill the stage go out in the last phase and the kShares - 1 that follow it.
+    constexpr int kShares = SPLIT ? 3 : 2, L = LA + LB, kFirst = (L + kShares - 1) / kShares;
+    half8 ah[2][TM], bh[2][TN], al[SPLIT ? TM : 1], bl[SPLIT ? TN : 1];
+    auto frag = [&](const char *from, int row, int c) {
+        row += lane & 31;
+        c += lane >> 5;
+        return *(const half8 *)(from + row * kPiece + ((c ^ (row >> 1 & 7)) << 4));
+    };
+    auto read_a = [&](const char *from, half8 *to, int c) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) to[i] = frag(from, wi + 32 * i, c);
+    };
+    auto read_b = [&](const char *from, half8 *to, int c) {
+#pragma unroll
+        for (int j = 0; j < TN; ++j) to[j] = frag(from, BM + wj + 32 * j, c);
+    };
+    auto multiply = [&](const half8 *x, const half8 *y) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] = mfma(x[i], y[j], acc[i][j]);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+
+    // share number `share` of the loads of the piece that `from_piece` chose
+    auto refill = [&](int share, int stage) {
+#pragma unroll
+        for (int q = 0; q < L; ++q)
+            if (q / kFirst == share) load(q, stage);
+    };
+#pragma unroll
+    for (int k = 0; k < STAGES; ++k) {
+        if (k >= steps) break;
+        from_piece(k);
+#pragma unroll
+        for (int share = 0; share < (k == STAGES - 1 ? 1 : kShares); ++share) refill(share, k);
+    }
+    if (steps >= STAGES)
+        arrive<(STAGES - 2) * L + kFirst, kShared>();
+    else
+        arrive<0, kShared>();
+    read_a(lds, ah[0], 0);
+    read_b(lds, bh[0], 0);
+    // before the second pair's first product
+    bool turned_sum = all == steps0;
+    auto turn = [&] {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < TN; ++j) acc[i][j] *= f.turn;
+        turned_sum = true;
+    };
+    int stage = 0;
+    for (int k = 0; k < steps; ++k) {
+        const char *const here = lds + stage * kStage;
+        const int next = stage == STAGES - 1 ? 0 : stage + 1;
+        const int before = stage == 0 ? STAGES - 1 : stage - 1;  // being refilled
+        const bool filling = k + STAGES - 1 < steps;
+        if (!turned_sum && part + KS * k >= steps0) turn();
+        __builtin_amdgcn_sched_barrier(0);
+        if (SPLIT) {
+            read_a(here, al, 4);
+            if (filling) refill(1, before);
+            multiply(ah[0], bh[0]);
+            read_b(here, bl, 4);
+            if (filling) refill(2, before);
+            multiply(al, bh[0]);
+            read_a(here, ah[1], 2);
+            read_b(here, bh[1], 2);
+            multiply(ah[0], bl);
+            read_a(here, al, 6);
+            multiply(ah[1], bh[1]);
+            read_b(here, bl, 6);
+            multiply(al, bh[1]);
+        } else {
+            read_a(here, ah[1], 2);
+            read_b(here, bh[1], 2);
+            if (filling) refill(1, before);
+            multiply(ah[0], bh[0]);
+            read_a(here, ah[0], 4);
+            read_b(here, bh[0], 4);
+            multiply(ah[1], bh[1]);
+            read_a(here, ah[1], 6);
+            read_b(here, bh[1], 6);
+            multiply(ah[0], bh[0]);
         }
-        const char *A = region + (pair ? p.a1 : p.a0), *B = region + (pair ? p.b1 : p.b0);
-        const int64_t lda = pair ? p.lda1 : p.lda0, ldb = pair ? p.ldb1 : p.ldb0;
-        for (int k = 0; k < steps; ++k) {
-            __syncthreads();
-            for (int q = threadIdx.x; q < (BM + BN) * 8; q += NT) {
-                const int row = q >> 3, chunk = q & 7;
-                // rows beyond the matrix repeat its last one; what comes of them is not stored
-                const char *src;
-                if (row < BM) {
-                    const int i = i0 + row < p.rows ? i0 + row : p.rows - 1;
-                    src = A + i * lda;
-                } else {
-                    const int j = j0 + row - BM < p.cols ? j0 + row - BM : p.cols - 1;
-                    src = B + j * ldb;
-                }
-                *(int4 *)(lds + row * kPiece + ((chunk ^ (row & 7)) << 4)) =
-                    *(const int4 *)(src + (int64_t)k * kPiece + (chunk << 4));
-            }
-            __syncthreads();
-            auto frag = [&](int row, int chunk) {
-                row += lane & 31;
-                chunk += lane >> 5;
-                return *(const half8 *)(lds + row * kPiece + ((chunk ^ (row & 7)) << 4));
-            };
-            if (SPLIT) {
+        // (towards the end fewer pieces are in flight: everything is waited for)
+        if (filling)
+            arrive<(STAGES - 2) * L, kShared>();
+        else
+            arrive<0, kShared>();
+        read_a(lds + next * kStage, ah[0], 0);
+        read_b(lds + next * kStage, bh[0], 0);
+        if (k + STAGES < steps) {
+            from_piece(k + STAGES);
+            refill(0, stage);
+        }
+        if (SPLIT)
+            multiply(ah[1], bl);
+        else
+            multiply(ah[1], bh[1]);
+        stage = next;
+    }
+    if (!turned_sum) turn();  // (a wave that had no piece of the second pair)
+    arrive<0>();
+    if (KS > 1) {
+        // each wave adds up one block
+        f32x16 *const sums = (f32x16 *)lds_;
 #pragma unroll
-                for (int slab = 0; slab < 2; ++slab) {
-                    half8 ah[TM], al[TM], bh[TN], bl[TN];
+        for (int b = 0; b < KS; ++b)
+            if (b != whole) sums[(b * KS + whole) * 64 + lane] = acc[b / TN][b % TN];
+        arrive<0>();
+        f32x16 sum;
 #pragma unroll
-                    for (int i = 0; i < TM; ++i) {
-                        ah[i] = frag(wi + 32 * i, 2 * slab);
-                        al[i] = frag(wi + 32 * i, 4 + 2 * slab);
-                    }
+        for (int q = 0; q < 16; ++q) sum[q] = 0.f;
 #pragma unroll
-                    for (int j = 0; j < TN; ++j) {
-                        bh[j] = frag(BM + wj + 32 * j, 2 * slab);
-                        bl[j] = frag(BM + wj + 32 * j, 4 + 2 * slab);
-                    }
+        for (int w = 0; w < KS; ++w) {
+            if (w == whole) {
 #pragma unroll
-                    for (int i = 0; i < TM; ++i)
-#pragma unroll
-                        for (int j = 0; j < TN; ++j) {
-                            acc[i][j] = mfma(al[i], bh[j], acc[i][j]);
-                            acc[i][j] = mfma(ah[i], bl[j], acc[i][j]);
-                            acc[i][j] = mfma(ah[i], bh[j], acc[i][j]);
-                        }
-                }
+                for (int b = 0; b < KS; ++b)
+                    if (b == whole) sum += acc[b / TN][b % TN];
             } else {
-#pragma unroll
-                for (int slab = 0; slab < 4; ++slab) {
-                    half8 ah[TM], bh[TN];
-#pragma unroll
-                    for (int i = 0; i < TM; ++i) ah[i] = frag(wi + 32 * i, 2 * slab);
-#pragma unroll
-                    for (int j = 0; j < TN; ++j) bh[j] = frag(BM + wj + 32 * j, 2 * slab);
-#pragma unroll
-                    for (int i = 0; i < TM; ++i)
-#pragma unroll
-                        for (int j = 0; j < TN; ++j) acc[i][j] = mfma(ah[i], bh[j], acc[i][j]);
-                }
+                sum += sums[(whole * KS + w) * 64 + lane];
             }
         }
+#pragma unroll
+        for (int b = 0; b < KS; ++b)
+            if (b == whole) acc[b / TN][b % TN] = sum;
+        arrive<0>();
     }
 
     // Results leave by 32 x 32 blocks through LDS, eight to a lane: along rows for the result,
     // along columns for its transpose.
-    __syncthreads();
-    float *box = (float *)(lds + wave * kScratch);
+    float *box = (float *)(lds_ + whole * kScratch);
     const MatRec &r = a.recs[mat];
     const bool tensor = a.mode == kToTensor || a.mode == kToParam;
     const bool turned = tensor && r.out_rs < r.out_cs;
+    for (int block = KS > 1 ? whole : 0; block < (KS > 1 ? whole + 1 : TM * TN); ++block) {
+        const int bi = i0 + wi + block / TN * 32, bj = j0 + wj + block % TN * 32;
+        if (bi >= p.rows && !(p.dt >= 0 && bi < padded(p.rows))) continue;
+        if (bj >= p.cols && !(p.d >= 0 && bj < padded(p.cols))) continue;
+        // (registers are picked by number: every block writes its own, the rest is shared code)
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+        for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < TN; ++j) {
-            const int bi = i0 + wi + 32 * i, bj = j0 + wj + 32 * j;
-            if (bi >= p.rows && !(p.dt >= 0 && bi < padded(p.rows))) continue;
-            if (bj >= p.cols && !(p.d >= 0 && bj < padded(p.cols))) continue;
+            for (int j = 0; j < TN; ++j)
+                if (block == i * TN + j)
 #pragma unroll
-            for (int q = 0; q < 16; ++q)
-                box[((q >> 2) * 8 + (lane >> 5) * 4 + (q & 3)) * 36 + (lane & 31)] = acc[i][j][q];
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
+                    for (int q = 0; q < 16; ++q)
+                        box[((q >> 2) * 8 + (lane >> 5) * 4 + (q & 3)) * 36 + (lane & 31)] =
+                            acc[i][j][q];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int row = half * 16 + (lane >> 2), col = (lane & 3) * 8;
-                float v[8], e[8];
+        for (int half = 0; half < 2; ++half) {
+            const int row = half * 16 + (lane >> 2), col = (lane & 3) * 8;
+            float v[8], e[8];
 #pragma unroll
-                for (int q = 0; q < 8; ++q) v[q] = box[row * 36 + col + q] * f.acc;
-                if (p.e >= 0 && bi + row < p.rows && bj + col < p.cols) {
-                    loadOperand(region + p.e + (int64_t)(bi + row) * p.lde, bj + col, e, SPLIT);
+            for (int q = 0; q < 8; ++q) v[q] = box[row * 36 + col + q] * f.acc;
+            if (p.e >= 0 && bi + row < p.rows && bj + col < p.cols) {
+                loadOperand(region + p.e + (int64_t)(bi + row) * p.lde, bj + col, e, SPLIT);
 #pragma unroll
-                    for (int q = 0; q < 8; ++q) v[q] += f.add * e[q];
-                }
+                for (int q = 0; q < 8; ++q) v[q] += f.add * e[q];
+            }
+            if (bi == bj) {
 #pragma unroll
                 for (int q = 0; q < 8; ++q)
-                    if (bi + row >= p.rows || bj + col + q >= p.cols) v[q] = 0.f;
-                if (a.mode == kToOperand) {
-                    if (p.d >= 0 && bi + row < p.rows)
-                        storeOperand(region + p.d + (int64_t)(bi + row) * p.ldd, bj + col, v,
-                                     a.split_out);
-                } else if (a.mode == kToFloat) {
-                    if (bi + row < p.rows && bj + col < p.cols) {
-                        float *o = (float *)(region + p.d + (int64_t)(bi + row) * p.ldd) + bj + col;
-                        store8(o, p.cols - bj - col, v);
+                    if (row == col + q) v[q] += f.diag;
+            }
+#pragma unroll
+            for (int q = 0; q < 8; ++q)
+                if (bi + row >= p.rows || bj + col + q >= p.cols) v[q] = 0.f;
+            if (a.mode == kToOperand) {
+                if (p.d >= 0 && bi + row < p.rows)
+                    storeOperand(region + p.d + (int64_t)(bi + row) * p.ldd, bj + col, v,
+                                 a.split_out);
+            } else if (a.mode == kToFloat) {
+                if (bi + row < p.rows && bj + col < p.cols) {
+                    float *o = (float *)(region + p.d + (int64_t)(bi + row) * p.ldd) + bj + col;
+                    store8(o, p.cols - bj - col, v);
+                }
+            } else if (!turned && bi + row < p.rows && bj + col < p.cols) {
+                T *o = (T *)r.out + (bi + row) * r.out_rs + (bj + col) * r.out_cs;
+                const int valid = p.cols - bj - col;
+                if (r.out_cs == 1) {
+                    if (a.mode == kToParam) {
+                        load8(o, valid, e);
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) v[q] = r.keep * e[q] - r.rate * v[q];
+                    } else {
+#pragma unroll
+                        for (int q = 0; q < 8; ++q) v[q] *= r.rate;
                     }
-                } else if (!turned && bi + row < p.rows && bj + col < p.cols) {
+                    store8(o, valid, v);
+                } else {
+                    for (int q = 0; q < 8 && q < valid; ++q) {
+                        T *x = o + q * r.out_cs;
+                        *x = fromFloat<T>(a.mode == kToParam ? r.keep * toFloat(*x) - r.rate * v[q]
+                                                             : r.rate * v[q]);
+                    }
+                }
+            }
+            if (p.dt >= 0 || turned) {
+#pragma unroll
+                for (int q = 0; q < 8; ++q) box[row * 36 + col + q] = v[q];
+            }
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+        if ((p.dt >= 0 && !(a.symmetric && ti == tj)) || turned) {
+#pragma unroll
+            for (int half = 0; half < 2; ++half) {
+                const int col = half * 16 + (lane >> 2), row = (lane & 3) * 8;
+                if (bj + col >= p.cols) continue;
+                float v[8], e[8];
+#pragma unroll
+                for (int q = 0; q < 8; ++q) v[q] = box[(row + q) * 36 + col];
+                if (a.mode == kToOperand) {
+                    storeOperand(region + p.dt + (int64_t)(bj + col) * p.lddt, bi + row, v,
+                                 a.split_out);
+                } else if (turned && bi + row < p.rows) {
                     T *o = (T *)r.out + (bi + row) * r.out_rs + (bj + col) * r.out_cs;
-                    const int valid = p.cols - bj - col;
-                    if (r.out_cs == 1) {
+                    const int valid = p.rows - bi - row;
+                    if (r.out_rs == 1) {
                         if (a.mode == kToParam) {
                             load8(o, valid, e);
 #pragma unroll
@@ -667,57 +858,18 @@ __global__ __launch_bounds__(WM *WN * 64) void gemm_kernel(GemmArgs a) {
                         store8(o, valid, v);
                     } else {
                         for (int q = 0; q < 8 && q < valid; ++q) {
-                            T *x = o + q * r.out_cs;
-                            *x = fromFloat<T>(a.mode == kToParam ? r.keep * toFloat(*x) - r.rate * v[q]
-                                                                 : r.rate * v[q]);
-                        }
-                    }
-                }
-                if (p.dt >= 0 || turned) {
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) box[row * 36 + col + q] = v[q];
-                }
-            }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
-            if ((p.dt >= 0 && !(a.symmetric && ti == tj)) || turned) {
-#pragma unroll
-                for (int half = 0; half < 2; ++half) {
-                    const int col = half * 16 + (lane >> 2), row = (lane & 3) * 8;
-                    if (bj + col >= p.cols) continue;
-                    float v[8], e[8];
-#pragma unroll
-                    for (int q = 0; q < 8; ++q) v[q] = box[(row + q) * 36 + col];
-                    if (a.mode == kToOperand) {
-                        storeOperand(region + p.dt + (int64_t)(bj + col) * p.lddt, bi + row, v,
-                                     a.split_out);
-                    } else if (turned && bi + row < p.rows) {
-                        T *o = (T *)r.out + (bi + row) * r.out_rs + (bj + col) * r.out_cs;
-                        const int valid = p.rows - bi - row;
-                        if (r.out_rs == 1) {
-                            if (a.mode == kToParam) {
-                                load8(o, valid, e);
-#pragma unroll
-                                for (int q = 0; q < 8; ++q) v[q] = r.keep * e[q] - r.rate * v[q];
-                            } else {
-#pragma unroll
-                                for (int q = 0; q < 8; ++q) v[q] *= r.rate;
-                            }
-                            store8(o, valid, v);
-                        } else {
-                            for (int q = 0; q < 8 && q < valid; ++q) {
-                                T *x = o + q * r.out_rs;
-                                *x = fromFloat<T>(a.mode == kToParam
-                                                      ? r.keep * toFloat(*x) - r.rate * v[q]
-                                                      : r.rate * v[q]);
-                            }
+                            T *x = o + q * r.out_rs;
+                            *x = fromFloat<T>(a.mode == kToParam
+                                                  ? r.keep * toFloat(*x) - r.rate * v[q]
+                                                  : r.rate * v[q]);
                         }
                     }
                 }
             }
-            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-            __builtin_amdgcn_wave_barrier();
         }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
 }
 
 // ---- the end of the gradient: through X_0 = G / (|G| + eps) ------------------------------------

@@ -4,7 +4,6 @@
 // allocates nothing and leaves nothing behind.
 #include <algorithm>
 #include <cmath>
-#include <cstring>
 #include <limits>
 #include <vector>
 
@@ -15,8 +14,10 @@ using namespace toa_muon;
 
 namespace {
 
-// A batch's regions stay below this (one matrix alone may be larger).
-constexpr int64_t kBatchBytes = (int64_t)1 << 30;
+// A batch's regions stay below this (one matrix alone may be larger).  Large batches fill whole
+// rounds of tiles: 96 matrices of 1024^2 take 7.3 ms in one batch, 8.1 in three, 8.9 in eight of a
+// size that stays in the 256 MB of last-level cache.
+constexpr int64_t kBatchBytes = (int64_t)4 << 30;
 constexpr int kBatchMats = 4096;
 constexpr int64_t kMaxDim = (int64_t)1 << 20;
 
@@ -178,11 +179,14 @@ int boundsOf(const toa_muon_series &q, FactorArgs &f) {
         f.x[k] = 1.01 * x;
         top = std::max(top, f.x[k]);
         if (k == q.steps) break;
+        f.r[k] = std::max(1.01 * largest(q.a, q.b, q.c, 0, f.x[k]), 1e-3);
         f.d[k] = std::max(1.01 * largest(q.a, 3.0 * q.b, 5.0 * q.c, 0, f.x[k]), 1e-3);
         x = std::max(largest(q.a, q.b, q.c, 1, f.x[k]), 1e-6);
         if (!(x <= 1048576.0)) return TOA_EVALUE;
     }
-    f.rho = std::max(1.01 * largest(q.a, q.b, q.c, 0, top), 1e-3);
+    // completing the square costs accuracy where h is large beside X X^T (at most x^2)
+    f.h = q.c != 0.0 ? q.b / (2.0 * q.c) : 0.0;
+    f.square = q.c != 0.0 && std::fabs(f.h) <= 4.0 * top * top;
     return 0;
 }
 
@@ -375,7 +379,8 @@ class Run {
         });
     }
 
-    // One launch of the product for every matrix of the batch.
+    // One launch of the product for every matrix of the batch.  `operands` names a matrix's
+    // buffers; steps1 = 1 there says that there is a second pair.
     template <typename F>
     int product(int stage, int k, bool split_out, bool symmetric, int mode, F operands) {
         GemmArgs a{};
@@ -388,41 +393,103 @@ class Run {
         a.mode = mode;
         a.split_out = split_out;
         const bool sp = split(k);
-        constexpr int BM = 64, BN = 64;
-        const int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int g) {
+        for (int g = 0; g < (int)b_.shapes.size(); ++g) {
+            const Batch::Shape &s = b_.shapes[g];
             Product &p = a.p[g];
             p.e = p.d = p.dt = -1;
-            p.rows = s.s;
             const int ld_s = (int)rowBytes(padded(s.s), sp), ld_w = (int)rowBytes(padded(s.w), sp);
             operands(p, s.lay, ld_s, ld_w);
+            p.rows = s.s;
             p.cols = symmetric ? s.s : s.w;
             p.lde = symmetric ? ld_s : ld_w;
             p.ldd = mode == kToFloat ? (int)padded(s.w) * 4
                                      : (int)rowBytes(padded(symmetric ? s.s : s.w), split_out);
             p.lddt = (int)rowBytes(padded(s.s), split_out);
-            p.steps0 = p.lda0 / kPiece;
-            p.steps1 = p.lda1 / kPiece;
-            const int64_t tm = (p.rows + BM - 1) / BM, tn = (p.cols + BN - 1) / BN;
-            return symmetric ? tm * (tm + 1) / 2 : tm * tn;
-        });
+            p.steps0 = p.lda / kPiece;
+            if (p.steps1) p.steps1 = p.steps0;
+        }
         const bool tensor = mode == kToTensor || mode == kToParam;
         return withType(tensor ? c_.dtype : TOA_F32, [&](auto t) {
             using T = decltype(t);
-            return launch(sp ? gemm_kernel<T, BM, BN, 2, 2, true> : gemm_kernel<T, BM, BN, 2, 2, false>,
-                          grid, 256, c_.stream, a);
+            switch (pickTiles(a)) {
+                case kTiles256:
+                    return sp ? tiles<T, 256, 2, 4, 1, 2, true>(a) : tiles<T, 256, 2, 4, 1, 2, false>(a);
+                case kTiles128Pair:
+                    return sp ? tiles<T, 128, 2, 2, 1, 2, true>(a) : tiles<T, 128, 2, 2, 1, 2, false>(a);
+                case kTiles128:
+                    return sp ? tiles<T, 128, 2, 4, 1, 4, true>(a) : tiles<T, 128, 2, 4, 1, 4, false>(a);
+                default:
+                    return sp ? tiles<T, 64, 1, 1, 4, 2, true>(a) : tiles<T, 64, 1, 1, 4, 2, false>(a);
+            }
         });
+    }
+
+    static int64_t tilesOf(const Product &p, bool symmetric, int size) {
+        const int64_t tm = (p.rows + size - 1) / size, tn = (p.cols + size - 1) / size;
+        return symmetric ? tm * (tm + 1) / 2 : tm * tn;
+    }
+
+    enum { kTiles256, kTiles128Pair, kTiles128, kTiles64, kVariants };
+
+    // The variant that finishes first.  A tile's time is its start and stores plus its pieces; it
+    // grows from `alone` to `full` as tiles fill the chip (measured: with the square of the share
+    // filled).  Microseconds from 8 x 512^2, 2..16 x 1024^2, 2048^2 and 4096^2: large tiles get
+    // most out of a full chip (1.4 PFLOP/s of half products in 256 x 256, 0.9 in 64 x 64), small
+    // ones start and end sooner and spread few results over more of it (a product of one 1024^2
+    // matrix: 72 us in 256 x 256, 34 in 128 x 128, 15 in 64 x 64; of sixteen: 115, 145, 220).
+    int pickTiles(const GemmArgs &a) const {
+        struct Variant {
+            int size, at_once;  // tiles that the whole chip holds
+            double alone, alone_piece, full, full_piece;
+        };
+        static const Variant variants[kVariants] = {{256, 256, 18.0, 1.69, 39.0, 2.3},
+                                                    {128, 512, 10.3, 0.70, 26.0, 1.45},
+                                                    {128, 256, 8.3, 0.56, 2.0, 1.03},
+                                                    {64, 256, 7.6, 0.20, 7.6, 0.22}};
+        int best = 0;
+        double least = 0.0;
+        for (int k = 0; k < kVariants; ++k) {
+            const Variant &v = variants[k];
+            double tiles = 0.0, pieces = 0.0;
+            for (int g = 0; g < (int)b_.shapes.size(); ++g) {
+                const double n = (double)tilesOf(a.p[g], a.symmetric, v.size) * b_.shapes[g].count;
+                tiles += n;
+                pieces += n * (a.p[g].steps0 + a.p[g].steps1);
+            }
+            pieces /= tiles;
+            const double alone = v.alone + v.alone_piece * pieces;
+            const double full = std::max(alone, v.full + v.full_piece * pieces);
+            const double rounds = std::floor(tiles / v.at_once), rest = tiles / v.at_once - rounds;
+            const double time =
+                rounds * full + (rest > 0.0 ? alone + (full - alone) * rest * rest : 0.0);
+            if (k == 0 || time < least) {
+                least = time;
+                best = k;
+            }
+        }
+        return best;
+    }
+
+    template <typename T, int B, int WM, int WN, int KS, int STAGES, bool SPLIT>
+    int tiles(GemmArgs &a) {
+        const int64_t grid = shapes(a.sh, [&](const Batch::Shape &, int g) {
+            return tilesOf(a.p[g], a.symmetric, B);
+        });
+        return launch(gemm_kernel<T, B, B, WM, WN, KS, STAGES, SPLIT>, grid, WM * WN * KS * 64,
+                      c_.stream, a);
     }
 
     int forwardStep(int k) {
         const bool sp = split(k), last = k + 1 == steps_;
         TRY(product(3 * k, k, sp, true, kToOperand, [&](Product &p, const Layout &l, int, int ld_w) {
             p.a0 = p.b0 = l.x[k];
-            p.lda0 = p.ldb0 = ld_w;
+            p.lda = p.ldb = ld_w;
             p.d = p.dt = l.s[k];
         }));
         TRY(product(3 * k + 1, k, sp, true, kToOperand, [&](Product &p, const Layout &l, int ld_s, int) {
-            p.a0 = p.b0 = p.e = l.s[k];
-            p.lda0 = p.ldb0 = ld_s;
+            p.a0 = p.b0 = l.s[k];
+            if (!f_.square) p.e = l.s[k];
+            p.lda = p.ldb = ld_s;
             p.d = p.dt = l.p[k];
         }));
         if (last && back_) return 0;  // the result itself is not needed
@@ -431,8 +498,7 @@ class Run {
                        [&](Product &p, const Layout &l, int ld_s, int) {
                            p.a0 = l.p[k];
                            p.b0 = l.xt[k];
-                           p.lda0 = p.ldb0 = ld_s;
-                           p.e = l.x[k];
+                           p.lda = p.ldb = ld_s;
                            if (!last) {
                                p.d = l.x[k + 1];
                                p.dt = l.xt[k + 1];
@@ -445,13 +511,16 @@ class Run {
         TRY(product(stage, k, true, true, kToOperand, [&](Product &p, const Layout &l, int, int ld_w) {
             p.a0 = p.b1 = l.y[from];
             p.b0 = p.a1 = l.x[k];
-            p.lda0 = p.ldb0 = p.lda1 = p.ldb1 = ld_w;
+            p.lda = p.ldb = ld_w;
+            p.steps1 = 1;
             p.d = p.dt = l.m;
         }));
         TRY(product(stage + 1, k, true, true, kToOperand, [&](Product &p, const Layout &l, int ld_s, int) {
-            p.a0 = p.b1 = p.e = l.m;
+            p.a0 = p.b1 = l.m;
+            if (!f_.square) p.e = l.m;
             p.b0 = p.a1 = l.s[k];
-            p.lda0 = p.ldb0 = p.lda1 = p.ldb1 = ld_s;
+            p.lda = p.ldb = ld_s;
+            p.steps1 = 1;
             p.d = p.dt = l.n;
         }));
         return product(stage + 2, k, true, false, k ? kToOperand : kToFloat,
@@ -460,8 +529,8 @@ class Run {
                            p.b0 = l.yt[from];
                            p.a1 = l.n;
                            p.b1 = l.xt[k];
-                           p.lda0 = p.ldb0 = p.lda1 = p.ldb1 = ld_s;
-                           p.e = l.y[from];
+                           p.lda = p.ldb = ld_s;
+            p.steps1 = 1;
                            p.d = k ? l.y[from ^ 1] : l.yf;
                            if (k) p.dt = l.yt[from ^ 1];
                        });
