@@ -30,6 +30,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <type_traits>
+
 namespace toa_muon {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
@@ -51,6 +53,7 @@ struct MatRec {
     float *scales;     // of an 8-bit momentum
     int64_t g_rs, g_cs, aux_rs, aux_cs, out_rs, out_cs;
     float rate, keep;  // out <- keep * out - rate * result (step), or rate * result
+    int s, w;
 };
 
 // Sums over a matrix and what follows from them.
@@ -71,6 +74,14 @@ struct Shapes {
     int n;
     Group g[kMaxGroups];
 };
+
+// The caller's tensors come as addresses in records: without this they would be read and written
+// with instructions that look for LDS behind every address.
+#define TOA_GLOBAL __attribute__((address_space(1)))
+template <typename T> __device__ inline const TOA_GLOBAL T *global(const void *p) {
+    return (const TOA_GLOBAL T *)p;
+}
+template <typename T> __device__ inline TOA_GLOBAL T *global(void *p) { return (TOA_GLOBAL T *)p; }
 
 __device__ inline float toFloat(float v) { return v; }
 __device__ inline float toFloat(_Float16 v) { return (float)v; }
@@ -118,13 +129,17 @@ __global__ void fill_kernel(FillArgs a, MatRec *dst, int n) {
 
 enum { kSumG = 0, kSumAux = 1, kMomentum = 2, kMomentumF32 = 3, kMomentumI8 = 4 };
 
+struct StepArgs {      // what the momentum's update needs
+    double momentum;
+    float sign;
+    int nesterov;
+};
+
 struct SumArgs {
     Shapes sh;
     const MatRec *recs;
     double *parts;     // [matrix][kMaxParts]
-    float momentum, sign;
-    double momentum64;
-    int nesterov;
+    StepArgs step;
     int64_t per[kMaxGroups];  // elements per workgroup, a multiple of 2048
 };
 
@@ -133,13 +148,13 @@ template <typename T> __device__ inline void load8(const T *p, int valid, float 
         typedef T vec __attribute__((ext_vector_type(16 / sizeof(T))));
 #pragma unroll
         for (unsigned q = 0; q < 8 / (16 / sizeof(T)); ++q) {
-            const vec t = ((const vec *)p)[q];
+            const vec t = global<vec>(p)[q];
 #pragma unroll
             for (unsigned i = 0; i < 16 / sizeof(T); ++i) v[q * (16 / sizeof(T)) + i] = toFloat((T)t[i]);
         }
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < valid ? toFloat(p[i]) : 0.f;
+        for (int i = 0; i < 8; ++i) v[i] = i < valid ? toFloat(global<T>(p)[i]) : 0.f;
     }
 }
 
@@ -151,12 +166,12 @@ template <typename T> __device__ inline void store8(T *p, int valid, const float
             vec t;
 #pragma unroll
             for (unsigned i = 0; i < 16 / sizeof(T); ++i) t[i] = fromFloat<T>(v[q * (16 / sizeof(T)) + i]);
-            ((vec *)p)[q] = t;
+            global<vec>(p)[q] = t;
         }
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < valid) p[i] = fromFloat<T>(v[i]);
+            if (i < valid) global<T>(p)[i] = fromFloat<T>(v[i]);
     }
 }
 
@@ -184,27 +199,32 @@ __device__ inline int codeOf(double v, float scale) {
     return (int)(q > 127.0 ? 127.0 : q < -127.0 ? -127.0 : q);
 }
 
+__device__ inline void unpack8(int64_t v, int8_t (&c)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) c[i] = (int8_t)(v >> (8 * i));
+}
+
+__device__ inline int64_t pack8(const int8_t (&c)[8]) {
+    uint64_t v = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v |= (uint64_t)(uint8_t)c[i] << (8 * i);
+    return (int64_t)v;
+}
+
+// A thread's share of the elements from `from` (a multiple of 128) to `to`: updates the momentum
+// there and returns the sum of squares.
 template <typename T, int KIND>
-__global__ __launch_bounds__(256) void sum_kernel(SumArgs a) {
-    __shared__ double lds[4];
-    int part = blockIdx.x, mat;
-    const int gi = findGroup(a.sh, part, mat);
-    const Group &g = a.sh.g[gi];
-    mat += g.mat0;
-    const MatRec &r = a.recs[mat];
-    const int64_t n = (int64_t)g.s * g.w;
-    const int64_t from = part * a.per[gi];
-    const int64_t to = from + a.per[gi] < n ? from + a.per[gi] : n;
+__device__ double sumPass(const MatRec &r, const StepArgs &a, int64_t from, int64_t to) {
     const T *src = (const T *)(KIND == kSumAux ? r.aux : r.g);
     const int64_t rs = KIND == kSumAux ? r.aux_rs : r.g_rs;
     const int64_t cs = KIND == kSumAux ? r.aux_cs : r.g_cs;
     // the steps' tensors are dense by contract
-    const bool flat = KIND >= kMomentum || (cs == 1 && rs == g.w) || (rs == 1 && cs == g.s);
+    const bool flat = KIND >= kMomentum || (cs == 1 && rs == r.w) || (rs == 1 && cs == r.s);
     double sum = 0.0;
     // In double: values next to a border (decay rates are short decimals, 16-bit values short
     // binary fractions, so ties are common) round as the exact sum does, whatever the type.
-    auto next = [&](double m, float grad) { return a.momentum64 * m + (double)grad; };
-    for (int64_t e = from + (int64_t)threadIdx.x * 8; (e & ~(int64_t)127) < to; e += 2048) {
+    auto next = [&](double m, float grad) { return a.momentum * m + (double)grad; };
+    for (int64_t e = from + (int64_t)threadIdx.x * 8; (e & ~(int64_t)127) < to; e += (int64_t)blockDim.x * 8) {
         // (the bound keeps the 16 lanes of an 8-bit block together)
         const int valid = e >= to ? 0 : to - e < 8 ? (int)(to - e) : 8;
         float v[8];
@@ -214,8 +234,8 @@ __global__ __launch_bounds__(256) void sum_kernel(SumArgs a) {
             } else {
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    const int64_t x = e + i, row = x / g.w, col = x - row * g.w;
-                    v[i] = i < valid ? toFloat(src[row * rs + col * cs]) : 0.f;
+                    const int64_t x = e + i, row = x / r.w, col = x - row * r.w;
+                    v[i] = i < valid ? toFloat(global<T>(src)[row * rs + col * cs]) : 0.f;
                 }
             }
         } else {
@@ -225,15 +245,15 @@ __global__ __launch_bounds__(256) void sum_kernel(SumArgs a) {
             for (int i = 0; i < 8; ++i) grad[i] *= a.sign;
             if (KIND == kMomentumI8) {
                 int8_t *codes = (int8_t *)const_cast<void *>(r.aux) + e;
-                const float old = valid ? r.scales[e >> 7] : 0.f;
+                const float old = valid ? global<float>(r.scales)[e >> 7] : 0.f;
                 double d[8];
                 unsigned long long peak = 0;
                 int8_t c[8];
                 if (valid == 8 && ((uintptr_t)codes & 7) == 0) {
-                    *(int2 *)c = *(const int2 *)codes;
+                    unpack8(*global<int64_t>(codes), c);
                 } else {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) c[i] = i < valid ? codes[i] : (int8_t)0;
+                    for (int i = 0; i < 8; ++i) c[i] = i < valid ? global<int8_t>(codes)[i] : (int8_t)0;
                 }
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -249,13 +269,13 @@ __global__ __launch_bounds__(256) void sum_kernel(SumArgs a) {
                     m[i] = (float)c[i] * scale;
                 }
                 if (valid == 8 && ((uintptr_t)codes & 7) == 0) {
-                    *(int2 *)codes = *(const int2 *)c;
+                    *global<int64_t>((void *)codes) = pack8(c);
                 } else {
 #pragma unroll
                     for (int i = 0; i < 8; ++i)
-                        if (i < valid) codes[i] = c[i];
+                        if (i < valid) global<int8_t>((void *)codes)[i] = c[i];
                 }
-                if (valid && (e & 127) == 0) r.scales[e >> 7] = scale;
+                if (valid && (e & 127) == 0) global<float>((void *)r.scales)[e >> 7] = scale;
             } else if (KIND == kMomentumF32) {
                 float *buf = (float *)const_cast<void *>(r.aux) + e;
                 load8(buf, valid, m);
@@ -272,14 +292,26 @@ __global__ __launch_bounds__(256) void sum_kernel(SumArgs a) {
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                v[i] = a.nesterov ? __builtin_fmaf(a.momentum, m[i], grad[i]) : m[i];
+                v[i] = a.nesterov ? __builtin_fmaf((float)a.momentum, m[i], grad[i]) : m[i];
                 if (i >= valid) v[i] = 0.f;  // (0 * NaN of a block that stands for NaN)
             }
         }
 #pragma unroll
         for (int i = 0; i < 8; ++i) sum += (double)v[i] * (double)v[i];
     }
-    sum = blockSum(sum, lds);
+    return sum;
+}
+
+template <typename T, int KIND>
+__global__ __launch_bounds__(256) void sum_kernel(SumArgs a) {
+    __shared__ double lds[4];
+    int part = blockIdx.x, mat;
+    const int gi = findGroup(a.sh, part, mat);
+    mat += a.sh.g[gi].mat0;
+    const MatRec &r = a.recs[mat];
+    const int64_t n = (int64_t)r.s * r.w, from = part * a.per[gi];
+    const int64_t to = from + a.per[gi] < n ? from + a.per[gi] : n;
+    const double sum = blockSum(sumPass<T, KIND>(r, a.step, from, to), lds);
     if (threadIdx.x == 0) a.parts[(int64_t)mat * kMaxParts + part] = sum;
 }
 
@@ -290,16 +322,21 @@ struct Factor {
                                  // turn: the sum is multiplied with it between the products
 };
 
-struct FactorArgs {
-    const double *parts, *parts_y;  // parts_y: of the cotangent, or null
-    MatNorm *norms;
-    Factor *factors;                // [matrix][stages]
-    int steps, stages, square;      // square: S carries h
+struct Series {
+    int steps, square;              // square: S carries h
     float a, b, c;
     double eps, h;
     double x[kMaxSteps + 1];        // bound of |X_k| from a start of norm 1
     double r[kMaxSteps];            // bound of |p(t) / t| on [0, x_k], which is |P|'s
     double d[kMaxSteps];            // bound of |p'| on [0, x_k]
+};
+
+struct FactorArgs {
+    Series q;
+    const double *parts, *parts_y;  // parts_y: of the cotangent, or null
+    MatNorm *norms;
+    Factor *factors;                // [matrix][stages]
+    int stages;
     int nparts[kMaxGroups], mat_end[kMaxGroups], ngroups;
 };
 
@@ -315,55 +352,83 @@ __device__ inline double startOf(double size, double eps) {
     return s0 > 1e-30 && s0 <= 1.0 ? s0 : s0 <= 1e-30 ? 1e-30 : 1.0;  // NaN: as if 1
 }
 
+// The arrays of a series, read by thread number: in LDS.
+struct SeriesTable {
+    double x[kMaxSteps + 1], r[kMaxSteps], d[kMaxSteps];
+    __device__ void load(const Series &q) {  // by all threads; a barrier has to follow
+        const int i = threadIdx.x;
+        if (i <= q.steps) x[i] = q.x[i];
+        if (i < q.steps) {
+            r[i] = q.r[i];
+            d[i] = q.d[i];
+        }
+    }
+};
+
+// Bounds of one matrix's iterates and cotangents.
+struct Bounds {
+    const Series &q;
+    const SeriesTable &table;
+    const double start, ysize;
+    __device__ Bounds(const Series &q_, const SeriesTable &table_, double size, double ysize_)
+        : q(q_), table(table_), start(startOf(size, q_.eps)),
+          ysize(ysize_ == ysize_ && ysize_ < 1e300 ? ysize_ : 1.0) {}
+    __device__ double x(int i) const {  // of X_i
+        double grown = start;
+        for (int j = 0; j < i; ++j) grown *= table.r[j];
+        return grown < table.x[i] ? grown : table.x[i];
+    }
+    __device__ double y(int i) const {  // of the cotangent of X_i
+        double v = ysize;
+        for (int j = q.steps - 1; j >= i; --j) v *= table.d[j];
+        return v;
+    }
+};
+
+__device__ inline MatNorm normOf(const Bounds &b, double size) {
+    const double plus = size + b.q.eps;
+    return {ldexp(1.0 / plus, expOf(b.x(0))), ldexp(1.0, expOf(b.y(b.q.steps))), size, plus};
+}
+
+// The factors of step t's stages: f[0..2] for S, P, X'; back[0..2] (or null) for M, N, Y.
+__device__ inline void stepFactors(const Bounds &b, int t, Factor *f, Factor *back) {
+    const Series &q = b.q;
+    const double x = b.x(t), x2 = x * x, ab = fabs((double)q.b), ac = fabs((double)q.c);
+    const double sbound = q.square ? fmax(fabs(q.h), fabs(q.h + x2)) : x2;
+    const int ex = expOf(x), es = expOf(sbound), ep = expOf(b.table.r[t]);
+    const bool last = t + 1 == q.steps;
+    const int ex1 = last && !back ? 0 : expOf(b.x(t + 1));
+    const float add = q.square ? 0.f : q.b;
+    const double unit = q.square ? (double)q.a - (double)q.b * q.h * 0.5 : (double)q.a;
+    f[0] = {ldexpf(1.f, es - 2 * ex), 0.f, 1.f, (float)(q.square ? ldexp(q.h, es) : 0.0)};
+    f[1] = {ldexpf(q.c, ep - 2 * es), ldexpf(add, ep - es), 1.f, (float)ldexp(unit, ep)};
+    f[2] = {ldexpf(1.f, ex1 - ep - ex), 0.f, 1.f, 0.f};
+    if (!back) return;
+    const double y1 = b.y(t + 1);
+    const int ey1 = expOf(y1), ey = t ? expOf(b.y(t)) : 0;
+    const int em = expOf(2.0 * x * y1), en = expOf((ab + 2.0 * ac * x2) * 2.0 * x * y1);
+    back[0] = {ldexpf(1.f, em - ey1 - ex), 0.f, 1.f, 0.f};
+    back[1] = {ldexpf(q.c, en - em - es), ldexpf(add, en - em), 1.f, 0.f};
+    back[2] = {ldexpf(1.f, ey - en - ex), 0.f, ldexpf(1.f, (en + ex) - (ep + ey1)), 0.f};
+}
+
 // One workgroup per matrix: norm, then a thread per step for the factors of its stages.
 __global__ __launch_bounds__(256) void factors_kernel(FactorArgs a) {
     __shared__ double lds[4];
+    __shared__ SeriesTable table;
     const int mat = blockIdx.x, t = threadIdx.x;
+    table.load(a.q);
     int k = 0;
     while (k + 1 < a.ngroups && mat >= a.mat_end[k]) ++k;
     const int np = a.nparts[k];
     const double size = sqrt(blockSum(t < np ? a.parts[(int64_t)mat * kMaxParts + t] : 0.0, lds));
     const double ysize =
         a.parts_y ? sqrt(blockSum(t < np ? a.parts_y[(int64_t)mat * kMaxParts + t] : 0.0, lds)) : 0.0;
-    const double s0 = startOf(size, a.eps), plus = size + a.eps;
-    auto bound = [&](int i) {  // of |X_i|
-        double grown = s0;
-        for (int j = 0; j < i; ++j) grown *= a.r[j];
-        return grown < a.x[i] ? grown : a.x[i];
-    };
-    auto ybound = [&](int i) {  // of the cotangent of X_i
-        double v = ysize == ysize && ysize < 1e300 ? ysize : 1.0;
-        for (int j = a.steps - 1; j >= i; --j) v *= a.d[j];
-        return v;
-    };
-    if (t == 0) {
-        MatNorm n;
-        n.x_scale = ldexp(1.0 / plus, expOf(bound(0)));
-        n.y_scale = ldexp(1.0, expOf(ybound(a.steps)));
-        n.size = size;
-        n.plus = plus;
-        a.norms[mat] = n;
-    }
-    if (t >= a.steps) return;
-    const double x = bound(t), x2 = x * x, ab = fabs((double)a.b), ac = fabs((double)a.c);
-    const double sbound = a.square ? fmax(fabs(a.h), fabs(a.h + x2)) : x2;
-    const int ex = expOf(x), es = expOf(sbound), ep = expOf(a.r[t]);
-    const bool last = t + 1 == a.steps;
-    const int ex1 = last && !a.parts_y ? 0 : expOf(bound(t + 1));
-    const float add = a.square ? 0.f : a.b;
-    const double unit = a.square ? (double)a.a - (double)a.b * a.h * 0.5 : (double)a.a;
+    const Bounds b(a.q, table, size, ysize);
+    if (t == 0) a.norms[mat] = normOf(b, size);
+    if (t >= a.q.steps) return;
     Factor *f = a.factors + (int64_t)mat * a.stages + 3 * t;
-    f[0] = {ldexpf(1.f, es - 2 * ex), 0.f, 1.f, (float)(a.square ? ldexp(a.h, es) : 0.0)};
-    f[1] = {ldexpf(a.c, ep - 2 * es), ldexpf(add, ep - es), 1.f, (float)ldexp(unit, ep)};
-    f[2] = {ldexpf(1.f, ex1 - ep - ex), 0.f, 1.f, 0.f};
-    if (!a.parts_y) return;
-    const double y1 = ybound(t + 1);
-    const int ey1 = expOf(y1), ey = t ? expOf(ybound(t)) : 0;
-    const int em = expOf(2.0 * x * y1), en = expOf((ab + 2.0 * ac * x2) * 2.0 * x * y1);
-    f = a.factors + (int64_t)mat * a.stages + 3 * a.steps + 3 * t;
-    f[0] = {ldexpf(1.f, em - ey1 - ex), 0.f, 1.f, 0.f};
-    f[1] = {ldexpf(a.c, en - em - es), ldexpf(add, en - em), 1.f, 0.f};
-    f[2] = {ldexpf(1.f, ey - en - ex), 0.f, ldexpf(1.f, (en + ex) - (ep + ey1)), 0.f};
+    stepFactors(b, t, f, a.parts_y ? f + 3 * a.q.steps : nullptr);
 }
 
 // ---- operands ----------------------------------------------------------------------------------
@@ -413,9 +478,26 @@ struct PackArgs {
     const MatNorm *norms;
     char *ws;
     int64_t off[kMaxGroups], off_t[kMaxGroups];  // of the operand and of its transpose
-    float momentum, sign;
-    int nesterov, split;
+    StepArgs step;
+    int split;
 };
+
+// An element of G, of the step's U, or of the cotangent, `at` elements behind the first.
+template <typename T, int KIND>
+__device__ inline float element(const MatRec &r, const StepArgs &a, int64_t at) {
+    float v = toFloat(global<T>(KIND == kPackAux ? r.aux : r.g)[at]);
+    if (KIND >= kPackM) {
+        float m;
+        if (KIND == kPackMI8)
+            m = (float)global<int8_t>(r.aux)[at] * global<float>(r.scales)[at >> 7];
+        else if (KIND == kPackMF32)
+            m = global<float>(r.aux)[at];
+        else
+            m = toFloat(global<T>(r.aux)[at]);
+        v = a.nesterov ? __builtin_fmaf((float)a.momentum, m, a.sign * v) : m;
+    }
+    return v;
+}
 
 // G (or the step's U, or the cotangent) -> the operand and its transpose, by tiles of 64 x 64.
 template <typename T, int KIND>
@@ -430,7 +512,6 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     const int across = (int)(padded(g.w) / 64);
     const int i0 = t / across * 64, j0 = t % across * 64;
     const double scale = KIND == kPackAux ? a.norms[mat].y_scale : a.norms[mat].x_scale;
-    const T *src = (const T *)(KIND == kPackAux ? r.aux : r.g);
     const int64_t rs = KIND == kPackAux ? r.aux_rs : r.g_rs, cs = KIND == kPackAux ? r.aux_cs : r.g_cs;
     const bool by_rows = cs <= rs;  // lanes run along the smaller stride
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -439,21 +520,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
         const int di = by_rows ? q : lane, dj = by_rows ? lane : q;
         const int i = i0 + di, j = j0 + dj;
         float v = 0.f;
-        if (i < g.s && j < g.w) {
-            const int64_t at = i * rs + j * cs;
-            v = toFloat(src[at]);
-            if (KIND >= kPackM) {
-                float m;
-                if (KIND == kPackMI8)
-                    m = (float)((const int8_t *)r.aux)[at] * r.scales[at >> 7];
-                else if (KIND == kPackMF32)
-                    m = ((const float *)r.aux)[at];
-                else
-                    m = toFloat(((const T *)r.aux)[at]);
-                v = a.nesterov ? __builtin_fmaf(a.momentum, m, a.sign * v) : m;
-            }
-            v = (float)((double)v * scale);
-        }
+        if (i < g.s && j < g.w) v = (float)((double)element<T, KIND>(r, a.step, i * rs + j * cs) * scale);
         tile[di][dj] = v;
     }
     __syncthreads();
@@ -500,6 +567,17 @@ struct GemmArgs {
 
 __device__ inline f32x16 mfma(half8 a, half8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+
+// Matrix instructions stand in groups between these two.  Without them the compiler mixes ordinary
+// instructions in that write a register which the matrix instruction just before them reads; in two
+// kernels such a write, by the very next instruction into a right operand's second register, was
+// lost, always and only there.
+__device__ inline void beforeMatrix() { __builtin_amdgcn_sched_barrier(0); }
+__device__ inline void afterMatrix() {
+    __builtin_amdgcn_sched_barrier(0);
+    asm volatile("s_nop 7");
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // Row and column of tile number t: row-major, or the lower triangle of a symmetric result.
@@ -640,11 +718,12 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void gemm_kernel(GemmArgs a) {
         for (int j = 0; j < TN; ++j) to[j] = frag(from, BM + wj + 32 * j, c);
     };
     auto multiply = [&](const half8 *x, const half8 *y) {
+        beforeMatrix();
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j) acc[i][j] = mfma(x[i], y[j], acc[i][j]);
-        __builtin_amdgcn_sched_barrier(0);
+        afterMatrix();
     };
 
     // share number `share` of the loads of the piece that `from_piece` chose
@@ -819,7 +898,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void gemm_kernel(GemmArgs a) {
                     store8(o, valid, v);
                 } else {
                     for (int q = 0; q < 8 && q < valid; ++q) {
-                        T *x = o + q * r.out_cs;
+                        TOA_GLOBAL T *x = global<T>((void *)(o + q * r.out_cs));
                         *x = fromFloat<T>(a.mode == kToParam ? r.keep * toFloat(*x) - r.rate * v[q]
                                                              : r.rate * v[q]);
                     }
@@ -858,7 +937,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void gemm_kernel(GemmArgs a) {
                         store8(o, valid, v);
                     } else {
                         for (int q = 0; q < 8 && q < valid; ++q) {
-                            T *x = o + q * r.out_rs;
+                            TOA_GLOBAL T *x = global<T>((void *)(o + q * r.out_rs));
                             *x = fromFloat<T>(a.mode == kToParam
                                                   ? r.keep * toFloat(*x) - r.rate * v[q]
                                                   : r.rate * v[q]);
@@ -869,6 +948,532 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void gemm_kernel(GemmArgs a) {
         }
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
+    }
+}
+
+// ---- small matrices ----------------------------------------------------------------------------
+//
+// Up to 32 rows and 864 columns, or 64 and 224: one workgroup takes a matrix through everything, and
+// the iterates never leave its LDS.  What a small matrix costs is not arithmetic but the way through
+// eighteen launches (32 x 288: 125 us by them, of which 100 are starts and ends).
+//
+// Eight waves share the columns by blocks of 32.  A block's result of a matrix instruction has a
+// column in each lane and rows in its registers (layout C); that is just the layout of the right
+// operand of P X -- the order of the rows within the sum is another one, but P can be read in the
+// same order.  The other way round, X^T P gives rows in the lanes and columns in the registers
+// (layout R), which is what X X^T wants of both its operands.  So each product is made twice, once
+// in each layout, and nothing is ever transposed.
+
+constexpr int kSmallWaves = 8;
+constexpr int kSmallInline = 24;  // records that fit in a launch's arguments
+
+struct SmallArgs {
+    Series q;
+    StepArgs step;
+    const MatRec *recs;  // or null: the records below
+    char *ws;            // gradient: the iterates, `stride` bytes for each matrix
+    int64_t stride;
+    int apply;
+    MatRec r[kSmallInline];
+};
+
+__host__ __device__ constexpr int smallRow(int rb) { return rb * 128 + 8; }  // (8: rows 32 lanes apart hit other banks)
+
+// Bytes the gradient keeps of one step: both layouts of every block of 32 columns, and S.
+__host__ __device__ constexpr int64_t smallKept(int rb, int w) {
+    return (int64_t)((w + 31) / 32) * rb * 2 * 4096 + (int64_t)rb * 32 * smallRow(rb);
+}
+
+// 16 values of a layout as operand registers: hi and lo for each half of the sum.
+struct Pair {
+    half8 hi[2], lo[2];
+    __device__ void set(const f32x16 &v) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            hi[i >> 3][i & 7] = (_Float16)v[i];
+            // (v - hi, which is exact, as the one instruction that reads a half in place)
+            lo[i >> 3][i & 7] = (_Float16)__builtin_fmaf((float)hi[i >> 3][i & 7], -1.f, v[i]);
+        }
+    }
+    __device__ float value(int i) const { return (float)hi[i >> 3][i & 7] + (float)lo[i >> 3][i & 7]; }
+};
+
+__device__ inline f32x16 multiply(const Pair &a, const Pair &b, f32x16 sum) {
+    beforeMatrix();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        sum = mfma(a.lo[t], b.hi[t], sum);
+        sum = mfma(a.hi[t], b.lo[t], sum);
+        sum = mfma(a.hi[t], b.hi[t], sum);
+    }
+    afterMatrix();
+    return sum;
+}
+
+// p x into one sum and x p into another, by turns: neither waits for its own last result.
+__device__ inline void multiplyBoth(const Pair &p, const Pair &x, f32x16 &px, f32x16 &xp) {
+    beforeMatrix();
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+        px = mfma(p.lo[t], x.hi[t], px);
+        xp = mfma(x.hi[t], p.lo[t], xp);
+        px = mfma(p.hi[t], x.lo[t], px);
+        xp = mfma(x.lo[t], p.hi[t], xp);
+        px = mfma(p.hi[t], x.hi[t], px);
+        xp = mfma(x.hi[t], p.hi[t], xp);
+    }
+    afterMatrix();
+}
+
+__device__ inline f32x16 zero16() {
+    f32x16 v;
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.f;
+    return v;
+}
+
+// Row (layout C) or column (layout R) within a block of register i.
+__device__ inline int laneRow(int i, int lane) { return (i >> 2) * 8 + (lane >> 5) * 4 + (i & 3); }
+
+// Block (r, k) of a symmetric matrix in LDS as an operand, its sum in the order of laneRow.
+template <int RB> __device__ inline Pair readSymmetric(const char *m, int r, int k, int lane) {
+    typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+    const char *row = m + (r * 32 + (lane & 31)) * smallRow(RB) + k * 128 + (lane >> 5) * 8;
+    Pair p;
+#pragma unroll
+    for (int t = 0; t < 2; ++t)
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const half4 hi = *(const half4 *)(row + (2 * t + u) * 16);
+            const half4 lo = *(const half4 *)(row + 64 + (2 * t + u) * 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                p.hi[t][4 * u + i] = hi[i];
+                p.lo[t][4 * u + i] = lo[i];
+            }
+        }
+    return p;
+}
+
+template <int RB> __device__ inline void writeElement(char *m, int row, int col, float v) {
+    _Float16 *p = (_Float16 *)(m + row * smallRow(RB) + (col >> 5) * 128) + (col & 31);
+    const _Float16 hi = (_Float16)v;
+    p[0] = hi;
+    p[32] = (_Float16)(v - (float)hi);
+}
+
+// A result block of a symmetric matrix (layout C) into LDS, with its mirror image.
+template <int RB>
+__device__ inline void writeSymmetric(char *m, int r, int k, int lane, const f32x16 &v, const Factor &f) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const int row = r * 32 + laneRow(i, lane), col = k * 32 + (lane & 31);
+        const float x = v[i] * f.acc + (row == col ? f.diag : 0.f);
+        writeElement<RB>(m, row, col, x);
+        if (r != k) writeElement<RB>(m, col, row, x);
+    }
+}
+
+// Adds up the waves' shares of a symmetric matrix (lower blocks, always in the same order) into LDS.
+// With 64 rows there is LDS for the shares of four waves: the others' are added to theirs first.
+constexpr int smallSlots(int rb) { return rb == 1 ? kSmallWaves : kSmallWaves / 2; }
+
+template <int RB>
+__device__ inline void gather(f32x16 (&share)[RB * (RB + 1) / 2], float *shares, char *m,
+                              const Factor &f) {
+    constexpr int kBlocks = RB * (RB + 1) / 2, kSlots = smallSlots(RB);
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    auto put = [&](int slot) {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) shares[((b * kSlots + slot) * 16 + i) * 64 + lane] = share[b][i];
+    };
+    if (kSlots < kSmallWaves) {
+        if (wave >= kSlots) put(wave - kSlots);
+        __syncthreads();
+        if (wave < kSlots) {
+#pragma unroll
+            for (int b = 0; b < kBlocks; ++b)
+#pragma unroll
+                for (int i = 0; i < 16; ++i)
+                    share[b][i] += shares[((b * kSlots + wave) * 16 + i) * 64 + lane];
+        }
+    }
+    if (wave < kSlots) put(wave);
+    __syncthreads();
+    for (int e = threadIdx.x; e < kBlocks * 1024; e += kSmallWaves * 64) {
+        const int b = e >> 10, x = e & 1023;
+        float v = 0.f;
+#pragma unroll
+        for (int w = 0; w < kSlots; ++w) v += shares[(b * kSlots + w) * 1024 + x];
+        const int r = b ? 1 : 0, k = b == 2 ? 1 : 0;  // (0,0), (1,0), (1,1)
+        const int row = r * 32 + laneRow(x >> 6, x & 63), col = k * 32 + (x & 31);
+        v = v * f.acc + (row == col ? f.diag : 0.f);
+        writeElement<RB>(m, row, col, v);
+        if (r != k) writeElement<RB>(m, col, row, v);
+    }
+    __syncthreads();
+}
+
+// A copy in scalar registers.
+__device__ inline MatRec uniform(const MatRec *p) {
+    MatRec r;
+    constexpr int kWords = sizeof(MatRec) / 4;
+    int words[kWords];
+    __builtin_memcpy(words, p, sizeof(MatRec));
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) words[i] = __builtin_amdgcn_readfirstlane(words[i]);
+    __builtin_memcpy(&r, words, sizeof(MatRec));
+    return r;
+}
+
+constexpr int smallColumnBlocks(int rb) { return rb == 1 ? 27 : 7; }
+
+template <typename T, int KIND, int RB, bool BACK>
+__global__ __launch_bounds__(kSmallWaves * 64) void small_kernel(SmallArgs a) {
+    using Word = half8;
+    constexpr int kBlocks = RB * (RB + 1) / 2, kMatrix = RB * 32 * smallRow(RB);
+    __shared__ Word X[smallColumnBlocks(RB) * RB * 256];
+    __shared__ float shares[kBlocks * smallSlots(RB) * 1024];
+    __shared__ __attribute__((aligned(16))) char S[kMatrix], P[kMatrix], M[BACK ? kMatrix : 16];
+    __shared__ Factor factors[(BACK ? 6 : 3) * kMaxSteps];
+    __shared__ double sums[kSmallWaves];
+    __shared__ SeriesTable table;
+
+    const MatRec r = uniform(a.recs ? a.recs + blockIdx.x : a.r + blockIdx.x);
+    const int s = r.s, w = r.w, steps = a.q.steps;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int64_t n = (int64_t)s * w;
+    char *kept = BACK ? a.ws + blockIdx.x * a.stride : nullptr;
+    table.load(a.q);
+
+    constexpr int kSum = KIND == kPackG ? kSumG : KIND == kPackM ? kMomentum
+                         : KIND == kPackMF32 ? kMomentumF32 : kMomentumI8;
+    const double size = sqrt(blockSum(sumPass<T, kSum>(r, a.step, 0, n), sums));
+    const double ysize = BACK ? sqrt(blockSum(sumPass<T, kSumAux>(r, a.step, 0, n), sums)) : 0.0;
+    const Bounds bounds(a.q, table, size, ysize);
+    const MatNorm norm = normOf(bounds, size);
+    if ((int)threadIdx.x < steps)
+        stepFactors(bounds, threadIdx.x, factors + 3 * threadIdx.x,
+                    BACK ? factors + 3 * (steps + threadIdx.x) : nullptr);
+    __syncthreads();
+
+    const int blocks = (w + 31) / 32;  // this wave's are number `wave`, wave + 8, ...
+    auto load = [&](auto kind, double scale, int b, int rb, bool by_rows) {
+        constexpr int kKind = decltype(kind)::value;
+        // a lane's first element, and the way to the others, which is the same for all lanes
+        const int row0 = rb * 32 + (by_rows ? lane & 31 : (lane >> 5) * 4);
+        const int j0 = b * 32 + (by_rows ? (lane >> 5) * 4 : lane & 31);
+        const int64_t rs = kKind == kPackAux ? r.aux_rs : r.g_rs, cs = kKind == kPackAux ? r.aux_cs : r.g_cs;
+        const int64_t at0 = row0 * rs + j0 * cs, by = by_rows ? cs : rs;
+        const int left = by_rows ? w - j0 : s - row0;  // elements along the registers
+        const bool inside = by_rows ? row0 < s : j0 < w;
+        f32x16 v;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int along = (i >> 2) * 8 + (i & 3);
+            const bool valid = inside && along < left;
+            // (read in any case, element 0 if need be: a branch would wait for every one in turn)
+            const float e = element<T, kKind>(r, a.step, valid ? at0 + along * by : 0);
+            v[i] = valid ? (float)((double)e * scale) : 0.f;
+        }
+        return v;
+    };
+    // registers in LDS, and (the gradient's iterates) in the workspace: 16 bytes of each lane in turn
+    auto putPair = [&](auto *to, const Pair &p) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            to[t * 64 + lane] = p.hi[t];
+            to[(2 + t) * 64 + lane] = p.lo[t];
+        }
+    };
+    auto getPair = [&](const auto *from) {
+        Pair p;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+            p.hi[t] = from[t * 64 + lane];
+            p.lo[t] = from[(2 + t) * 64 + lane];
+        }
+        return p;
+    };
+    auto inLds = [&](int b, int rb) { return X + (b * RB + rb) * 256; };
+    auto inKept = [&](int k, int b, int rb, int layout) {
+        return global<Word>((void *)(kept + k * smallKept(RB, w) +
+                                     (((int64_t)b * RB + rb) * 2 + layout) * 4096));
+    };
+    auto inKeptS = [&](int k) {
+        return global<int64_t>((void *)(kept + (k + 1) * smallKept(RB, w) - kMatrix));
+    };
+    auto copyMatrix = [&](auto *to, const auto *from) {
+        for (int i = threadIdx.x; i < kMatrix / 8; i += kSmallWaves * 64) to[i] = from[i];
+    };
+
+    using Main = std::integral_constant<int, KIND>;
+    f32x16 share[kBlocks];
+    auto clear = [&] {
+#pragma unroll
+        for (int b = 0; b < kBlocks; ++b) share[b] = zero16();
+    };
+    // adds a block's part of X X^T
+    auto addGram = [&](const Pair (&l)[RB]) {
+#pragma unroll
+        for (int p = 0; p < RB; ++p)
+#pragma unroll
+            for (int q = 0; q <= p; ++q)
+                share[p * (p + 1) / 2 + q] = multiply(l[p], l[q], share[p * (p + 1) / 2 + q]);
+    };
+    clear();
+#pragma unroll 1
+    for (int b = wave; b < blocks; b += kSmallWaves) {
+        Pair l[RB];
+#pragma unroll
+        for (int p = 0; p < RB; ++p) {
+            Pair c;
+            c.set(load(Main(), norm.x_scale, b, p, false));
+            l[p].set(load(Main(), norm.x_scale, b, p, true));
+            putPair(inLds(b, p), c);
+            if (BACK) {
+                putPair(inKept(0, b, p, 0), c);
+                putPair(inKept(0, b, p, 1), l[p]);
+            }
+        }
+        addGram(l);
+    }
+    // the block of a symmetric result that a wave makes
+    const int bp = wave ? 1 : 0, bq = wave == 2 ? 1 : 0;
+    // v * f.acc + f.add * (block of m)
+    auto withThird = [&](f32x16 v, const char *m, const Factor &f) {
+        v *= f.acc;
+        if (f.add != 0.f) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const _Float16 *e =
+                    (const _Float16 *)(m + ((RB == 1 ? 0 : bp * 32) + laneRow(i, lane)) * smallRow(RB) +
+                                       (RB == 1 ? 0 : bq * 128)) + (lane & 31);
+                v[i] += f.add * ((float)e[0] + (float)e[32]);
+            }
+        }
+        return v;
+    };
+    // P from S.  With one block every wave makes it for itself: a result of a symmetric product is
+    // an operand as it stands (lanes and registers change places).  With four they share the work.
+    Pair own_p, own_n;
+    auto asOperand = [&](f32x16 v, float diag) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] += laneRow(i, lane) == (lane & 31) ? diag : 0.f;
+        Pair p;
+        p.set(v);
+        return p;
+    };
+    auto makeP = [&](const Factor &f) {
+        if (RB == 1) {
+            const Pair e = readSymmetric<RB>(S, 0, 0, lane);
+            own_p = asOperand(withThird(multiply(e, e, zero16()), S, f), f.diag);
+        } else {
+            if (wave < kBlocks) {
+                f32x16 v = zero16();
+#pragma unroll
+                for (int e = 0; e < RB; ++e)
+                    v = multiply(readSymmetric<RB>(S, bp, e, lane), readSymmetric<RB>(S, bq, e, lane), v);
+                writeSymmetric<RB>(P, bp, bq, lane, withThird(v, S, f), {1.f, 0.f, 1.f, f.diag});
+            }
+            __syncthreads();
+        }
+    };
+    auto operandP = [&](int p, int e) { return RB == 1 ? own_p : readSymmetric<RB>(P, p, e, lane); };
+#pragma unroll 1
+    for (int k = 0; k < steps; ++k) {
+        const Factor f0 = factors[3 * k], f1 = factors[3 * k + 1], f2 = factors[3 * k + 2];
+        const bool last = k + 1 == steps;
+        gather<RB>(share, shares, S, f0);
+        makeP(f1);
+        if (BACK) {
+            copyMatrix(inKeptS(k), (const int64_t *)S);
+            if (last) break;
+        }
+        clear();
+#pragma unroll 1
+        for (int b = wave; b < blocks; b += kSmallWaves) {
+            Pair x[RB], l[RB];
+#pragma unroll
+            for (int p = 0; p < RB; ++p) x[p] = getPair(inLds(b, p));
+#pragma unroll
+            for (int p = 0; p < RB; ++p) {
+                f32x16 vc = zero16(), vr = zero16();
+#pragma unroll
+                for (int e = 0; e < RB; ++e) {
+                    const Pair pe = operandP(p, e);
+                    if (last)
+                        vc = multiply(pe, x[e], vc);
+                    else
+                        multiplyBoth(pe, x[e], vc, vr);
+                }
+                vc *= f2.acc;
+                if (last) {
+                    const int j = b * 32 + (lane & 31);
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) {
+                        const int row = p * 32 + laneRow(i, lane);
+                        TOA_GLOBAL T *o = global<T>(r.out) + (row < s ? row : s - 1) * r.out_rs +
+                                          (j < w ? j : w - 1) * r.out_cs;
+                        float v = r.rate * vc[i];
+                        if (a.apply) v = r.keep * toFloat(*o) - v;
+                        if (row < s && j < w) *o = fromFloat<T>(v);
+                    }
+                } else {
+                    Pair c;
+                    c.set(vc);
+                    putPair(inLds(b, p), c);  // (x has been read)
+                    l[p].set(vr * f2.acc);
+                    if (BACK) {
+                        putPair(inKept(k + 1, b, p, 0), c);
+                        putPair(inKept(k + 1, b, p, 1), l[p]);
+                    }
+                }
+            }
+            if (!last) addGram(l);
+        }
+    }
+    if (!BACK) return;
+
+    // The way back: X holds the cotangent Y in layout C, share its part of Y X^T + X Y^T.
+    using Aux = std::integral_constant<int, kPackAux>;
+    auto addBoth = [&](const Pair (&y)[RB], const Pair (&l)[RB]) {
+#pragma unroll
+        for (int p = 0; p < RB; ++p)
+#pragma unroll
+            for (int q = 0; q <= p; ++q) {
+                f32x16 &v = share[p * (p + 1) / 2 + q];
+                v = multiply(y[p], l[q], v);
+                v = multiply(l[p], y[q], v);
+            }
+    };
+    clear();
+#pragma unroll 1
+    for (int b = wave; b < blocks; b += kSmallWaves) {
+        Pair l[RB];
+#pragma unroll
+        for (int p = 0; p < RB; ++p) {
+            Pair c;
+            c.set(load(Aux(), norm.y_scale, b, p, false));
+            l[p].set(load(Aux(), norm.y_scale, b, p, true));
+            putPair(inLds(b, p), c);
+        }
+        Pair xr[RB];
+#pragma unroll
+        for (int p = 0; p < RB; ++p) xr[p] = getPair(inKept(steps - 1, b, p, 1));
+        addBoth(l, xr);
+    }
+    // both layouts of a block of X_k and X_k-1, from the workspace: asked for well before their use
+    Pair next_c[RB], next_r[RB];
+    auto prefetch = [&](int k, int b) {
+        if (RB > 1 || b >= blocks) return;  // (two rows of blocks leave no registers for it)
+#pragma unroll
+        for (int p = 0; p < RB; ++p) {
+            next_c[p] = getPair(inKept(k, b, p, 0));
+            if (k) next_r[p] = getPair(inKept(k - 1, b, p, 1));
+        }
+    };
+    double dot = 0.0;
+#pragma unroll 1
+    for (int k = steps - 1; k >= 0; --k) {
+        const Factor f0 = factors[3 * (steps + k)], f1 = factors[3 * (steps + k) + 1],
+                     f2 = factors[3 * (steps + k) + 2];
+        prefetch(k, wave);
+        __syncthreads();  // S, P and M of the step before are no longer read
+        copyMatrix((int64_t *)S, inKeptS(k));
+        gather<RB>(share, shares, M, f0);
+        if (k + 1 < steps) makeP(factors[3 * k + 1]);  // (the last step's is still there)
+        f32x16 v = zero16();
+        if (RB == 1 || wave < kBlocks) {
+#pragma unroll
+            for (int e = 0; e < RB; ++e) {
+                const int p = RB == 1 ? 0 : bp, q = RB == 1 ? 0 : bq;
+                v = multiply(readSymmetric<RB>(M, p, e, lane), readSymmetric<RB>(S, q, e, lane), v);
+                v = multiply(readSymmetric<RB>(S, p, e, lane), readSymmetric<RB>(M, q, e, lane), v);
+            }
+            v = withThird(v, M, f1);
+        }
+        if (RB == 1) {
+            own_n.set(v);
+        } else {
+            __syncthreads();
+            if (wave < kBlocks) writeSymmetric<RB>(M, bp, bq, lane, v, {1.f, 0.f, 1.f, 0.f});  // N
+            __syncthreads();
+        }
+        clear();
+#pragma unroll 1
+        for (int b = wave; b < blocks; b += kSmallWaves) {
+            Pair y[RB], x[RB], xr[RB], l[RB];
+#pragma unroll
+            for (int e = 0; e < RB; ++e) {
+                y[e] = getPair(inLds(b, e));
+                x[e] = RB > 1 ? getPair(inKept(k, b, e, 0)) : next_c[e];
+                if (RB == 1) xr[e] = next_r[e];
+            }
+            prefetch(k, b + kSmallWaves);
+#pragma unroll
+            for (int o = 0; o < RB; ++o) {
+                f32x16 vc = zero16(), vr = zero16();
+#pragma unroll
+                for (int e = 0; e < RB; ++e) {
+                    const Pair pe = operandP(o, e);
+                    if (k)
+                        multiplyBoth(pe, y[e], vc, vr);
+                    else
+                        vc = multiply(pe, y[e], vc);
+                }
+                vc *= f2.turn;
+                vr *= f2.turn;
+#pragma unroll
+                for (int e = 0; e < RB; ++e) {
+                    const Pair ne = RB == 1 ? own_n : readSymmetric<RB>(M, o, e, lane);
+                    if (k)
+                        multiplyBoth(ne, x[e], vc, vr);
+                    else
+                        vc = multiply(ne, x[e], vc);
+                }
+                vc *= f2.acc;
+                if (k) {
+                    Pair c;
+                    c.set(vc);
+                    putPair(inLds(b, o), c);  // (y has been read)
+                    l[o].set(vr * f2.acc);
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) dot += (double)vc[i] * (double)x[o].value(i);
+                    putPair(inLds(b, o), __builtin_bit_cast(Pair, vc));  // Y_0 stays in float32
+                }
+            }
+            if (k) {
+                if (RB > 1) {
+#pragma unroll
+                    for (int e = 0; e < RB; ++e) xr[e] = getPair(inKept(k - 1, b, e, 1));
+                }
+                addBoth(l, xr);
+            }
+        }
+    }
+    // through X_0 = G / (|G| + eps), as in tail_kernel
+    dot = blockSum(dot, sums);
+    const double back = 1.0 / (norm.x_scale * norm.plus), ky = 1.0 / norm.plus;
+    const double kx = norm.size > 0.0 ? dot * back / norm.size * back : norm.size;
+#pragma unroll 1
+    for (int b = wave; b < blocks; b += kSmallWaves) {
+        const int j = b * 32 + (lane & 31);
+#pragma unroll
+        for (int p = 0; p < RB; ++p) {
+            const Pair x = getPair(inKept(0, b, p, 0));
+            const f32x16 y = __builtin_bit_cast(f32x16, getPair(inLds(b, p)));
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int row = p * 32 + laneRow(i, lane);
+                if (row < s && j < w)
+                    global<T>(r.out)[row * r.out_rs + j * r.out_cs] =
+                        fromFloat<T>((float)(ky * (double)y[i] - kx * (double)x.value(i)));
+            }
+        }
     }
 }
 
@@ -946,7 +1551,7 @@ template <typename T> __global__ __launch_bounds__(256) void tail_kernel(TailArg
     for (int q = threadIdx.x >> 6; q < 64; q += 4) {
         const int di = by_rows ? q : lane, dj = by_rows ? lane : q;
         if (i0 + di < g.s && j0 + dj < g.w)
-            ((T *)r.out)[(i0 + di) * r.out_rs + (j0 + dj) * r.out_cs] = fromFloat<T>(tile[di][dj]);
+            global<T>(r.out)[(i0 + di) * r.out_rs + (j0 + dj) * r.out_cs] = fromFloat<T>(tile[di][dj]);
     }
 }
 
@@ -991,13 +1596,13 @@ template <typename T> __global__ __launch_bounds__(256) void quantize_kernel(Blo
     for (int i = 0; i < 8; ++i) c[i] = (int8_t)codeOf((double)v[i], scale);
     int8_t *o = (int8_t *)a.out[k] + e;
     if (valid == 8 && ((uintptr_t)o & 7) == 0) {
-        *(int2 *)o = *(const int2 *)c;
+        *global<int64_t>((void *)o) = pack8(c);
     } else {
 #pragma unroll
         for (int i = 0; i < 8; ++i)
-            if (i < valid) o[i] = c[i];
+            if (i < valid) global<int8_t>((void *)o)[i] = c[i];
     }
-    if (valid && (e & 127) == 0) a.scales[k][e >> 7] = scale;
+    if (valid && (e & 127) == 0) global<float>((void *)a.scales[k])[e >> 7] = scale;
 }
 
 template <typename T> __global__ __launch_bounds__(256) void dequantize_kernel(BlocksArgs a) {
@@ -1007,13 +1612,13 @@ template <typename T> __global__ __launch_bounds__(256) void dequantize_kernel(B
     if (e >= n) return;
     const int valid = n - e < 8 ? (int)(n - e) : 8;
     const int8_t *p = (const int8_t *)a.in[k] + e;
-    const float scale = a.scales[k][e >> 7];
+    const float scale = global<float>(a.scales[k])[e >> 7];
     int8_t c[8];
     if (valid == 8 && ((uintptr_t)p & 7) == 0) {
-        *(int2 *)c = *(const int2 *)p;
+        unpack8(*global<int64_t>(p), c);
     } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = i < valid ? p[i] : (int8_t)0;
+        for (int i = 0; i < 8; ++i) c[i] = i < valid ? global<int8_t>(p)[i] : (int8_t)0;
     }
     float v[8];
 #pragma unroll

@@ -94,15 +94,53 @@ Head headOf(int64_t mats, int stages) {
     return h;
 }
 
+// Small matrices (see small_kernel): those of one kernel variant, `stride` bytes of kept iterates
+// for each in the gradient.
+struct SmallBatch {
+    int rb;
+    std::vector<size_t> mats;
+    int64_t stride = 0;
+
+    // records (where they do not fit in the launch), then the kept iterates
+    int64_t records() const {
+        return mats.size() > kSmallInline ? align256((int64_t)mats.size() * (int64_t)sizeof(MatRec)) : 0;
+    }
+    int64_t bytes() const { return records() + (int64_t)mats.size() * stride; }
+};
+
+// Rows / 32 of the variant that takes an s x w matrix, or 0.
+int smallVariant(int64_t s, int64_t w) {
+    for (int rb = 1; rb <= 2; ++rb)
+        if (s <= 32 * rb) return w <= 32 * smallColumnBlocks(rb) ? rb : 0;
+    return 0;
+}
+
 int plan(size_t num, const int64_t *rows, const int64_t *cols, int steps, bool backward,
-         std::vector<Batch> &batches, int64_t &bytes) {
+         std::vector<Batch> &batches, std::vector<SmallBatch> &smalls, int64_t &bytes) {
     bytes = 0;
     std::vector<size_t> order;
     order.reserve(num);
     for (size_t i = 0; i < num; ++i) {
         if (rows[i] < 0 || cols[i] < 0 || rows[i] > kMaxDim || cols[i] > kMaxDim) return TOA_ESIZE;
-        if (rows[i] && cols[i]) order.push_back(i);
+        if (!rows[i] || !cols[i]) continue;
+        const int64_t s = std::min(rows[i], cols[i]), w = std::max(rows[i], cols[i]);
+        const int rb = smallVariant(s, w);
+        if (!rb) {
+            order.push_back(i);
+            continue;
+        }
+        const int64_t kept = backward ? align256(steps * smallKept(rb, (int)w)) : 0;
+        auto it = std::find_if(smalls.rbegin(), smalls.rend(),
+                               [&](const SmallBatch &b) { return b.rb == rb; });
+        SmallBatch *b = it == smalls.rend() ? nullptr : &*it;
+        if (!b || ((int64_t)b->mats.size() + 1) * std::max(b->stride, kept) > kBatchBytes) {
+            smalls.push_back({rb, {}, 0});
+            b = &smalls.back();
+        }
+        b->mats.push_back(i);
+        b->stride = std::max(b->stride, kept);
     }
+    for (const SmallBatch &b : smalls) bytes = std::max(bytes, b.bytes());
     auto key = [&](size_t i) {
         return std::make_pair(std::min(rows[i], cols[i]), std::max(rows[i], cols[i]));
     };
@@ -168,7 +206,7 @@ int checkSeries(const toa_muon_series *q) {
 }
 
 // Bounds of the iterates from a start of norm 1 (with a hundredth of slack for rounding).
-int boundsOf(const toa_muon_series &q, FactorArgs &f) {
+int boundsOf(const toa_muon_series &q, Series &f) {
     f.a = (float)q.a;
     f.b = (float)q.b;
     f.c = (float)q.c;
@@ -235,15 +273,81 @@ double shapeRate(int adjust, int64_t rows, int64_t cols) {
     return 1.0;
 }
 
+MatRec recordOf(const Call &c, size_t i) {
+    const bool turned = c.rows[i] > c.cols[i];
+    MatRec r{};
+    auto put = [&](const toa_muon_view &v, int64_t &rs, int64_t &cs) {
+        rs = turned ? v.col_stride : v.row_stride;
+        cs = turned ? v.row_stride : v.col_stride;
+        return v.data;
+    };
+    r.g = put(c.g[i], r.g_rs, r.g_cs);
+    r.out = put(c.out[i], r.out_rs, r.out_cs);
+    if (c.aux) r.aux = put(c.aux[i], r.aux_rs, r.aux_cs);
+    r.scales = c.scales ? c.scales[i] : nullptr;
+    r.rate = 1.f;
+    if (c.hyper) {
+        const double rate = shapeRate(c.hyper->adjust, c.rows[i], c.cols[i]);
+        r.rate = (float)(c.hyper->apply ? c.hyper->lr * rate : rate);
+        r.keep = (float)(1.0 - c.hyper->lr * c.hyper->weight_decay);
+    }
+    r.s = (int)std::min(c.rows[i], c.cols[i]);
+    r.w = (int)std::max(c.rows[i], c.cols[i]);
+    return r;
+}
+
+int fillRecords(const Call &c, const std::vector<size_t> &mats, MatRec *to) {
+    for (size_t from = 0; from < mats.size(); from += kFill) {
+        FillArgs a{};
+        const int n = (int)std::min<size_t>(kFill, mats.size() - from);
+        for (int k = 0; k < n; ++k) a.r[k] = recordOf(c, mats[from + k]);
+        TRY(launch(fill_kernel, 1, 64, c.stream, a, to + from, n));
+    }
+    return 0;
+}
+
+StepArgs stepOf(const Call &c) {
+    if (!c.hyper) return StepArgs{};
+    return {c.hyper->momentum, c.hyper->maximize ? -1.f : 1.f, c.hyper->nesterov};
+}
+
+template <typename T, int RB> auto smallKernel(const Call &c) {
+    if (c.what == kBackward) return small_kernel<T, kPackG, RB, true>;
+    if (c.what == kOrthogonalize) return small_kernel<T, kPackG, RB, false>;
+    return c.momentum_dtype == TOA_I8      ? small_kernel<T, kPackMI8, RB, false>
+           : c.momentum_dtype == c.dtype ? small_kernel<T, kPackM, RB, false>
+                                          : small_kernel<T, kPackMF32, RB, false>;
+}
+
+int runSmall(const Call &c, const SmallBatch &b, const Series &series) {
+    SmallArgs a{};
+    a.q = series;
+    a.step = stepOf(c);
+    a.apply = c.hyper && c.hyper->apply;
+    a.stride = b.stride;
+    a.ws = c.ws + b.records();
+    if (b.records()) {
+        a.recs = (const MatRec *)c.ws;
+        TRY(fillRecords(c, b.mats, (MatRec *)c.ws));
+    } else {
+        for (size_t k = 0; k < b.mats.size(); ++k) a.r[k] = recordOf(c, b.mats[k]);
+    }
+    return withType(c.dtype, [&](auto t) {
+        using T = decltype(t);
+        return launch(b.rb == 1 ? smallKernel<T, 1>(c) : smallKernel<T, 2>(c),
+                      (int64_t)b.mats.size(), kSmallWaves * 64, c.stream, a);
+    });
+}
+
 class Run {
   public:
-    Run(const Call &c, const Batch &b, const FactorArgs &bounds)
+    Run(const Call &c, const Batch &b, const Series &series)
         : c_(c), b_(b), steps_(c.series.steps), back_(c.what == kBackward),
           stages_(3 * steps_ * (back_ ? 2 : 1)), head_(headOf((int64_t)b.mats.size(), stages_)),
-          f_(bounds) {}
+          f_{series} {}
 
     int go() {
-        TRY(fill());
+        TRY(fillRecords(c_, b_.mats, (MatRec *)(c_.ws + head_.recs)));
         TRY(sums());
         TRY(factors());
         TRY(pack(back_ ? 0 : -1));
@@ -258,35 +362,6 @@ class Run {
     bool split(int k) const { return back_ || c_.dtype != TOA_BF16 || k < steps_ - 2; }
 
     const MatRec *recs() const { return (const MatRec *)(c_.ws + head_.recs); }
-
-    int fill() {
-        for (size_t from = 0; from < b_.mats.size(); from += kFill) {
-            FillArgs a{};
-            const int n = (int)std::min<size_t>(kFill, b_.mats.size() - from);
-            for (int k = 0; k < n; ++k) {
-                const size_t i = b_.mats[from + k];
-                const bool turned = c_.rows[i] > c_.cols[i];
-                MatRec &r = a.r[k];
-                auto put = [&](const toa_muon_view &v, int64_t &rs, int64_t &cs) {
-                    rs = turned ? v.col_stride : v.row_stride;
-                    cs = turned ? v.row_stride : v.col_stride;
-                    return v.data;
-                };
-                r.g = put(c_.g[i], r.g_rs, r.g_cs);
-                r.out = put(c_.out[i], r.out_rs, r.out_cs);
-                if (c_.aux) r.aux = put(c_.aux[i], r.aux_rs, r.aux_cs);
-                r.scales = c_.scales ? c_.scales[i] : nullptr;
-                r.rate = 1.f;
-                if (c_.hyper) {
-                    const double rate = shapeRate(c_.hyper->adjust, c_.rows[i], c_.cols[i]);
-                    r.rate = (float)(c_.hyper->apply ? c_.hyper->lr * rate : rate);
-                    r.keep = (float)(1.0 - c_.hyper->lr * c_.hyper->weight_decay);
-                }
-            }
-            TRY(launch(fill_kernel, 1, 64, c_.stream, a, (MatRec *)(c_.ws + head_.recs) + from, n));
-        }
-        return 0;
-    }
 
     // Shapes of a launch with tilesOf(shape) workgroups for each matrix.
     template <typename F> int64_t shapes(Shapes &sh, F tilesOf) const {
@@ -306,12 +381,7 @@ class Run {
         SumArgs a{};
         a.recs = recs();
         a.parts = (double *)(c_.ws + head_.parts);
-        if (c_.hyper) {
-            a.momentum = (float)c_.hyper->momentum;
-            a.momentum64 = c_.hyper->momentum;
-            a.sign = c_.hyper->maximize ? -1.f : 1.f;
-            a.nesterov = c_.hyper->nesterov;
-        }
+        a.step = stepOf(c_);
         const int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int k) {
             const int64_t n = (int64_t)s.s * s.w;
             int64_t per = std::max<int64_t>(8192, (n + kMaxParts - 1) / kMaxParts);
@@ -352,11 +422,7 @@ class Run {
         a.norms = (const MatNorm *)(c_.ws + head_.norms);
         a.ws = c_.ws;
         a.split = split(0);
-        if (c_.hyper) {
-            a.momentum = (float)c_.hyper->momentum;
-            a.sign = c_.hyper->maximize ? -1.f : 1.f;
-            a.nesterov = c_.hyper->nesterov;
-        }
+        a.step = stepOf(c_);
         const int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int k) {
             a.off[k] = s.lay.x[0];
             a.off_t[k] = s.lay.xt[0];
@@ -488,7 +554,7 @@ class Run {
         }));
         TRY(product(3 * k + 1, k, sp, true, kToOperand, [&](Product &p, const Layout &l, int ld_s, int) {
             p.a0 = p.b0 = l.s[k];
-            if (!f_.square) p.e = l.s[k];
+            if (!f_.q.square) p.e = l.s[k];
             p.lda = p.ldb = ld_s;
             p.d = p.dt = l.p[k];
         }));
@@ -517,7 +583,7 @@ class Run {
         }));
         TRY(product(stage + 1, k, true, true, kToOperand, [&](Product &p, const Layout &l, int ld_s, int) {
             p.a0 = p.b1 = l.m;
-            if (!f_.square) p.e = l.m;
+            if (!f_.q.square) p.e = l.m;
             p.b0 = p.a1 = l.s[k];
             p.lda = p.ldb = ld_s;
             p.steps1 = 1;
@@ -572,21 +638,23 @@ class Run {
 
 int run(const Call &call, size_t num, const void *workspace, size_t workspace_bytes) {
     if (call.dtype != TOA_F32 && call.dtype != TOA_F16 && call.dtype != TOA_BF16) return TOA_EDTYPE;
-    FactorArgs bounds{};
-    TRY(boundsOf(call.series, bounds));
+    Series series{};
+    TRY(boundsOf(call.series, series));
     if (num == 0) return 0;
     if (!call.rows || !call.cols) return TOA_ENULL;
     std::vector<Batch> batches;
+    std::vector<SmallBatch> smalls;
     int64_t bytes;
-    TRY(plan(num, call.rows, call.cols, call.series.steps, call.what == kBackward, batches, bytes));
-    if (batches.empty()) return 0;
+    TRY(plan(num, call.rows, call.cols, call.series.steps, call.what == kBackward, batches, smalls,
+             bytes));
+    if (batches.empty() && smalls.empty()) return 0;
     if (!call.g || !call.out || (call.what != kOrthogonalize && !call.aux)) return TOA_ENULL;
-    for (const Batch &b : batches)
-        for (size_t i : b.mats)
-            if (!call.g[i].data || !call.out[i].data || (call.aux && !call.aux[i].data) ||
-                (call.momentum_dtype == TOA_I8 && (!call.scales || !call.scales[i])))
-                return TOA_ENULL;
-    if (!workspace) return TOA_ENULL;
+    for (size_t i = 0; i < num; ++i)
+        if (call.rows[i] && call.cols[i] &&
+            (!call.g[i].data || !call.out[i].data || (call.aux && !call.aux[i].data) ||
+             (call.momentum_dtype == TOA_I8 && (!call.scales || !call.scales[i]))))
+            return TOA_ENULL;
+    if (bytes && !workspace) return TOA_ENULL;
     if (workspace_bytes < (size_t)bytes || ((uintptr_t)workspace & 255)) return TOA_EWORKSPACE;
     // (every launch of every batch is checked against the grid's limits before the first goes out)
     for (const Batch &b : batches)
@@ -594,7 +662,8 @@ int run(const Call &call, size_t num, const void *workspace, size_t workspace_by
             if (padded(s.s) / 64 * (padded(s.w) / 64) * (int64_t)b.mats.size() >
                 std::numeric_limits<int>::max())
                 return TOA_ESIZE;
-    for (const Batch &b : batches) TRY(Run(call, b, bounds).go());
+    for (const SmallBatch &b : smalls) TRY(runSmall(call, b, series));
+    for (const Batch &b : batches) TRY(Run(call, b, series).go());
     return 0;
 }
 
@@ -604,10 +673,11 @@ size_t workspaceOf(int dtype, size_t num, const int64_t *rows, const int64_t *co
     int64_t bytes = 0;
     try {
         std::vector<Batch> batches;
+        std::vector<SmallBatch> smalls;
         rc = dtype != TOA_F32 && dtype != TOA_F16 && dtype != TOA_BF16 ? TOA_EDTYPE
              : steps < 1 || steps > kMaxSteps                        ? TOA_EVALUE
              : num && (!rows || !cols)                               ? TOA_ENULL
-                                       : plan(num, rows, cols, steps, backward, batches, bytes);
+                                       : plan(num, rows, cols, steps, backward, batches, smalls, bytes);
     } catch (...) {
         rc = (int)hipErrorOutOfMemory;
     }
