@@ -14,6 +14,13 @@
 // (Where c is zero or tiny beside b: S = X X^T, P = c S S + b S + a I, N = c (M S + S M) + b M, with
 // that third matrix.)
 //
+// Two steps at once, where X is wide: the S of the next step is P S P, so X itself is needed once:
+//     S = X X^T,  P = c S S + b S + a I,  T = P S,  S' = T P + h I,  P' = c S' S' + (a - b h / 2) I,
+//     Q = P' P,   X'' = Q X
+// takes 3 w + 5 s instead of 6 w + 2 s (times s^2).  It is no less accurate than two single steps as
+// long as the first S is kept without h: there X X^T is small beside h I, whose rounding would pass
+// through T.  (Three at once lose: P S P magnifies the error of S by a^2.)
+//
 // Operands.  The matrix cores multiply halves; an operand element is kept as hi + lo, two halves
 // that together carry 22 bits, and a product is hi hi + hi lo + lo hi with float32 sums (what is
 // dropped, lo lo, is 2^-22 of it).  Halves have few exponents, so every matrix is stored times a
@@ -67,7 +74,8 @@ struct MatNorm {
 struct Group {         // matrices of one shape
     int64_t base;      // bytes from the workspace to the first one's region
     int64_t stride;    // bytes from one region to the next
-    int s, w, mat0, tile0, tiles;  // tiles: per matrix, of this launch
+    int s, w, mat0;
+    int tile0, tiles, all;  // workgroups of this launch: first, per matrix, of all its matrices
 };
 
 struct Shapes {
@@ -192,10 +200,16 @@ __device__ inline float scaleOf(unsigned long long peak) {
     return (float)(__longlong_as_double((long long)peak) / 127.0);
 }
 
-__device__ inline int codeOf(double v, float scale) {
+// v / scale rounded half to even: the multiple that v times the reciprocal suggests, set right by its
+// exact remainder (a division for every element costs the pass over a momentum 2.5 times its time).
+__device__ inline int codeOf(double v, float scale, double reciprocal) {
     if (!(scale > 0.f)) return 0;
+    double q = __builtin_rint(v * reciprocal);
+    const double rest = __builtin_fma(-q, (double)scale, v), half = 0.5 * (double)scale;
+    const bool odd = ((int)q & 1) != 0;
+    if (rest > half || (rest == half && odd)) q += 1.0;
+    if (rest < -half || (rest == -half && odd)) q -= 1.0;
     // (a scale too small for float32's normal range may be rounded to half of peak / 127)
-    const double q = __builtin_rint(v / (double)scale);
     return (int)(q > 127.0 ? 127.0 : q < -127.0 ? -127.0 : q);
 }
 
@@ -263,9 +277,10 @@ __device__ double sumPass(const MatRec &r, const StepArgs &a, int64_t from, int6
                     peak = mag > peak ? mag : peak;
                 }
                 const float scale = scaleOf(blockPeak(peak));
+                const double reciprocal = 1.0 / (double)scale;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
-                    c[i] = (int8_t)codeOf(d[i], scale);
+                    c[i] = (int8_t)codeOf(d[i], scale, reciprocal);
                     m[i] = (float)c[i] * scale;
                 }
                 if (valid == 8 && ((uintptr_t)codes & 7) == 0) {
@@ -324,6 +339,7 @@ struct Factor {
 
 struct Series {
     int steps, square;              // square: S carries h
+    int paired;                     // so many steps are taken by twos
     float a, b, c;
     double eps, h;
     double x[kMaxSteps + 1];        // bound of |X_k| from a start of norm 1
@@ -390,6 +406,27 @@ __device__ inline MatNorm normOf(const Bounds &b, double size) {
     return {ldexp(1.0 / plus, expOf(b.x(0))), ldexp(1.0, expOf(b.y(b.q.steps))), size, plus};
 }
 
+// Factors of a step: 4 of its own, so 8 of a pair's; in the gradient 3 more, behind all of those.
+constexpr int kStepFactors = 4;
+
+// The factors of the stages of steps t and t + 1 taken at once: f[0..6] for S, P, T, S', P', Q, X''.
+__device__ inline void pairFactors(const Bounds &b, int t, Factor *f) {
+    const Series &q = b.q;
+    const double x = b.x(t), x2 = x * x, x1 = b.x(t + 1), r = b.table.r[t], r1 = b.table.r[t + 1];
+    const int ex = expOf(x), es = expOf(x2), ep = expOf(r), et = expOf(r * x2), eq = expOf(r * r1);
+    const int es1 = expOf(q.square ? fmax(fabs(q.h), fabs(q.h + x1 * x1)) : x1 * x1), ep1 = expOf(r1);
+    const int ex2 = t + 2 == q.steps ? 0 : expOf(b.x(t + 2));
+    const double unit = q.square ? (double)q.a - (double)q.b * q.h * 0.5 : (double)q.a;
+    f[0] = {ldexpf(1.f, es - 2 * ex), 0.f, 1.f, 0.f};
+    f[1] = {ldexpf(q.c, ep - 2 * es), ldexpf(q.b, ep - es), 1.f, ldexpf(q.a, ep)};
+    f[2] = {ldexpf(1.f, et - ep - es), 0.f, 1.f, 0.f};
+    f[3] = {ldexpf(1.f, es1 - et - ep), 0.f, 1.f, (float)(q.square ? ldexp(q.h, es1) : 0.0)};
+    f[4] = {ldexpf(q.c, ep1 - 2 * es1), q.square ? 0.f : ldexpf(q.b, ep1 - es1), 1.f,
+            (float)ldexp(unit, ep1)};
+    f[5] = {ldexpf(1.f, eq - ep1 - ep), 0.f, 1.f, 0.f};
+    f[6] = {ldexpf(1.f, ex2 - eq - ex), 0.f, 1.f, 0.f};
+}
+
 // The factors of step t's stages: f[0..2] for S, P, X'; back[0..2] (or null) for M, N, Y.
 __device__ inline void stepFactors(const Bounds &b, int t, Factor *f, Factor *back) {
     const Series &q = b.q;
@@ -427,8 +464,13 @@ __global__ __launch_bounds__(256) void factors_kernel(FactorArgs a) {
     const Bounds b(a.q, table, size, ysize);
     if (t == 0) a.norms[mat] = normOf(b, size);
     if (t >= a.q.steps) return;
-    Factor *f = a.factors + (int64_t)mat * a.stages + 3 * t;
-    stepFactors(b, t, f, a.parts_y ? f + 3 * a.q.steps : nullptr);
+    Factor *f = a.factors + (int64_t)mat * a.stages + kStepFactors * t;
+    if (t >= a.q.paired)
+        stepFactors(b, t, f,
+                    a.parts_y ? a.factors + (int64_t)mat * a.stages + kStepFactors * a.q.steps + 3 * t
+                              : nullptr);
+    else if (t % 2 == 0)
+        pairFactors(b, t, f);
 }
 
 // ---- operands ----------------------------------------------------------------------------------
@@ -499,10 +541,42 @@ __device__ inline float element(const MatRec &r, const StepArgs &a, int64_t at) 
     return v;
 }
 
-// G (or the step's U, or the cotangent) -> the operand and its transpose, by tiles of 64 x 64.
+// Eight elements of G (U, the cotangent), consecutive in memory from `at` on.
+template <typename T, int KIND>
+__device__ inline void elements8(const MatRec &r, const StepArgs &a, int64_t at, int valid, float (&v)[8]) {
+    load8((const T *)(KIND == kPackAux ? r.aux : r.g) + at, valid, v);
+    if (KIND < kPackM) return;
+    float m[8];
+    if (KIND == kPackMI8) {
+        const int8_t *p = (const int8_t *)r.aux + at;
+        int8_t c[8];
+        if (valid >= 8 && ((uintptr_t)p & 7) == 0) {
+            unpack8(*global<int64_t>(p), c);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) c[i] = i < valid ? global<int8_t>(p)[i] : (int8_t)0;
+        }
+        // (they lie in one block, or in two)
+        const int64_t last = at + (valid < 8 ? valid : 8) - 1;
+        const float s0 = global<float>(r.scales)[at >> 7], s1 = global<float>(r.scales)[last >> 7];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) m[i] = (float)c[i] * ((at + i) >> 7 == at >> 7 ? s0 : s1);
+    } else if (KIND == kPackMF32) {
+        load8((const float *)r.aux + at, valid, m);
+    } else {
+        load8((const T *)r.aux + at, valid, m);
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        v[i] = a.nesterov ? __builtin_fmaf((float)a.momentum, m[i], a.sign * v[i]) : m[i];
+}
+
+// G (or the step's U, or the cotangent) -> the operand and its transpose, by tiles of 64 x 64.  Eight
+// elements that are neighbours in memory are eight columns of one of the two and go there at once;
+// the other is made through LDS.  HBM-bound: 4 bytes (bfloat16 and its momentum) in, 8 out.
 template <typename T, int KIND>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
-    __shared__ float tile[64][65];
+    __shared__ float tile[64][65];  // [operand row or column][the other]
     int t = blockIdx.x, mat;
     const int gi = findGroup(a.sh, t, mat);
     const Group &g = a.sh.g[gi];
@@ -513,32 +587,46 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     const int i0 = t / across * 64, j0 = t % across * 64;
     const double scale = KIND == kPackAux ? a.norms[mat].y_scale : a.norms[mat].x_scale;
     const int64_t rs = KIND == kPackAux ? r.aux_rs : r.g_rs, cs = KIND == kPackAux ? r.aux_cs : r.g_cs;
-    const bool by_rows = cs <= rs;  // lanes run along the smaller stride
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll 4
-    for (int q = wave; q < 64; q += 4) {
-        const int di = by_rows ? q : lane, dj = by_rows ? lane : q;
-        const int i = i0 + di, j = j0 + dj;
-        float v = 0.f;
-        if (i < g.s && j < g.w) v = (float)((double)element<T, KIND>(r, a.step, i * rs + j * cs) * scale);
-        tile[di][dj] = v;
+    // "lines" run along the smaller stride: rows of the operand, or (turned) its columns
+    const bool by_rows = cs <= rs;
+    const int64_t along = by_rows ? cs : rs, across_lines = by_rows ? rs : cs;
+    const int lines = by_rows ? g.s : g.w, length = by_rows ? g.w : g.s;
+    const int line0 = by_rows ? i0 : j0, at0 = by_rows ? j0 : i0;
+    const int64_t ld = rowBytes(padded(g.w), a.split), ld_t = rowBytes(padded(g.s), a.split);
+    char *const direct = region + (by_rows ? a.off[gi] : a.off_t[gi]);
+    char *const turned = region + (by_rows ? a.off_t[gi] : a.off[gi]);
+    const int64_t direct_ld = by_rows ? ld : ld_t, turned_ld = by_rows ? ld_t : ld;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int q = half * 256 + threadIdx.x, d = q >> 3, c = (q & 7) * 8;
+        const int line = line0 + d, valid = line < lines ? length - at0 - c : 0;
+        float v[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = 0.f;
+        if (valid > 0) {
+            const int64_t at = line * across_lines + (at0 + c) * along;
+            if (along == 1) {
+                elements8<T, KIND>(r, a.step, at, valid, v);
+            } else {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (i < valid) v[i] = element<T, KIND>(r, a.step, at + i * along);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = i < valid ? (float)((double)v[i] * scale) : 0.f;
+        }
+        if (line < lines) storeOperand(direct + line * direct_ld, at0 + c, v, a.split);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) tile[d][c + i] = v[i];
     }
     __syncthreads();
-    const int64_t sp = padded(g.s), wp = padded(g.w);
-    const int64_t ld = rowBytes(wp, a.split), ld_t = rowBytes(sp, a.split);
-    for (int q = threadIdx.x; q < 512; q += 256) {
-        const int d = q >> 3, c = (q & 7) * 8;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+        const int q = half * 256 + threadIdx.x, d = q >> 3, c = (q & 7) * 8;
         float v[8];
-        if (i0 + d < g.s) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = tile[d][c + i];
-            storeOperand(region + a.off[gi] + (i0 + d) * ld, j0 + c, v, a.split);
-        }
-        if (j0 + d < g.w) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) v[i] = tile[c + i][d];
-            storeOperand(region + a.off_t[gi] + (j0 + d) * ld_t, i0 + c, v, a.split);
-        }
+        for (int i = 0; i < 8; ++i) v[i] = tile[c + i][d];
+        if (at0 + d < length) storeOperand(turned + (at0 + d) * turned_ld, line0 + c, v, a.split);
     }
 }
 
@@ -576,7 +664,7 @@ __device__ inline f32x16 mfma(half8 a, half8 b, f32x16 c) {
 __device__ inline void beforeMatrix() { __builtin_amdgcn_sched_barrier(0); }
 __device__ inline void afterMatrix() {
     __builtin_amdgcn_sched_barrier(0);
-    asm volatile("s_nop 7");
+    asm volatile("s_nop 3");
     __builtin_amdgcn_sched_barrier(0);
 }
 
@@ -593,11 +681,18 @@ __device__ inline void tileOf(int t, int across, bool symmetric, int &ti, int &t
     }
 }
 
-// Consecutive tiles go to one XCD (workgroups are dealt to the eight in turn), so that the tiles of
-// a matrix share an L2.
-__device__ inline int tileForWorkgroup(int b, int total) {
-    const int xcd = b & 7, q = total >> 3, r = total & 7;
-    return xcd * q + (xcd < r ? xcd : r) + (b >> 3);
+// The group, matrix and tile of a workgroup of the product.  Workgroups are dealt to the eight XCDs in
+// turn; each of them gets an eighth of every group, in one run, so that the tiles of a matrix share
+// an L2 and no XCD gets more of the long tiles than the others.
+__device__ inline int findTile(const Shapes &sh, int &tile, int &mat) {
+    int k = 0;
+    while (k + 1 < sh.n && tile >= sh.g[k + 1].tile0) ++k;
+    tile -= sh.g[k].tile0;
+    const int total = sh.g[k].all, xcd = tile & 7, q = total >> 3, r = total & 7;
+    tile = xcd * q + (xcd < r ? xcd : r) + (tile >> 3);
+    mat = tile / sh.g[k].tiles;
+    tile -= mat * sh.g[k].tiles;
+    return k;
 }
 
 // 16 bytes for each lane from global memory straight into LDS: the wave's 1 KiB from `lds` on.
@@ -636,8 +731,8 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void gemm_kernel(GemmArgs a) {
     static_assert((NW == 1 || NW % 2 == 0) && BM % 32 == 0, "the permutation of a load's rows");
     __shared__ __attribute__((aligned(16))) char lds_[kLds];
 
-    int t = tileForWorkgroup(blockIdx.x, gridDim.x), mat;
-    const int gi = findGroup(a.sh, t, mat);
+    int t = blockIdx.x, mat;
+    const int gi = findTile(a.sh, t, mat);
     const Product &p = a.p[gi];
     char *region = a.ws + a.sh.g[gi].base + mat * a.sh.g[gi].stride;
     mat += a.sh.g[gi].mat0;
@@ -1591,9 +1686,10 @@ template <typename T> __global__ __launch_bounds__(256) void quantize_kernel(Blo
         peak = m > peak ? m : peak;
     }
     const float scale = scaleOf(blockPeak(peak));
+    const double reciprocal = 1.0 / (double)scale;
     int8_t c[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) c[i] = (int8_t)codeOf((double)v[i], scale);
+    for (int i = 0; i < 8; ++i) c[i] = (int8_t)codeOf((double)v[i], scale, reciprocal);
     int8_t *o = (int8_t *)a.out[k] + e;
     if (valid == 8 && ((uintptr_t)o & 7) == 0) {
         *global<int64_t>((void *)o) = pack8(c);

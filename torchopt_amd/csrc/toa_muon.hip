@@ -25,8 +25,8 @@ int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 // Where one matrix's buffers lie in its region.
 struct Layout {
-    int64_t x[kMaxSteps + 1], xt[kMaxSteps + 1], s[kMaxSteps], p[kMaxSteps];
-    int64_t y[2], yt[2], m, n, yf, bytes;
+    int64_t x[kMaxSteps + 1], xt[kMaxSteps + 1], s[kMaxSteps], p[kMaxSteps];  // (gradient: step by step)
+    int64_t t, y[2], yt[2], m, n, yf, bytes;
 };
 
 Layout layoutOf(int s, int w, int steps, bool backward) {
@@ -56,9 +56,12 @@ Layout layoutOf(int s, int w, int steps, bool backward) {
         const int64_t x0 = take(s, w), x0t = take(w, s);
         const int64_t x1 = steps > 1 ? take(s, w) : 0, x1t = steps > 1 ? take(w, s) : 0;
         const int64_t ss = take(s, s), pp = take(s, s);
-        for (int k = 0; k < steps; ++k) {
+        l.t = take(s, s);
+        for (int k = 0; k <= steps; ++k) {
             l.x[k] = k & 1 ? x1 : x0;
             l.xt[k] = k & 1 ? x1t : x0t;
+        }
+        for (int k = 0; k < steps; ++k) {
             l.s[k] = ss;
             l.p[k] = pp;
         }
@@ -82,6 +85,8 @@ struct Batch {
 struct Head {
     int64_t recs, norms, parts, parts_y, factors, regions;
 };
+
+int stagesOf(int steps, bool backward) { return (kStepFactors + (backward ? 3 : 0)) * steps; }
 
 Head headOf(int64_t mats, int stages) {
     Head h;
@@ -144,7 +149,10 @@ int plan(size_t num, const int64_t *rows, const int64_t *cols, int steps, bool b
     auto key = [&](size_t i) {
         return std::make_pair(std::min(rows[i], cols[i]), std::max(rows[i], cols[i]));
     };
-    std::stable_sort(order.begin(), order.end(), [&](size_t i, size_t j) { return key(i) < key(j); });
+    // (long rows first: their tiles take longest and should not be what a launch ends with)
+    std::stable_sort(order.begin(), order.end(), [&](size_t i, size_t j) {
+        return std::make_pair(key(i).second, key(i).first) > std::make_pair(key(j).second, key(j).first);
+    });
     Layout lay{};
     for (size_t k = 0; k < order.size(); ++k) {
         const auto shape = key(order[k]);
@@ -163,9 +171,8 @@ int plan(size_t num, const int64_t *rows, const int64_t *cols, int steps, bool b
         b->mats.push_back(order[k]);
         b->bytes += lay.bytes;
     }
-    const int stages = 3 * steps * (backward ? 2 : 1);
     for (const Batch &b : batches)
-        bytes = std::max(bytes, headOf((int64_t)b.mats.size(), stages).regions + b.bytes);
+        bytes = std::max(bytes, headOf((int64_t)b.mats.size(), stagesOf(steps, backward)).regions + b.bytes);
     return 0;
 }
 
@@ -343,15 +350,19 @@ class Run {
   public:
     Run(const Call &c, const Batch &b, const Series &series)
         : c_(c), b_(b), steps_(c.series.steps), back_(c.what == kBackward),
-          stages_(3 * steps_ * (back_ ? 2 : 1)), head_(headOf((int64_t)b.mats.size(), stages_)),
-          f_{series} {}
+          stages_(stagesOf(steps_, back_)), head_(headOf((int64_t)b.mats.size(), stages_)),
+          f_{series} {
+        f_.q.paired = pairedSteps();
+    }
 
     int go() {
         TRY(fillRecords(c_, b_.mats, (MatRec *)(c_.ws + head_.recs)));
         TRY(sums());
         TRY(factors());
         TRY(pack(back_ ? 0 : -1));
-        for (int k = 0; k < steps_; ++k) TRY(forwardStep(k));
+        int from = 0;  // which of the two buffers holds X
+        for (int k = 0; k < f_.q.paired; k += 2, from ^= 1) TRY(forwardPair(k, from));
+        for (int k = f_.q.paired; k < steps_; ++k, from ^= 1) TRY(forwardStep(k, back_ ? k : from));
         if (!back_) return 0;
         for (int k = steps_ - 1; k >= 0; --k) TRY(backwardStep(k));
         return tail();
@@ -359,7 +370,20 @@ class Run {
 
   private:
     // whether step k's operands carry 22 bits (see the header)
-    bool split(int k) const { return back_ || c_.dtype != TOA_BF16 || k < steps_ - 2; }
+    bool split(int k) const {
+        return back_ || c_.dtype != TOA_BF16 || k < f_.q.paired || k < steps_ - 2;
+    }
+
+    // Steps taken by twos: where that is less work for the batch (see muon_kernels.hpp).
+    int pairedSteps() const {
+        double one = 0.0, two = 0.0;  // of two steps
+        for (const auto &s : b_.shapes) {
+            const double n = (double)s.count * s.s * s.s;
+            one += n * (6.0 * s.w + 2.0 * s.s);
+            two += n * (3.0 * s.w + 5.0 * s.s);
+        }
+        return !back_ && two < 0.95 * one ? steps_ / 2 * 2 : 0;
+    }
 
     const MatRec *recs() const { return (const MatRec *)(c_.ws + head_.recs); }
 
@@ -370,7 +394,8 @@ class Run {
         for (int k = 0; k < sh.n; ++k) {
             const auto &s = b_.shapes[k];
             const int64_t tiles = tilesOf(s, k);
-            sh.g[k] = {head_.regions + s.base, s.lay.bytes, s.s, s.w, s.mat0, (int)at, (int)tiles};
+            sh.g[k] = {head_.regions + s.base, s.lay.bytes, s.s, s.w, s.mat0,
+                       (int)at, (int)tiles, (int)(tiles * s.count)};
             at += tiles * s.count;
             if (at > std::numeric_limits<int>::max()) return at;
         }
@@ -477,7 +502,7 @@ class Run {
         const bool tensor = mode == kToTensor || mode == kToParam;
         return withType(tensor ? c_.dtype : TOA_F32, [&](auto t) {
             using T = decltype(t);
-            switch (pickTiles(a)) {
+            switch (pickTiles(a, sp)) {
                 case kTiles256:
                     return sp ? tiles<T, 256, 2, 4, 1, 2, true>(a) : tiles<T, 256, 2, 4, 1, 2, false>(a);
                 case kTiles128Pair:
@@ -503,15 +528,22 @@ class Run {
     // most out of a full chip (1.4 PFLOP/s of half products in 256 x 256, 0.9 in 64 x 64), small
     // ones start and end sooner and spread few results over more of it (a product of one 1024^2
     // matrix: 72 us in 256 x 256, 34 in 128 x 128, 15 in 64 x 64; of sixteen: 115, 145, 220).
-    int pickTiles(const GemmArgs &a) const {
+    int pickTiles(const GemmArgs &a, bool split_in) const {
         struct Variant {
             int size, at_once;  // tiles that the whole chip holds
             double alone, alone_piece, full, full_piece;
         };
-        static const Variant variants[kVariants] = {{256, 256, 18.0, 1.69, 39.0, 2.3},
-                                                    {128, 512, 10.3, 0.70, 26.0, 1.45},
-                                                    {128, 256, 8.3, 0.56, 2.0, 1.03},
-                                                    {64, 256, 7.6, 0.20, 7.6, 0.22}};
+        // with 22-bit operands, and with halves
+        static const Variant table[2][kVariants] = {
+            {{256, 256, 18.0, 1.69, 39.0, 2.3},
+             {128, 512, 10.3, 0.70, 26.0, 1.45},
+             {128, 256, 8.3, 0.56, 2.0, 1.03},
+             {64, 256, 7.6, 0.20, 7.6, 0.22}},
+            {{256, 256, 14.0, 1.4, 22.0, 2.3},
+             {128, 512, 9.0, 0.62, 13.0, 1.45},
+             {128, 256, 7.5, 0.50, 3.3, 1.03},
+             {64, 256, 7.6, 0.20, 7.1, 0.22}}};
+        const Variant *variants = table[!split_in];
         int best = 0;
         double least = 0.0;
         for (int k = 0; k < kVariants; ++k) {
@@ -545,35 +577,89 @@ class Run {
                       c_.stream, a);
     }
 
-    int forwardStep(int k) {
-        const bool sp = split(k), last = k + 1 == steps_;
-        TRY(product(3 * k, k, sp, true, kToOperand, [&](Product &p, const Layout &l, int, int ld_w) {
-            p.a0 = p.b0 = l.x[k];
-            p.lda = p.ldb = ld_w;
-            p.d = p.dt = l.s[k];
-        }));
-        TRY(product(3 * k + 1, k, sp, true, kToOperand, [&](Product &p, const Layout &l, int ld_s, int) {
-            p.a0 = p.b0 = l.s[k];
-            if (!f_.q.square) p.e = l.s[k];
-            p.lda = p.ldb = ld_s;
-            p.d = p.dt = l.p[k];
-        }));
-        if (last && back_) return 0;  // the result itself is not needed
-        const int mode = !last ? kToOperand : c_.hyper && c_.hyper->apply ? kToParam : kToTensor;
-        return product(3 * k + 2, k, last || split(k + 1), false, mode,
+    // How the last product leaves.
+    int lastMode() const { return c_.hyper && c_.hyper->apply ? kToParam : kToTensor; }
+
+    // X' (or X'') = by(layout) X, from one buffer of X to another.
+    template <typename F> int advance(int stage, int k, int next, int from, int to, F by) {
+        const bool last = next == steps_;
+        return product(stage, k, last || split(next), false, last ? lastMode() : kToOperand,
                        [&](Product &p, const Layout &l, int ld_s, int) {
-                           p.a0 = l.p[k];
-                           p.b0 = l.xt[k];
+                           p.a0 = by(l);
+                           p.b0 = l.xt[from];
                            p.lda = p.ldb = ld_s;
                            if (!last) {
-                               p.d = l.x[k + 1];
-                               p.dt = l.xt[k + 1];
+                               p.d = l.x[to];
+                               p.dt = l.xt[to];
                            }
                        });
     }
 
+    // A product of symmetric matrices that is symmetric itself.
+    template <typename F> int symmetric(int stage, int k, F operands) {
+        return product(stage, k, split(k), true, kToOperand,
+                       [&](Product &p, const Layout &l, int ld_s, int) {
+                           p.lda = p.ldb = ld_s;
+                           operands(p, l);
+                           p.dt = p.d;
+                       });
+    }
+
+    int gram(int stage, int k, int from) {
+        return product(stage, k, split(k), true, kToOperand,
+                       [&](Product &p, const Layout &l, int, int ld_w) {
+                           p.a0 = p.b0 = l.x[from];
+                           p.lda = p.ldb = ld_w;
+                           p.d = p.dt = l.s[k];
+                       });
+    }
+
+    int forwardStep(int k, int from) {
+        const int stage = kStepFactors * k;
+        TRY(gram(stage, k, from));
+        TRY(symmetric(stage + 1, k, [&](Product &p, const Layout &l) {
+            p.a0 = p.b0 = l.s[k];
+            if (!f_.q.square) p.e = l.s[k];
+            p.d = l.p[k];
+        }));
+        if (back_ && k + 1 == steps_) return 0;  // the result itself is not needed
+        return advance(stage + 2, k, k + 1, from, back_ ? k + 1 : from ^ 1,
+                       [&](const Layout &l) { return l.p[k]; });
+    }
+
+    // Two steps (S, P, T, S', P', Q, X''); S' takes S's place, P' T's, and Q that of S'.
+    int forwardPair(int k, int from) {
+        const int stage = kStepFactors * k;
+        TRY(gram(stage, k, from));
+        TRY(symmetric(stage + 1, k, [&](Product &p, const Layout &l) {
+            p.a0 = p.b0 = p.e = l.s[k];
+            p.d = l.p[k];
+        }));
+        TRY(symmetric(stage + 2, k, [&](Product &p, const Layout &l) {
+            p.a0 = l.p[k];
+            p.b0 = l.s[k];
+            p.d = l.t;
+        }));
+        TRY(symmetric(stage + 3, k, [&](Product &p, const Layout &l) {
+            p.a0 = l.t;
+            p.b0 = l.p[k];
+            p.d = l.s[k];
+        }));
+        TRY(symmetric(stage + 4, k, [&](Product &p, const Layout &l) {
+            p.a0 = p.b0 = l.s[k];
+            if (!f_.q.square) p.e = l.s[k];
+            p.d = l.t;
+        }));
+        TRY(symmetric(stage + 5, k, [&](Product &p, const Layout &l) {
+            p.a0 = l.t;
+            p.b0 = l.p[k];
+            p.d = l.s[k];
+        }));
+        return advance(stage + 6, k, k + 2, from, from ^ 1, [&](const Layout &l) { return l.s[k]; });
+    }
+
     int backwardStep(int k) {
-        const int from = (steps_ - 1 - k) & 1, stage = 3 * steps_ + 3 * k;
+        const int from = (steps_ - 1 - k) & 1, stage = kStepFactors * steps_ + 3 * k;
         TRY(product(stage, k, true, true, kToOperand, [&](Product &p, const Layout &l, int, int ld_w) {
             p.a0 = p.b1 = l.y[from];
             p.b0 = p.a1 = l.x[k];
