@@ -14,6 +14,8 @@ underneath are one code path.
     torch.ops.torchopt_amd.forward_multi_ / fused_step_multi_(lists..., count, ...)  -> None
     torch.ops.torchopt_amd.count_advance_ / forward_multi_devcount_ /
         fused_step_multi_devcount_(..., bias_rows, first_count, count_tensor, ...)   -> None
+    torch.ops.torchopt_amd.orthogonalize_multi / orthogonalize_backward_multi(lists...) -> Tensor[]
+    torch.ops.torchopt_amd.muon_fused_step_multi_ / muon_forward_multi_(lists..., ...)  -> None
 
 In-place operators return nothing (an operator's outputs may not alias its inputs); `dispatch`
 below gives every function the calling convention of its pybind11 twin and picks the registered
@@ -23,12 +25,12 @@ microseconds of dispatcher time per call, which an eager per-leaf loop would fee
 
 from __future__ import annotations
 
-from typing import List, Tuple
+from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
 
-from torchopt_amd._C import adam_op
+from torchopt_amd._C import adam_op, muon_op
 
 _NS = 'torchopt_amd'
 
@@ -140,6 +142,63 @@ def _fused_step_multi_devcount_(params: List[Tensor], updates: List[Tensor], mu:
                                        first_count, count, lr, maximize=maximize,
                                        write_updates=write_updates, weight_decay=weight_decay,
                                        decoupled=decoupled)
+
+
+# ---- matrix-shaped parameters ---------------------------------------------------------------
+
+
+@_define('orthogonalize_multi')
+def _orthogonalize_multi(inputs: List[Tensor], steps: int, coefficients: List[float],
+                         eps: float) -> List[Tensor]:
+    return muon_op.orthogonalize_multi(inputs, steps, coefficients, eps)
+
+
+@_define('orthogonalize_backward_multi')
+def _orthogonalize_backward_multi(grads: List[Tensor], inputs: List[Tensor], steps: int,
+                                  coefficients: List[float], eps: float) -> List[Tensor]:
+    return muon_op.orthogonalize_backward_multi(grads, inputs, steps, coefficients, eps)
+
+
+_orthogonalize_multi.register_fake(
+    lambda inputs, steps, coefficients, eps: [torch.empty_like(x) for x in inputs])
+_orthogonalize_backward_multi.register_fake(
+    lambda grads, inputs, steps, coefficients, eps: [torch.empty_like(x) for x in inputs])
+
+
+def _orthogonalize_setup(ctx, inputs, output):
+    matrices, *ctx.series = inputs
+    ctx.save_for_backward(*matrices)
+
+
+def _orthogonalize_backward(ctx, grads):
+    grads = [torch.zeros_like(x) if g is None else g for g, x in zip(grads, ctx.saved_tensors)]
+    out = torch.ops.torchopt_amd.orthogonalize_backward_multi(grads, list(ctx.saved_tensors),
+                                                              *ctx.series)
+    return out, None, None, None
+
+
+_orthogonalize_multi.register_autograd(_orthogonalize_backward,
+                                       setup_context=_orthogonalize_setup)
+
+
+@_define('muon_forward_multi_', ('updates', 'mu', 'scales'))
+def _muon_forward_multi_(updates: List[Tensor], mu: List[Tensor], scales: List[Tensor],
+                         momentum: float, nesterov: bool, steps: int, coefficients: List[float],
+                         eps: float, adjust_lr_fn: Optional[str]) -> None:
+    muon_op.forward_multi_(updates, mu, scales or None, momentum, nesterov=nesterov, steps=steps,
+                           coefficients=coefficients, eps=eps, adjust_lr_fn=adjust_lr_fn)
+
+
+@_define('muon_fused_step_multi_', ('params', 'mu', 'scales'))
+def _muon_fused_step_multi_(params: List[Tensor], updates: List[Tensor], mu: List[Tensor],
+                            scales: List[Tensor], momentum: float, lr: float, nesterov: bool,
+                            weight_decay: float, maximize: bool, steps: int,
+                            coefficients: List[float], eps: float,
+                            adjust_lr_fn: Optional[str]) -> None:
+    muon_op.fused_step_multi_(params, updates, mu, scales or None, momentum, lr,
+                              nesterov=nesterov, weight_decay=weight_decay, maximize=maximize,
+                              steps=steps, coefficients=coefficients, eps=eps,
+                              adjust_lr_fn=adjust_lr_fn)
 
 
 # ---- one calling convention for both routes -------------------------------------------------

@@ -34,6 +34,9 @@ except ImportError as exc:  # no fallback module: the op is the compiled extensi
 
 from torch.autograd.function import once_differentiable
 
+# the same functions, visible to torch.compile while it traces
+from torchopt_amd.accelerated_op import library  # noqa: E402, F401
+
 
 __all__ = ['COEFFICIENTS', 'dequantize_blocks', 'orthogonalize', 'quantize_blocks']
 
@@ -113,7 +116,10 @@ def orthogonalize(
     grad = torch.is_grad_enabled()
     for ks in _by_kind(tensors) if tensors else []:
         group = [tensors[k] for k in ks]
-        if grad and any(t.requires_grad for t in group):
+        if torch.compiler.is_compiling():
+            fresh = torch.ops.torchopt_amd.orthogonalize_multi(group, series[0], list(series[1]),
+                                                               series[2])
+        elif grad and any(t.requires_grad for t in group):
             fresh = _Orthogonalize.apply(series, *group)
         else:
             fresh = muon_op.orthogonalize_multi(group, *series)

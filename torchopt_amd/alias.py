@@ -16,6 +16,8 @@ place so gradients flow, and with one fused list call per transformation in plac
 the transformations and keeps one state per transformation; `apply_updates`
 (/root/reference/torchopt/update.py:50-81) adds updates to parameters.
 
+`muon` is the same chain with `scale_by_muon` for matrices; the reference has no counterpart.
+
 Trees are plain containers (``None`` is a leaf), flattened by `torchopt_amd._tree`: flat lists,
 tuples and dicts of tensors directly, anything else with ``torch.utils._pytree``.
 """
@@ -28,12 +30,13 @@ from typing import Any, Callable, NamedTuple
 
 import torch
 
-from torchopt_amd._tree import flatten, leaves_like, rebuild
+from torchopt_amd._tree import DictSpec, flatten, leaves_like, rebuild
 from torchopt_amd.base import GradientTransformation, accelerated_only
 from torchopt_amd.transform.scale_by_adam import _inc_counts, _remember, scale_by_accelerated_adam
+from torchopt_amd.transform.scale_by_muon import COEFFICIENTS, scale_by_muon
 
 
-__all__ = ['adam', 'adamw', 'apply_updates', 'chain']
+__all__ = ['adam', 'adamw', 'apply_updates', 'chain', 'muon']
 
 
 class EmptyState(NamedTuple):
@@ -249,6 +252,84 @@ def adamw(
     return chain(
         _flip_sign_and_add_weight_decay(0.0, maximize),
         scale_by_accelerated_adam(b1, b2, eps, eps_root, moment_requires_grad),
+        _add_decayed_weights(weight_decay, mask),
+        _scale_by_neg_lr(lr),
+    )
+
+
+class MatrixPartitionState(NamedTuple):
+    """States of the transformation for matrices and of the one for the other leaves, each over
+    the flat list of all leaves with None in the place of the other's, and the names in their order
+    if the parameters were a flat dict."""
+
+    matrices: Any
+    others: Any
+    keys: Any
+
+
+def _by_dimensions(matrices: GradientTransformation,
+                   others: GradientTransformation) -> GradientTransformation:
+    """Leaves of two dimensions or more through one transformation, the rest through the other."""
+
+    def split(leaves, is_matrix):
+        return ([x if m else None for x, m in zip(leaves, is_matrix)],
+                [None if m else x for x, m in zip(leaves, is_matrix)])
+
+    def init_fn(params):
+        leaves, spec = flatten(params)
+        ms, os = split(leaves, [t is not None and t.dim() >= 2 for t in leaves])
+        return MatrixPartitionState(matrices=matrices.init(ms), others=others.init(os),
+                                    keys=spec.keys if type(spec) is DictSpec else None)
+
+    def update_fn(updates, state, *, params=None, inplace=True):
+        leaves, spec = flatten(updates)
+        if state.keys is not None and type(spec) is DictSpec and spec.keys != state.keys:
+            # the same names in another order: line the gradients up with the state
+            spec = DictSpec(spec.kind, state.keys)
+            leaves = leaves_like(updates, spec)
+        is_matrix = [m is not None for m in state.matrices.momentum]
+        if len(is_matrix) != len(leaves):
+            raise ValueError('updates and optimizer state have different tree structures; '
+                             'make sure `init` was called on matching parameters')
+        ms, os = split(leaves, is_matrix)
+        ms, m_state = matrices.update(ms, state.matrices, params=params, inplace=inplace)
+        os, o_state = others.update(os, state.others, params=params, inplace=inplace)
+        merged = [m if flag else o for m, o, flag in zip(ms, os, is_matrix)]
+        return (rebuild(merged, updates, spec),
+                MatrixPartitionState(matrices=m_state, others=o_state, keys=state.keys))
+
+    return GradientTransformation(init_fn, update_fn)
+
+
+def muon(
+    lr=1e-3,
+    weight_decay: float = 0.1,
+    momentum: float = 0.95,
+    nesterov: bool = True,
+    ns_coefficients: tuple[float, float, float] = COEFFICIENTS,
+    eps: float = 1e-7,
+    ns_steps: int = 5,
+    adjust_lr_fn: str | None = None,
+    *,
+    adam_betas: tuple[float, float] = (0.9, 0.95),
+    adam_eps: float = 1e-8,
+    adam_eps_root: float = 0.0,
+    mask: Any = None,
+    moment_requires_grad: bool = False,
+    maximize: bool = False,
+    momentum_dtype: torch.dtype | None = None,
+) -> GradientTransformation:
+    """Functional Muon: matrices (leaves of two dimensions or more) through `scale_by_muon`, all
+    other leaves through the accelerated Adam, then decoupled weight decay and the learning rate,
+    which are the same for both (``adjust_lr_fn='match_rms_adamw'`` gives matrices updates of
+    Adam's size)."""
+    _check(lr, *adam_betas, adam_eps, weight_decay)
+    return chain(
+        _flip_sign_and_add_weight_decay(0.0, maximize),
+        _by_dimensions(
+            scale_by_muon(momentum, nesterov, ns_steps, ns_coefficients, eps, adjust_lr_fn,
+                          moment_requires_grad, momentum_dtype),
+            scale_by_accelerated_adam(*adam_betas, adam_eps, adam_eps_root, moment_requires_grad)),
         _add_decayed_weights(weight_decay, mask),
         _scale_by_neg_lr(lr),
     )

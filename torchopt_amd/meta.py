@@ -18,7 +18,7 @@ from torchopt_amd import alias
 from torchopt_amd.base import accelerated_only
 
 
-__all__ = ['MetaAdam', 'MetaAdamW']
+__all__ = ['MetaAdam', 'MetaAdamW', 'MetaMuon']
 
 
 class _MetaOptimizer:
@@ -91,3 +91,20 @@ class MetaAdamW(_MetaOptimizer):
                                              mask=mask,
                                              moment_requires_grad=moment_requires_grad,
                                              maximize=maximize))
+
+
+class MetaMuon(_MetaOptimizer):
+    """Differentiable Muon over a module's parameters (`alias.muon`: its vectors and scalars are
+    stepped by the accelerated Adam).  The outer gradient flows through every Newton-Schulz step;
+    `adam_eps_root` keeps Adam's part of it finite, as in `MetaAdam`."""
+
+    def __init__(self, module: nn.Module, lr=1e-3, weight_decay: float = 0.0,
+                 momentum: float = 0.95, nesterov: bool = True,
+                 ns_coefficients=alias.COEFFICIENTS, eps: float = 1e-7, ns_steps: int = 5,
+                 adjust_lr_fn=None, *, adam_betas=(0.9, 0.95), adam_eps: float = 1e-8,
+                 adam_eps_root: float = 0.0, mask=None, moment_requires_grad: bool = True,
+                 maximize: bool = False) -> None:
+        super().__init__(module, alias.muon(
+            lr, weight_decay, momentum, nesterov, ns_coefficients, eps, ns_steps, adjust_lr_fn,
+            adam_betas=adam_betas, adam_eps=adam_eps, adam_eps_root=adam_eps_root, mask=mask,
+            moment_requires_grad=moment_requires_grad, maximize=maximize))
