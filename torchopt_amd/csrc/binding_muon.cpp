@@ -162,17 +162,24 @@ bool sameOrder(const Tensor &a, const Tensor &b) {
     return true;
 }
 
-// No element that the call writes may be written twice or read as something else.
-void requireApart(const char *name, std::vector<std::pair<char *, char *>> &spans) {
-    std::sort(spans.begin(), spans.end());
-    for (size_t k = 1; k < spans.size(); ++k)
-        TORCH_CHECK(spans[k].first >= spans[k - 1].second, name,
-                    ": tensors that are written overlap (is one of them given twice?)");
-}
+struct Span {
+    char *from, *to;
+    bool written;
+    Span(const Tensor &t, bool written)
+        : from((char *)t.data_ptr()), to(from + (size_t)t.numel() * t.element_size()),
+          written(written) {}
+};
 
-std::pair<char *, char *> spanOf(const Tensor &t) {
-    char *p = (char *)t.data_ptr();
-    return {p, p + (size_t)t.numel() * t.element_size()};
+// No element that the call writes may be written twice or be read as something else.
+void requireApart(const char *name, std::vector<Span> &spans) {
+    std::sort(spans.begin(), spans.end(), [](const Span &a, const Span &b) { return a.from < b.from; });
+    char *any = nullptr, *written = nullptr;  // how far what came before reaches
+    for (const Span &s : spans) {
+        TORCH_CHECK(s.from >= (s.written ? any : written), name,
+                    ": a tensor that is written overlaps another one (is it given twice?)");
+        any = std::max(any, s.to);
+        if (s.written) written = std::max(written, s.to);
+    }
 }
 
 void touch(const Tensor &t) {
@@ -213,7 +220,7 @@ void stepMulti(const char *name, const TensorList &out, TensorList grads, const 
     std::vector<int64_t> rows(out.size()), cols(out.size());
     std::vector<toa_muon_view> vo(out.size()), vg(out.size()), vm(out.size());
     std::vector<float *> vs(out.size(), nullptr);
-    std::vector<std::pair<char *, char *>> spans;
+    std::vector<Span> spans;
     for (size_t k = 0; k < out.size(); ++k) {
         TORCH_CHECK(mu[k].device() == out[0].device() && mu[k].scalar_type() == kept, name,
                     ": the momentum must live on ", out[0].device(), " with one scalar type, ", kept);
@@ -234,12 +241,12 @@ void stepMulti(const char *name, const TensorList &out, TensorList grads, const 
                         name, ": scales must be contiguous Float tensors on ", out[0].device(),
                         " with one element for each 128 of their momentum");
             vs[k] = s.data_ptr<float>();
-            if (s.numel()) spans.push_back(spanOf(s));
+            if (s.numel()) spans.emplace_back(s, true);
         }
         if (out[k].numel()) {
-            spans.push_back(spanOf(out[k]));
-            spans.push_back(spanOf(mu[k]));
-            if (grads[k].data_ptr() != out[k].data_ptr()) spans.push_back(spanOf(grads[k]));
+            spans.emplace_back(out[k], true);
+            spans.emplace_back(mu[k], true);
+            if (hyper.apply) spans.emplace_back(grads[k], false);
         }
     }
     requireApart(name, spans);
@@ -324,7 +331,7 @@ py::object dequantizeMulti(const py::object &out_o, const py::object &codes_o,
     std::vector<const float *> src_scales;
     std::vector<size_t> n;
     std::vector<void *> dst;
-    std::vector<std::pair<char *, char *>> spans;
+    std::vector<Span> spans;
     for (size_t k = 0; k < out.size(); ++k) {
         requireDense(name, "out", out[k]);
         TORCH_CHECK(codes[k].device() == out[0].device() && codes[k].scalar_type() == at::kChar &&
@@ -340,7 +347,10 @@ py::object dequantizeMulti(const py::object &out_o, const py::object &codes_o,
         src_scales.push_back((const float *)scales[k].data_ptr());
         n.push_back((size_t)out[k].numel());
         dst.push_back(out[k].data_ptr());
-        if (n.back()) spans.push_back(spanOf(out[k]));
+        if (!n.back()) continue;
+        spans.emplace_back(out[k], true);
+        spans.emplace_back(codes[k], false);
+        spans.emplace_back(scales[k], false);
     }
     requireApart(name, spans);
     const OnDeviceOf dev(out[0]);

@@ -200,17 +200,21 @@ __device__ inline float scaleOf(unsigned long long peak) {
     return (float)(__longlong_as_double((long long)peak) / 127.0);
 }
 
-// v / scale rounded half to even: the multiple that v times the reciprocal suggests, set right by its
-// exact remainder (a division for every element costs the pass over a momentum 2.5 times its time).
+// v / scale rounded half to even: the multiple that v times the reciprocal suggests and, where that
+// lies next to a border, its exact remainder decides.
 __device__ inline int codeOf(double v, float scale, double reciprocal) {
     if (!(scale > 0.f)) return 0;
-    double q = __builtin_rint(v * reciprocal);
-    const double rest = __builtin_fma(-q, (double)scale, v), half = 0.5 * (double)scale;
-    const bool odd = ((int)q & 1) != 0;
-    if (rest > half || (rest == half && odd)) q += 1.0;
-    if (rest < -half || (rest == -half && odd)) q -= 1.0;
+    const double t = v * reciprocal;
+    double q = __builtin_rint(t);
+    if (__builtin_fabs(t - q) > 0.499999) {
+        const double rest = __builtin_fma(-q, (double)scale, v), half = 0.5 * (double)scale;
+        const bool odd = ((int)q & 1) != 0;
+        if (rest > half || (rest == half && odd)) q += 1.0;
+        if (rest < -half || (rest == -half && odd)) q -= 1.0;
+    }
     // (a scale too small for float32's normal range may be rounded to half of peak / 127)
-    return (int)(q > 127.0 ? 127.0 : q < -127.0 ? -127.0 : q);
+    const int code = (int)q;
+    return code > 127 ? 127 : code < -127 ? -127 : code;
 }
 
 __device__ inline void unpack8(int64_t v, int8_t (&c)[8]) {
@@ -312,7 +316,7 @@ __device__ double sumPass(const MatRec &r, const StepArgs &a, int64_t from, int6
             }
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum += (double)v[i] * (double)v[i];
+        for (int i = 0; i < 8; ++i) sum = __builtin_fma((double)v[i], (double)v[i], sum);
     }
     return sum;
 }
@@ -443,7 +447,9 @@ __device__ inline void stepFactors(const Bounds &b, int t, Factor *f, Factor *ba
     if (!back) return;
     const double y1 = b.y(t + 1);
     const int ey1 = expOf(y1), ey = t ? expOf(b.y(t)) : 0;
-    const int em = expOf(2.0 * x * y1), en = expOf((ab + 2.0 * ac * x2) * 2.0 * x * y1);
+    // (where N X is nothing beside P Y, N needs no more range than to be added to it)
+    const int em = expOf(2.0 * x * y1);
+    const int en = min(expOf((ab + 2.0 * ac * x2) * 2.0 * x * y1), ep + ey1 - ex + 24);
     back[0] = {ldexpf(1.f, em - ey1 - ex), 0.f, 1.f, 0.f};
     back[1] = {ldexpf(q.c, en - em - es), ldexpf(add, en - em), 1.f, 0.f};
     back[2] = {ldexpf(1.f, ey - en - ex), 0.f, ldexpf(1.f, (en + ex) - (ep + ey1)), 0.f};

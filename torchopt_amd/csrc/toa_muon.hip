@@ -219,19 +219,19 @@ int boundsOf(const toa_muon_series &q, Series &f) {
     f.c = (float)q.c;
     f.eps = q.eps;
     f.steps = q.steps;
-    double x = 1.0, top = 1.0;
+    double x = 1.0;
     for (int k = 0; k <= q.steps; ++k) {
         f.x[k] = 1.01 * x;
-        top = std::max(top, f.x[k]);
         if (k == q.steps) break;
         f.r[k] = std::max(1.01 * largest(q.a, q.b, q.c, 0, f.x[k]), 1e-3);
         f.d[k] = std::max(1.01 * largest(q.a, 3.0 * q.b, 5.0 * q.c, 0, f.x[k]), 1e-3);
         x = std::max(largest(q.a, q.b, q.c, 1, f.x[k]), 1e-6);
         if (!(x <= 1048576.0)) return TOA_EVALUE;
     }
-    // completing the square costs accuracy where h is large beside X X^T (at most x^2)
+    // completing the square takes c h^2 away from what (X X^T + h I)^2 brings in: a bit of a or so
+    // at most
     f.h = q.c != 0.0 ? q.b / (2.0 * q.c) : 0.0;
-    f.square = q.c != 0.0 && std::fabs(f.h) <= 4.0 * top * top;
+    f.square = q.c != 0.0 && std::fabs(q.c) * f.h * f.h <= 2.0 * std::fabs(q.a);
     return 0;
 }
 
