@@ -674,17 +674,32 @@ __device__ inline void afterMatrix() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
-// Row and column of tile number t: row-major, or the lower triangle of a symmetric result.
-__device__ inline void tileOf(int t, int across, bool symmetric, int &ti, int &tj) {
-    if (symmetric) {
-        ti = (int)((__builtin_sqrtf(8.f * (float)t + 1.f) - 1.f) * 0.5f);
-        while (ti * (ti + 1) / 2 > t) --ti;
-        while ((ti + 1) * (ti + 2) / 2 <= t) ++ti;
-        tj = t - ti * (ti + 1) / 2;
+// Row and column of tile number t, of all or of the lower triangle of a symmetric result: by bands
+// of four rows, down the columns of each.  So a run of tiles is as square as can be, and an XCD reads
+// few rows of both operands.
+__device__ inline void tileOf(int t, int down, int across, bool symmetric, int &ti, int &tj) {
+    constexpr int kBand = 4;
+    int band;
+    if (symmetric) {  // band b has kBand^2 b tiles left of its triangle, and begins at 8 b^2 + 2 b
+        band = (int)((__builtin_sqrtf(8.f * (float)t + 1.f) - 1.f) * (1.f / 8.f));
+        while (8 * band * band + 2 * band > t) --band;
+        while (8 * (band + 1) * (band + 1) + 2 * (band + 1) <= t) ++band;
+        t -= 8 * band * band + 2 * band;
+        across = kBand * band;
     } else {
-        ti = t / across;
-        tj = t - ti * across;
+        band = t / (kBand * across);
+        t -= band * kBand * across;
     }
+    const int rows = down - kBand * band < kBand ? down - kBand * band : kBand;
+    tj = t / rows;
+    ti = t - tj * rows;
+    if (symmetric && tj >= across) {
+        t -= rows * across;
+        for (tj = 0; t >= rows - tj; ++tj) t -= rows - tj;
+        ti = tj + t;
+        tj += across;
+    }
+    ti += kBand * band;
 }
 
 // The group, matrix and tile of a workgroup of the product.  Workgroups are dealt to the eight XCDs in
@@ -743,7 +758,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void gemm_kernel(GemmArgs a) {
     char *region = a.ws + a.sh.g[gi].base + mat * a.sh.g[gi].stride;
     mat += a.sh.g[gi].mat0;
     int ti, tj;
-    tileOf(t, (p.cols + BN - 1) / BN, a.symmetric, ti, tj);
+    tileOf(t, (p.rows + BM - 1) / BM, (p.cols + BN - 1) / BN, a.symmetric, ti, tj);
     const int i0 = ti * BM, j0 = tj * BN;
     const int lane = threadIdx.x & 63;
     const int whole = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
