@@ -29,9 +29,11 @@
 // element is at most the spectral norm, so nothing overflows, and what lies 2^-24 below the bound
 // still has all its bits.  ("half" operands keep hi alone: 11 bits.)
 //
-// Layout.  A row of an operand is a run of 128-byte pieces: [32 hi | 32 lo] of 32 columns, or 64
-// halves of 64 columns.  Either way one piece of each row is what a tile step consumes.  Columns
-// beyond the matrix are zero up to a multiple of 64.
+// Layout.  An operand lies the way the matrix instructions read it: by blocks of 32 rows, and in
+// them by pieces of 4 KiB, [32 hi | 32 lo] of 32 columns or 64 halves of 64 columns of each row.  A
+// piece is eight chunks of eight columns, 16 bytes of every row, rows next to each other: two chunks
+// are the 1 KiB that the lanes of a wave hold for one instruction.  Columns beyond the matrix are
+// zero up to a multiple of 64; rows beyond it, up to a multiple of 32, hold anything.
 #pragma once
 
 #include <hip/hip_runtime.h>
@@ -42,6 +44,9 @@
 namespace toa_muon {
 
 typedef _Float16 half8 __attribute__((ext_vector_type(8)));
+typedef _Float16 half4 __attribute__((ext_vector_type(4)));
+typedef unsigned u32x2 __attribute__((ext_vector_type(2)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
@@ -50,6 +55,7 @@ constexpr int kMaxSteps = 32;
 constexpr int kMaxParts = 256;   // partial sums per matrix
 constexpr int kBlock = 128;      // elements of an 8-bit block
 constexpr int kPiece = 128;      // bytes of a row that one tile step consumes
+constexpr int kRows = 32;        // rows of a block of an operand
 constexpr int kPad = 64;         // columns are padded to a multiple of this
 
 // What a kernel needs to know of the caller's tensors, in the wide orientation.
@@ -481,34 +487,29 @@ __global__ __launch_bounds__(256) void factors_kernel(FactorArgs a) {
 
 // ---- operands ----------------------------------------------------------------------------------
 
-// Eight consecutive columns (a multiple of 8) of an operand row.
-__device__ inline void storeOperand(char *row, int col, const float (&v)[8], bool split) {
+// Where eight consecutive columns, from a multiple of 8 on, of a row of an operand lie; `ld` is the
+// bytes of a row.  Their low halves follow 2 KiB behind.
+__device__ inline char *chunkOf(char *operand, int64_t ld, int row, int col, bool split) {
+    const int piece = split ? col >> 5 : col >> 6, chunk = split ? (col >> 3) & 3 : (col >> 3) & 7;
+    return operand + (int64_t)(row / kRows) * kRows * ld + (int64_t)piece * kRows * kPiece +
+           chunk * 512 + row % kRows * 16;
+}
+
+__device__ inline void storeOperand(char *to, const float (&v)[8], bool split) {
     half8 hi, lo;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         hi[i] = (_Float16)v[i];
         lo[i] = (_Float16)(v[i] - (float)hi[i]);
     }
-    if (split) {
-        char *p = row + (col >> 5) * kPiece + (col & 31) * 2;
-        *(half8 *)p = hi;
-        *(half8 *)(p + 64) = lo;
-    } else {
-        *(half8 *)(row + col * 2) = hi;
-    }
+    *global<half8>(to) = hi;
+    if (split) *global<half8>(to + 2048) = lo;
 }
 
-__device__ inline void loadOperand(const char *row, int col, float (&v)[8], bool split) {
-    if (split) {
-        const char *p = row + (col >> 5) * kPiece + (col & 31) * 2;
-        const half8 hi = *(const half8 *)p, lo = *(const half8 *)(p + 64);
+__device__ inline void loadOperand(const char *from, float (&v)[8]) {  // 22-bit operands only
+    const half8 hi = *global<half8>(from), lo = *global<half8>(from + 2048);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)hi[i] + (float)lo[i];
-    } else {
-        const half8 hi = *(const half8 *)(row + col * 2);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = (float)hi[i];
-    }
+    for (int i = 0; i < 8; ++i) v[i] = (float)hi[i] + (float)lo[i];
 }
 
 // Bytes of an operand row of `cols` padded columns.
@@ -621,18 +622,19 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = i < valid ? (float)((double)v[i] * scale) : 0.f;
         }
-        if (line < lines) storeOperand(direct + line * direct_ld, at0 + c, v, a.split);
+        if (line < lines) storeOperand(chunkOf(direct, direct_ld, line, at0 + c, a.split), v, a.split);
 #pragma unroll
         for (int i = 0; i < 8; ++i) tile[d][c + i] = v[i];
     }
     __syncthreads();
 #pragma unroll
     for (int half = 0; half < 2; ++half) {
-        const int q = half * 256 + threadIdx.x, d = q >> 3, c = (q & 7) * 8;
+        const int q = half * 256 + threadIdx.x, d = q & 63, c = (q >> 6) * 8;
         float v[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = tile[c + i][d];
-        if (at0 + d < length) storeOperand(turned + (at0 + d) * turned_ld, line0 + c, v, a.split);
+        if (at0 + d < length)
+            storeOperand(chunkOf(turned, turned_ld, at0 + d, line0 + c, a.split), v, a.split);
     }
 }
 
@@ -730,31 +732,31 @@ template <int N, bool BARRIER = true> __device__ inline void arrive() {
         asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(N) : "memory");
 }
 
-// Tile BM x BN by WM x WN waves.  A stage of LDS holds one 128-byte piece of every row of both
-// operands; STAGES of them are in flight, filled by loads that bypass the registers.  The 16-byte
-// chunks of a row are permuted (chunk ^ row / 2 % 8): sixteen lanes of a 16-byte read, which go down
-// the rows, then touch each of the 64 banks once.
+// Tile BM x BN by WM x WN waves.  A stage of LDS holds one piece of every row of both operands; STAGES
+// of them are in flight, filled by loads that bypass the registers.  In LDS an operand lies as in
+// memory, so a wave's read of two chunks is 1 KiB in a row.
 //
-// KS > 1 (one wave to a tile) splits the sum instead: each of KS waves takes every KS-th piece
-// through stages of its own, without a barrier, and the partial sums are added through LDS, always
-// in the same order.
+// KS > 1 (one wave to a tile) splits the sum instead: each of KS waves takes every KS-th piece and the
+// partial sums are added through LDS, always in the same order.  No wave shares what it reads with
+// another, so nothing goes through LDS: the pieces go from memory to the registers that the
+// instructions read, kAhead of them in flight.  (Through LDS a step of a wave took 0.86 us, waiting
+// for reads that one wave on a SIMD cannot hide; this way .)
 template <typename T, int BM, int BN, int WM, int WN, int KS, int STAGES, bool SPLIT>
 __global__ __launch_bounds__(WM *WN *KS * 64) void gemm_kernel(GemmArgs a) {
     constexpr int NW = WM * WN;                          // waves that share a stage
     constexpr int TM = BM / WM / 32, TN = BN / WN / 32;  // 32 x 32 results per wave
-    constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;    // loads of 8 rows, per wave and stage
     constexpr int kStage = (BM + BN) * kPiece;
     constexpr int kScratch = 32 * 36 * 4;                // per wave, for the stores
-    constexpr bool kShared = NW > 1;
-    constexpr int kLds = STAGES * kStage * KS > NW * KS * kScratch ? STAGES * kStage * KS
-                                                                   : NW * KS * kScratch;
+    constexpr int kMain = KS > 1 ? KS * KS * 4096 : STAGES * kStage;
+    constexpr int kLds = kMain > NW * KS * kScratch ? kMain : NW * KS * kScratch;
     static_assert(KS == 1 || (NW == 1 && TM * TN == KS), "one block of the sum for each wave");
-    static_assert((NW == 1 || NW % 2 == 0) && BM % 32 == 0, "the permutation of a load's rows");
-    __shared__ __attribute__((aligned(16))) char lds_[kLds];
+    __shared__ __attribute__((aligned(16))) char lds[kLds];
 
     int t = blockIdx.x, mat;
     const int gi = findTile(a.sh, t, mat);
-    const Product &p = a.p[gi];
+    Product p = a.p[gi];
+    // (read now, all at once: what only the stores need would be waited for there, one by one)
+    asm volatile("" : "+s"(p.d), "+s"(p.dt), "+s"(p.e), "+s"(p.ldd), "+s"(p.lddt), "+s"(p.rows), "+s"(p.cols));
     char *region = a.ws + a.sh.g[gi].base + mat * a.sh.g[gi].stride;
     mat += a.sh.g[gi].mat0;
     int ti, tj;
@@ -763,7 +765,6 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void gemm_kernel(GemmArgs a) {
     const int lane = threadIdx.x & 63;
     const int whole = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int wave = KS > 1 ? 0 : whole, part = KS > 1 ? whole : 0;
-    char *const lds = lds_ + part * STAGES * kStage;
     const int wi = wave / WN * (BM / WM), wj = wave % WN * (BN / WN);
     const Factor f = a.factors[(int64_t)mat * a.stages + a.stage];
 
@@ -775,23 +776,8 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void gemm_kernel(GemmArgs a) {
 #pragma unroll
             for (int q = 0; q < 16; ++q) acc[i][j][q] = 0.f;
 
-    // Where a lane's chunks come from, relative to the tile's first row (a row of both pairs has
-    // the same length).  Rows beyond the matrix repeat its last one; what comes of them is not
-    // stored.
-    auto chunk = [&](int group) { return ((lane & 7) ^ ((group & 1) * 4 + (lane >> 4))) << 4; };
-    unsigned from_a[LA], from_b[LB];
-#pragma unroll
-    for (int q = 0; q < LA; ++q) {
-        const int row = (q * NW + wave) * 8 + (lane >> 3);
-        from_a[q] = (unsigned)(i0 + row < p.rows ? row : p.rows - 1 - i0) * (unsigned)p.lda +
-                    chunk(q * NW + wave);
-    }
-#pragma unroll
-    for (int q = 0; q < LB; ++q) {
-        const int row = (q * NW + wave) * 8 + (lane >> 3);
-        from_b[q] = (unsigned)(j0 + row < p.cols ? row : p.cols - 1 - j0) * (unsigned)p.ldb +
-                    chunk(q * NW + wave);
-    }
+    // Blocks of rows beyond the matrix repeat its last one; what comes of them is not stored.
+    const int last_a = (p.rows - 1) / kRows - i0 / kRows, last_b = (p.cols - 1) / kRows - j0 / kRows;
     const char *const a0 = region + p.a0 + (int64_t)i0 * p.lda;
     const char *const b0 = region + p.b0 + (int64_t)j0 * p.ldb;
     const char *const a1 = region + p.a1 + (int64_t)i0 * p.lda;
@@ -803,64 +789,10 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void gemm_kernel(GemmArgs a) {
     auto from_piece = [&](int k) {
         k = part + KS * k;
         const bool second = k >= steps0;
-        const int64_t at = (int64_t)(second ? k - steps0 : k) * kPiece;
+        const int64_t at = (int64_t)(second ? k - steps0 : k) * (kRows * kPiece);
         A = (second ? a1 : a0) + at;
         B = (second ? b1 : b0) + at;
     };
-    auto load = [&](int q, int stage) {
-        char *to = lds + stage * kStage;
-        if (q < LA)
-            loadToLds(A + from_a[q < LA ? q : 0], to + (q * NW + wave) * 1024);
-        else
-            loadToLds(B + from_b[q < LA ? 0 : q - LA], to + BM * kPiece + ((q - LA) * NW + wave) * 1024);
-    };
-    // Phases of TM * TN matrix instructions.  The registers of a phase are read from LDS during the
-    // one before.  Before a step's last phase everybody has read the stage and the next one is
-    // waited for; the last phase's instructions cover the first reads from that one, and the loads
-    // that refill the stage go out in the last phase and the kShares - 1 that follow it.
-    constexpr int kShares = SPLIT ? 3 : 2, L = LA + LB, kFirst = (L + kShares - 1) / kShares;
-    half8 ah[2][TM], bh[2][TN], al[SPLIT ? TM : 1], bl[SPLIT ? TN : 1];
-    auto frag = [&](const char *from, int row, int c) {
-        row += lane & 31;
-        c += lane >> 5;
-        return *(const half8 *)(from + row * kPiece + ((c ^ (row >> 1 & 7)) << 4));
-    };
-    auto read_a = [&](const char *from, half8 *to, int c) {
-#pragma unroll
-        for (int i = 0; i < TM; ++i) to[i] = frag(from, wi + 32 * i, c);
-    };
-    auto read_b = [&](const char *from, half8 *to, int c) {
-#pragma unroll
-        for (int j = 0; j < TN; ++j) to[j] = frag(from, BM + wj + 32 * j, c);
-    };
-    auto multiply = [&](const half8 *x, const half8 *y) {
-        beforeMatrix();
-#pragma unroll
-        for (int i = 0; i < TM; ++i)
-#pragma unroll
-            for (int j = 0; j < TN; ++j) acc[i][j] = mfma(x[i], y[j], acc[i][j]);
-        afterMatrix();
-    };
-
-    // share number `share` of the loads of the piece that `from_piece` chose
-    auto refill = [&](int share, int stage) {
-#pragma unroll
-        for (int q = 0; q < L; ++q)
-            if (q / kFirst == share) load(q, stage);
-    };
-#pragma unroll
-    for (int k = 0; k < STAGES; ++k) {
-        if (k >= steps) break;
-        from_piece(k);
-#pragma unroll
-        for (int share = 0; share < (k == STAGES - 1 ? 1 : kShares); ++share) refill(share, k);
-    }
-    if (steps >= STAGES)
-        arrive<(STAGES - 2) * L + kFirst, kShared>();
-    else
-        arrive<0, kShared>();
-    read_a(lds, ah[0], 0);
-    read_b(lds, bh[0], 0);
     // before the second pair's first product
     bool turned_sum = all == steps0;
     auto turn = [&] {
@@ -870,195 +802,362 @@ __global__ __launch_bounds__(WM *WN *KS * 64) void gemm_kernel(GemmArgs a) {
             for (int j = 0; j < TN; ++j) acc[i][j] *= f.turn;
         turned_sum = true;
     };
-    int stage = 0;
-    for (int k = 0; k < steps; ++k) {
-        const char *const here = lds + stage * kStage;
-        const int next = stage == STAGES - 1 ? 0 : stage + 1;
-        const int before = stage == 0 ? STAGES - 1 : stage - 1;  // being refilled
-        const bool filling = k + STAGES - 1 < steps;
-        if (!turned_sum && part + KS * k >= steps0) turn();
-        __builtin_amdgcn_sched_barrier(0);
-        if (SPLIT) {
-            read_a(here, al, 4);
-            if (filling) refill(1, before);
-            multiply(ah[0], bh[0]);
-            read_b(here, bl, 4);
-            if (filling) refill(2, before);
-            multiply(al, bh[0]);
-            read_a(here, ah[1], 2);
-            read_b(here, bh[1], 2);
-            multiply(ah[0], bl);
-            read_a(here, al, 6);
-            multiply(ah[1], bh[1]);
-            read_b(here, bl, 6);
-            multiply(al, bh[1]);
+
+    if constexpr (KS > 1) {
+        constexpr int kAhead = STAGES;
+        unsigned from_a[TM], from_b[TN];
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+            from_a[i] = (unsigned)(i < last_a ? i : last_a) * (unsigned)(kRows * p.lda) + lane * 16;
+#pragma unroll
+        for (int j = 0; j < TN; ++j)
+            from_b[j] = (unsigned)(j < last_b ? j : last_b) * (unsigned)(kRows * p.ldb) + lane * 16;
+        half8 xa[kAhead][TM][4], xb[kAhead][TN][4];  // chunks 0 2 4 6 of a piece
+        auto fetch = [&](int k, int to) {
+            from_piece(k);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i) xa[to][i][q] = *global<half8>(A + from_a[i] + q * 1024);
+#pragma unroll
+                for (int j = 0; j < TN; ++j) xb[to][j][q] = *global<half8>(B + from_b[j] + q * 1024);
+            }
+        };
+        auto multiply = [&](int k, int from) {
+            if (!turned_sum && part + KS * k >= steps0) turn();
+            auto each = [&](int q, int r) {
+#pragma unroll
+                for (int i = 0; i < TM; ++i)
+#pragma unroll
+                    for (int j = 0; j < TN; ++j)
+                        acc[i][j] = mfma(xa[from][i][q], xb[from][j][r], acc[i][j]);
+            };
+            beforeMatrix();
+            each(0, 0);
+            each(1, 1);
+            if (SPLIT) {
+                each(2, 0);
+                each(3, 1);
+                each(0, 2);
+                each(1, 3);
+            } else {
+                each(2, 2);
+                each(3, 3);
+            }
+            afterMatrix();
+        };
+        // (whole rounds have no condition inside and are reached by one way only, so that the waits
+        // are for the oldest loads alone)
+        if (steps >= kAhead) {
+#pragma unroll
+            for (int d = 0; d < kAhead; ++d) fetch(d, d);
+            int k = 0;
+            for (; k + 2 * kAhead <= steps; k += kAhead) {
+#pragma unroll
+                for (int d = 0; d < kAhead; ++d) {
+                    multiply(k + d, d);
+                    fetch(k + d + kAhead, d);
+                }
+            }
+#pragma unroll
+            for (int d = 0; d < 2 * kAhead - 1; ++d) {
+                if (d >= kAhead && k + d >= steps) break;
+                multiply(k + d, d % kAhead);
+                if (d < kAhead - 1 && k + d + kAhead < steps) fetch(k + d + kAhead, d);
+            }
         } else {
-            read_a(here, ah[1], 2);
-            read_b(here, bh[1], 2);
-            if (filling) refill(1, before);
-            multiply(ah[0], bh[0]);
-            read_a(here, ah[0], 4);
-            read_b(here, bh[0], 4);
-            multiply(ah[1], bh[1]);
-            read_a(here, ah[1], 6);
-            read_b(here, bh[1], 6);
-            multiply(ah[0], bh[0]);
+#pragma unroll
+            for (int d = 0; d < kAhead - 1; ++d)
+                if (d < steps) fetch(d, d);
+#pragma unroll
+            for (int d = 0; d < kAhead - 1; ++d)
+                if (d < steps) multiply(d, d);
         }
-        // (towards the end fewer pieces are in flight: everything is waited for)
-        if (filling)
-            arrive<(STAGES - 2) * L, kShared>();
-        else
-            arrive<0, kShared>();
-        read_a(lds + next * kStage, ah[0], 0);
-        read_b(lds + next * kStage, bh[0], 0);
-        if (k + STAGES < steps) {
-            from_piece(k + STAGES);
-            refill(0, stage);
+    } else {
+        constexpr int LA = BM / 8 / NW, LB = BN / 8 / NW;  // loads of 1 KiB, per wave and stage
+        unsigned from_a[LA], from_b[LB];
+#pragma unroll
+        for (int q = 0; q < LA; ++q) {
+            const int n = q * NW + wave, block = n / 4;
+            from_a[q] = (unsigned)(block < last_a ? block : last_a) * (unsigned)(kRows * p.lda) +
+                        n % 4 * 1024 + lane * 16;
         }
-        if (SPLIT)
-            multiply(ah[1], bl);
+#pragma unroll
+        for (int q = 0; q < LB; ++q) {
+            const int n = q * NW + wave, block = n / 4;
+            from_b[q] = (unsigned)(block < last_b ? block : last_b) * (unsigned)(kRows * p.ldb) +
+                        n % 4 * 1024 + lane * 16;
+        }
+        auto load = [&](int q, int stage) {
+            char *to = lds + stage * kStage;
+            if (q < LA)
+                loadToLds(A + from_a[q < LA ? q : 0], to + (q * NW + wave) * 1024);
+            else
+                loadToLds(B + from_b[q < LA ? 0 : q - LA],
+                          to + BM * kPiece + ((q - LA) * NW + wave) * 1024);
+        };
+        // Phases of TM * TN matrix instructions.  The registers of a phase are read from LDS during
+        // the one before.  Before a step's last phase everybody has read the stage and the next one
+        // is waited for; the last phase's instructions cover the first reads from that one, and the
+        // loads that refill the stage go out in the last phase and the kShares - 1 that follow it.
+        constexpr int kShares = SPLIT ? 3 : 2, L = LA + LB, kFirst = (L + kShares - 1) / kShares;
+        half8 ah[2][TM], bh[2][TN], al[SPLIT ? TM : 1], bl[SPLIT ? TN : 1];
+        auto read_a = [&](const char *from, half8 *to, int c) {
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+                to[i] = *(const half8 *)(from + (wi + 32 * i) * kPiece + c * 512 + lane * 16);
+        };
+        auto read_b = [&](const char *from, half8 *to, int c) {
+#pragma unroll
+            for (int j = 0; j < TN; ++j)
+                to[j] = *(const half8 *)(from + (BM + wj + 32 * j) * kPiece + c * 512 + lane * 16);
+        };
+        auto multiply = [&](const half8 *x, const half8 *y) {
+            beforeMatrix();
+#pragma unroll
+            for (int i = 0; i < TM; ++i)
+#pragma unroll
+                for (int j = 0; j < TN; ++j) acc[i][j] = mfma(x[i], y[j], acc[i][j]);
+            afterMatrix();
+        };
+        // share number `share` of the loads of the piece that `from_piece` chose
+        auto refill = [&](int share, int stage) {
+#pragma unroll
+            for (int q = 0; q < L; ++q)
+                if (q / kFirst == share) load(q, stage);
+        };
+#pragma unroll
+        for (int k = 0; k < STAGES; ++k) {
+            if (k >= steps) break;
+            from_piece(k);
+#pragma unroll
+            for (int share = 0; share < (k == STAGES - 1 ? 1 : kShares); ++share) refill(share, k);
+        }
+        if (steps >= STAGES)
+            arrive<(STAGES - 2) * L + kFirst>();
         else
-            multiply(ah[1], bh[1]);
-        stage = next;
+            arrive<0>();
+        read_a(lds, ah[0], 0);
+        read_b(lds, bh[0], 0);
+        int stage = 0;
+        for (int k = 0; k < steps; ++k) {
+            const char *const here = lds + stage * kStage;
+            const int next = stage == STAGES - 1 ? 0 : stage + 1;
+            const int before = stage == 0 ? STAGES - 1 : stage - 1;  // being refilled
+            const bool filling = k + STAGES - 1 < steps;
+            if (!turned_sum && k >= steps0) turn();
+            __builtin_amdgcn_sched_barrier(0);
+            if (SPLIT) {
+                read_a(here, al, 4);
+                if (filling) refill(1, before);
+                multiply(ah[0], bh[0]);
+                read_b(here, bl, 4);
+                if (filling) refill(2, before);
+                multiply(al, bh[0]);
+                read_a(here, ah[1], 2);
+                read_b(here, bh[1], 2);
+                multiply(ah[0], bl);
+                read_a(here, al, 6);
+                multiply(ah[1], bh[1]);
+                read_b(here, bl, 6);
+                multiply(al, bh[1]);
+            } else {
+                read_a(here, ah[1], 2);
+                read_b(here, bh[1], 2);
+                if (filling) refill(1, before);
+                multiply(ah[0], bh[0]);
+                read_a(here, ah[0], 4);
+                read_b(here, bh[0], 4);
+                multiply(ah[1], bh[1]);
+                read_a(here, ah[1], 6);
+                read_b(here, bh[1], 6);
+                multiply(ah[0], bh[0]);
+            }
+            // (towards the end fewer pieces are in flight: everything is waited for)
+            if (filling)
+                arrive<(STAGES - 2) * L>();
+            else
+                arrive<0>();
+            read_a(lds + next * kStage, ah[0], 0);
+            read_b(lds + next * kStage, bh[0], 0);
+            if (k + STAGES < steps) {
+                from_piece(k + STAGES);
+                refill(0, stage);
+            }
+            if (SPLIT)
+                multiply(ah[1], bl);
+            else
+                multiply(ah[1], bh[1]);
+            stage = next;
+        }
+        arrive<0>();
     }
     if (!turned_sum) turn();  // (a wave that had no piece of the second pair)
-    arrive<0>();
-    if (KS > 1) {
+    if constexpr (KS > 1) {
         // each wave adds up one block
-        f32x16 *const sums = (f32x16 *)lds_;
+        f32x4 *const sums = (f32x4 *)lds;
+        auto at = [&](int block, int from, int q) { return ((block * KS + from) * 4 + q) * 64 + lane; };
+#pragma unroll
+        for (int b = 0; b < KS; ++b) {
+            if (b == whole) continue;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const f32x16 &s = acc[b / TN][b % TN];
+                sums[at(b, whole, q)] = f32x4{s[4 * q], s[4 * q + 1], s[4 * q + 2], s[4 * q + 3]};
+            }
+        }
+        __syncthreads();
+        f32x16 sum, own;
 #pragma unroll
         for (int b = 0; b < KS; ++b)
-            if (b != whole) sums[(b * KS + whole) * 64 + lane] = acc[b / TN][b % TN];
-        arrive<0>();
-        f32x16 sum;
-#pragma unroll
-        for (int q = 0; q < 16; ++q) sum[q] = 0.f;
+            if (b == whole) own = acc[b / TN][b % TN];
 #pragma unroll
         for (int w = 0; w < KS; ++w) {
-            if (w == whole) {
 #pragma unroll
-                for (int b = 0; b < KS; ++b)
-                    if (b == whole) sum += acc[b / TN][b % TN];
-            } else {
-                sum += sums[(whole * KS + w) * 64 + lane];
+            for (int q = 0; q < 4; ++q) {
+                const f32x4 s = sums[at(whole, w == whole ? 0 : w, q)];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float v = w == whole ? own[4 * q + i] : s[i];
+                    sum[4 * q + i] = w ? sum[4 * q + i] + v : v;
+                }
             }
         }
 #pragma unroll
         for (int b = 0; b < KS; ++b)
             if (b == whole) acc[b / TN][b % TN] = sum;
-        arrive<0>();
+        __syncthreads();
     }
 
-    // Results leave by 32 x 32 blocks through LDS, eight to a lane: along rows for the result,
-    // along columns for its transpose.
-    float *box = (float *)(lds_ + whole * kScratch);
+    // Results leave by 32 x 32 blocks.  A lane has four times four neighbours of one column: halves of
+    // chunks of the transpose, which is stored as it is; by rows they go through LDS, as the two halves
+    // they end as.  (Instructions count here, up to eight blocks to a wave: what only some blocks need
+    // stands behind a branch.)
+    float *box = (float *)(lds + whole * kScratch);
     const MatRec &r = a.recs[mat];
     const bool tensor = a.mode == kToTensor || a.mode == kToParam;
     const bool turned = tensor && r.out_rs < r.out_cs;
+    const bool mirror = p.dt >= 0 && !(a.symmetric && ti == tj);
     for (int block = KS > 1 ? whole : 0; block < (KS > 1 ? whole + 1 : TM * TN); ++block) {
         const int bi = i0 + wi + block / TN * 32, bj = j0 + wj + block % TN * 32;
         if (bi >= p.rows && !(p.dt >= 0 && bi < padded(p.rows))) continue;
         if (bj >= p.cols && !(p.d >= 0 && bj < padded(p.cols))) continue;
-        // (registers are picked by number: every block writes its own, the rest is shared code)
+        const int col = bj + (lane & 31), row0 = bi + (lane >> 5) * 4;  // and rows (q / 4) * 8 + q % 4 on
+        // (registers are picked by number: every block has its own, the rest is shared code)
+        float v[16];
 #pragma unroll
         for (int i = 0; i < TM; ++i)
 #pragma unroll
             for (int j = 0; j < TN; ++j)
                 if (block == i * TN + j)
 #pragma unroll
-                    for (int q = 0; q < 16; ++q)
-                        box[((q >> 2) * 8 + (lane >> 5) * 4 + (q & 3)) * 36 + (lane & 31)] =
-                            acc[i][j][q];
+                    for (int q = 0; q < 16; ++q) v[q] = acc[i][j][q] * f.acc;
+        // (the third matrix is symmetric, so it can be read as the transpose is stored)
+        if (p.e >= 0 && col < p.cols) {
+            const char *from = chunkOf(region + p.e, p.lde, col, bi, SPLIT) + (lane >> 5) * 8;
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const half4 hi = *global<half4>(from + q * 512);
+                half4 lo = {};
+                if (SPLIT) lo = *global<half4>(from + q * 512 + 2048);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[4 * q + i] += f.add * ((float)hi[i] + (float)lo[i]);
+            }
+        }
+        if (bi == bj && f.diag != 0.f) {
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+                if (row0 + (q >> 2) * 8 + (q & 3) == col) v[q] += f.diag;
+        }
+        if (bi + 32 > p.rows || bj + 32 > p.cols) {
+#pragma unroll
+            for (int q = 0; q < 16; ++q)
+                if (row0 + (q >> 2) * 8 + (q & 3) >= p.rows || col >= p.cols) v[q] = 0.f;
+        }
+        const int box_at = (lane >> 5) * 4 * 36 + (lane & 31);
+        if (a.mode == kToOperand) {
+            unsigned u[16];  // low 16 bits: hi; high 16 bits: lo
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                const _Float16 hi = (_Float16)v[q];
+                const _Float16 lo = (_Float16)__builtin_fmaf((float)hi, -1.f, v[q]);
+                u[q] = __builtin_bit_cast(unsigned short, hi) |
+                       (unsigned)__builtin_bit_cast(unsigned short, lo) << 16;
+            }
+            auto his = [](unsigned x, unsigned y) { return __builtin_amdgcn_perm(y, x, 0x05040100); };
+            auto los = [](unsigned x, unsigned y) { return __builtin_amdgcn_perm(y, x, 0x07060302); };
+            if (mirror && col < p.cols) {
+                char *to = chunkOf(region + p.dt, p.lddt, col, bi, a.split_out) + (lane >> 5) * 8;
+#pragma unroll
+                for (int q = 0; q < 16; q += 4)
+                    *global<u32x2>(to + q * 128) = u32x2{his(u[q], u[q + 1]), his(u[q + 2], u[q + 3])};
+                if (a.split_out)
+#pragma unroll
+                    for (int q = 0; q < 16; q += 4)
+                        *global<u32x2>(to + q * 128 + 2048) =
+                            u32x2{los(u[q], u[q + 1]), los(u[q + 2], u[q + 3])};
+            }
+            if (p.d < 0) continue;
+            unsigned *const ubox = (unsigned *)box;
+#pragma unroll
+            for (int q = 0; q < 16; ++q) ubox[box_at + ((q >> 2) * 8 + (q & 3)) * 36] = u[q];
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            const int row = lane & 31, c = (lane >> 5) * 8;
+            char *to = chunkOf(region + p.d, p.ldd, bi + row, bj, a.split_out) + c * 64;
+            unsigned x[16];
+#pragma unroll
+            for (int q = 0; q < 16; ++q) x[q] = ubox[row * 36 + c + (q >> 3) * 16 + (q & 7)];
+            if (bi + row < p.rows) {
+#pragma unroll
+                for (int q = 0; q < 16; q += 8) {
+                    const unsigned *y = x + q;
+                    *global<u32x4>(to + q * 128) = u32x4{his(y[0], y[1]), his(y[2], y[3]),
+                                                         his(y[4], y[5]), his(y[6], y[7])};
+                    if (a.split_out)
+                        *global<u32x4>(to + q * 128 + 2048) = u32x4{los(y[0], y[1]), los(y[2], y[3]),
+                                                                    los(y[4], y[5]), los(y[6], y[7])};
+                }
+            }
+            __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+            __builtin_amdgcn_wave_barrier();
+            continue;
+        }
+#pragma unroll
+        for (int q = 0; q < 16; ++q) box[box_at + ((q >> 2) * 8 + (q & 3)) * 36] = v[q];
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            const int row = half * 16 + (lane >> 2), col = (lane & 3) * 8;
-            float v[8], e[8];
+            float x[8], e[8];
+            // eight neighbours of the caller's tensor, along the way it lies
+            const int line = half * 16 + (lane >> 2), c = (lane & 3) * 8;
+            const int row = bi + (turned ? c : line), column = bj + (turned ? line : c);
+            if (row >= p.rows || column >= p.cols) continue;
 #pragma unroll
-            for (int q = 0; q < 8; ++q) v[q] = box[row * 36 + col + q] * f.acc;
-            if (p.e >= 0 && bi + row < p.rows && bj + col < p.cols) {
-                loadOperand(region + p.e + (int64_t)(bi + row) * p.lde, bj + col, e, SPLIT);
-#pragma unroll
-                for (int q = 0; q < 8; ++q) v[q] += f.add * e[q];
+            for (int q = 0; q < 8; ++q) x[q] = turned ? box[(c + q) * 36 + line] : box[line * 36 + c + q];
+            const int valid = turned ? p.rows - row : p.cols - column;
+            if (a.mode == kToFloat) {
+                store8((float *)(region + p.d + (int64_t)row * p.ldd) + column, valid, x);
+                continue;
             }
-            if (bi == bj) {
+            T *o = (T *)r.out + row * r.out_rs + column * r.out_cs;
+            const int64_t by = turned ? r.out_rs : r.out_cs;
+            if (by == 1) {
+                if (a.mode == kToParam) {
+                    load8(o, valid, e);
 #pragma unroll
-                for (int q = 0; q < 8; ++q)
-                    if (row == col + q) v[q] += f.diag;
-            }
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-                if (bi + row >= p.rows || bj + col + q >= p.cols) v[q] = 0.f;
-            if (a.mode == kToOperand) {
-                if (p.d >= 0 && bi + row < p.rows)
-                    storeOperand(region + p.d + (int64_t)(bi + row) * p.ldd, bj + col, v,
-                                 a.split_out);
-            } else if (a.mode == kToFloat) {
-                if (bi + row < p.rows && bj + col < p.cols) {
-                    float *o = (float *)(region + p.d + (int64_t)(bi + row) * p.ldd) + bj + col;
-                    store8(o, p.cols - bj - col, v);
-                }
-            } else if (!turned && bi + row < p.rows && bj + col < p.cols) {
-                T *o = (T *)r.out + (bi + row) * r.out_rs + (bj + col) * r.out_cs;
-                const int valid = p.cols - bj - col;
-                if (r.out_cs == 1) {
-                    if (a.mode == kToParam) {
-                        load8(o, valid, e);
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) v[q] = r.keep * e[q] - r.rate * v[q];
-                    } else {
-#pragma unroll
-                        for (int q = 0; q < 8; ++q) v[q] *= r.rate;
-                    }
-                    store8(o, valid, v);
+                    for (int q = 0; q < 8; ++q) x[q] = r.keep * e[q] - r.rate * x[q];
                 } else {
-                    for (int q = 0; q < 8 && q < valid; ++q) {
-                        TOA_GLOBAL T *x = global<T>((void *)(o + q * r.out_cs));
-                        *x = fromFloat<T>(a.mode == kToParam ? r.keep * toFloat(*x) - r.rate * v[q]
-                                                             : r.rate * v[q]);
-                    }
+#pragma unroll
+                    for (int q = 0; q < 8; ++q) x[q] *= r.rate;
                 }
-            }
-            if (p.dt >= 0 || turned) {
-#pragma unroll
-                for (int q = 0; q < 8; ++q) box[row * 36 + col + q] = v[q];
-            }
-        }
-        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-        __builtin_amdgcn_wave_barrier();
-        if ((p.dt >= 0 && !(a.symmetric && ti == tj)) || turned) {
-#pragma unroll
-            for (int half = 0; half < 2; ++half) {
-                const int col = half * 16 + (lane >> 2), row = (lane & 3) * 8;
-                if (bj + col >= p.cols) continue;
-                float v[8], e[8];
-#pragma unroll
-                for (int q = 0; q < 8; ++q) v[q] = box[(row + q) * 36 + col];
-                if (a.mode == kToOperand) {
-                    storeOperand(region + p.dt + (int64_t)(bj + col) * p.lddt, bi + row, v,
-                                 a.split_out);
-                } else if (turned && bi + row < p.rows) {
-                    T *o = (T *)r.out + (bi + row) * r.out_rs + (bj + col) * r.out_cs;
-                    const int valid = p.rows - bi - row;
-                    if (r.out_rs == 1) {
-                        if (a.mode == kToParam) {
-                            load8(o, valid, e);
-#pragma unroll
-                            for (int q = 0; q < 8; ++q) v[q] = r.keep * e[q] - r.rate * v[q];
-                        } else {
-#pragma unroll
-                            for (int q = 0; q < 8; ++q) v[q] *= r.rate;
-                        }
-                        store8(o, valid, v);
-                    } else {
-                        for (int q = 0; q < 8 && q < valid; ++q) {
-                            TOA_GLOBAL T *x = global<T>((void *)(o + q * r.out_rs));
-                            *x = fromFloat<T>(a.mode == kToParam
-                                                  ? r.keep * toFloat(*x) - r.rate * v[q]
-                                                  : r.rate * v[q]);
-                        }
-                    }
+                store8(o, valid, x);
+            } else {
+                for (int q = 0; q < 8 && q < valid; ++q) {
+                    TOA_GLOBAL T *y = global<T>((void *)(o + q * by));
+                    *y = fromFloat<T>(a.mode == kToParam ? r.keep * toFloat(*y) - r.rate * x[q]
+                                                         : r.rate * x[q]);
                 }
             }
         }
@@ -1604,8 +1703,8 @@ struct TailArgs {
     char *ws;
     double *parts;                              // <Y_0, X_0 * 2^e>
     int64_t y[kMaxGroups], x[kMaxGroups];       // float rows of Y_0; operand rows of X_0
-    int64_t rows_per[kMaxGroups];               // dot: rows per workgroup
-    int nparts[kMaxGroups], split;
+    int64_t per[kMaxGroups];                    // dot: cells of 32 x 32 per workgroup
+    int nparts[kMaxGroups];
 };
 
 __global__ __launch_bounds__(256) void dot_kernel(TailArgs a) {
@@ -1613,18 +1712,21 @@ __global__ __launch_bounds__(256) void dot_kernel(TailArgs a) {
     int part = blockIdx.x, mat;
     const int gi = findGroup(a.sh, part, mat);
     const Group &g = a.sh.g[gi];
-    const char *region = a.ws + g.base + mat * g.stride;
+    char *region = a.ws + g.base + mat * g.stride;
     mat += g.mat0;
-    const int64_t wp = padded(g.w), ld = rowBytes(wp, a.split);
-    const int from = (int)(part * a.rows_per[gi]);
-    const int to = from + a.rows_per[gi] < g.s ? (int)(from + a.rows_per[gi]) : g.s;
+    const int64_t wp = padded(g.w), ld = rowBytes(wp, true);
+    const int across = (int)(wp / 32);
+    const int64_t cells = (int64_t)((g.s + 31) / 32) * across, from = part * a.per[gi];
+    const int64_t to = from + a.per[gi] < cells ? from + a.per[gi] : cells;
     double sum = 0.0;
-    const int across = (int)(wp / 8);
-    for (int64_t q = threadIdx.x; q < (int64_t)(to - from) * across; q += 256) {
-        const int i = from + (int)(q / across), j = (int)(q % across) * 8;
-        if (j >= g.w) continue;
+    // 128 chunks to a cell
+    for (int64_t q = from * 128 + threadIdx.x; q < to * 128; q += 256) {
+        const int64_t cell = q >> 7;
+        const int i = (int)(cell / across) * 32 + (int)(q & 31);
+        const int j = (int)(cell % across) * 32 + (int)(q >> 5 & 3) * 8;
+        if (i >= g.s || j >= g.w) continue;
         float x[8], y[8];
-        loadOperand(region + a.x[gi] + i * ld, j, x, a.split);
+        loadOperand(chunkOf(region + a.x[gi], ld, i, j, true), x);
         load8((const float *)(region + a.y[gi]) + i * wp + j, g.w - j, y);
 #pragma unroll
         for (int k = 0; k < 8; ++k) sum += (double)x[k] * (double)y[k];
@@ -1639,7 +1741,7 @@ template <typename T> __global__ __launch_bounds__(256) void tail_kernel(TailArg
     int t = blockIdx.x, mat;
     const int gi = findGroup(a.sh, t, mat);
     const Group &g = a.sh.g[gi];
-    const char *region = a.ws + g.base + mat * g.stride;
+    char *region = a.ws + g.base + mat * g.stride;
     mat += g.mat0;
     const MatRec &r = a.recs[mat];
     const MatNorm n = a.norms[mat];
@@ -1648,13 +1750,13 @@ template <typename T> __global__ __launch_bounds__(256) void tail_kernel(TailArg
     const double back = 1.0 / (n.x_scale * n.plus);  // stored X_0 * back = X_0 (a power of two)
     const double ky = 1.0 / n.plus;
     const double kx = n.size > 0.0 ? dot * back / n.size * back : n.size;  // (NaN stays NaN)
-    const int64_t wp = padded(g.w), ld = rowBytes(wp, a.split);
+    const int64_t wp = padded(g.w), ld = rowBytes(wp, true);
     const int across = (int)(wp / 64), i0 = t / across * 64, j0 = t % across * 64;
     for (int q = threadIdx.x; q < 512; q += 256) {
         const int i = i0 + (q >> 3), c = (q & 7) * 8, j = j0 + c;
         float x[8], y[8];
         if (i < g.s && j < g.w) {
-            loadOperand(region + a.x[gi] + i * ld, j, x, a.split);
+            loadOperand(chunkOf(region + a.x[gi], ld, i, j, true), x);
             load8((const float *)(region + a.y[gi]) + i * wp + j, g.w - j, y);
 #pragma unroll
             for (int k = 0; k < 8; ++k)

@@ -34,7 +34,7 @@ Layout layoutOf(int s, int w, int steps, bool backward) {
     int64_t at = 0;
     auto take = [&](int64_t rows, int64_t cols) {
         const int64_t here = at;
-        at += align256(rows * rowBytes(padded(cols), true));
+        at += align256((rows + kRows - 1) / kRows * kRows * rowBytes(padded(cols), true));
         return here;
     };
     if (backward) {
@@ -510,7 +510,7 @@ class Run {
                 case kTiles128:
                     return sp ? tiles<T, 128, 2, 4, 1, 4, true>(a) : tiles<T, 128, 2, 4, 1, 4, false>(a);
                 default:
-                    return sp ? tiles<T, 64, 1, 1, 4, 2, true>(a) : tiles<T, 64, 1, 1, 4, 2, false>(a);
+                    return sp ? tiles<T, 64, 1, 1, 4, 3, true>(a) : tiles<T, 64, 1, 1, 4, 3, false>(a);
             }
         });
     }
@@ -694,13 +694,13 @@ class Run {
         a.norms = (const MatNorm *)(c_.ws + head_.norms);
         a.ws = c_.ws;
         a.parts = (double *)(c_.ws + head_.parts);
-        a.split = split(0);
         int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int k) {
             a.y[k] = s.lay.yf;
             a.x[k] = s.lay.x[0];
             int64_t parts = std::min<int64_t>(kMaxParts, ((int64_t)s.s * s.w + 8191) / 8192);
-            a.rows_per[k] = (s.s + parts - 1) / parts;
-            a.nparts[k] = (int)((s.s + a.rows_per[k] - 1) / a.rows_per[k]);
+            const int64_t cells = (s.s + 31) / 32 * (padded(s.w) / 32);
+            a.per[k] = (cells + parts - 1) / parts;
+            a.nparts[k] = (int)((cells + a.per[k] - 1) / a.per[k]);
             return (int64_t)a.nparts[k];
         });
         TRY(launch(dot_kernel, grid, 256, c_.stream, a));
