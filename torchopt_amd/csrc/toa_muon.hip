@@ -510,7 +510,7 @@ class Run {
                 case kTiles128:
                     return sp ? tiles<T, 128, 2, 4, 1, 4, true>(a) : tiles<T, 128, 2, 4, 1, 4, false>(a);
                 default:
-                    return sp ? tiles<T, 64, 1, 1, 4, 3, true>(a) : tiles<T, 64, 1, 1, 4, 3, false>(a);
+                    return sp ? tiles<T, 64, 1, 1, 4, 2, true>(a) : tiles<T, 64, 1, 1, 4, 2, false>(a);
             }
         });
     }
@@ -522,12 +522,17 @@ class Run {
 
     enum { kTiles256, kTiles128Pair, kTiles128, kTiles64, kVariants };
 
-    // The variant that finishes first.  A tile's time is its start and stores plus its pieces; it
-    // grows from `alone` to `full` as tiles fill the chip (measured: with the square of the share
-    // filled).  Microseconds from 8 x 512^2, 2..16 x 1024^2, 2048^2 and 4096^2: large tiles get
-    // most out of a full chip (1.4 PFLOP/s of half products in 256 x 256, 0.9 in 64 x 64), small
-    // ones start and end sooner and spread few results over more of it (a product of one 1024^2
-    // matrix: 72 us in 256 x 256, 34 in 128 x 128, 15 in 64 x 64; of sixteen: 115, 145, 220).
+    // The variant that finishes first.  A tile's time is its start and stores plus its pieces: `alone`
+    // on an empty chip, `full` where as many as fit are at work.  What is left after whole rounds
+    // takes between the two: the large tiles as the square of the share filled; the 128 x 128 of which
+    // two fit on a compute unit little more than one alone up to one to a unit, and most of a round
+    // beyond; the 64 x 64 follow each other without rounds.
+    // Microseconds fitted to 1..48 matrices of 1024^2, 2048^2, 4096^2, 16 x 512^2 and 64 x 256^2, to
+    // 3..10 % (the 64 x 64 then 8 % up: long lists of different operands miss the L2 more); the variant
+    // chosen is 0.3 % from the best of the four on average, 7 % at most.  Large
+    // tiles get most out of a full chip (P X of 48 matrices of 1024^2: 324 us in 256 x 256, 379, 400
+    // and 436 in 64 x 64), small ones start and end sooner and spread few results over more of it (of
+    // one matrix: 65, 29, 26 and 13 us).
     int pickTiles(const GemmArgs &a, bool split_in) const {
         struct Variant {
             int size, at_once;  // tiles that the whole chip holds
@@ -535,14 +540,14 @@ class Run {
         };
         // with 22-bit operands, and with halves
         static const Variant table[2][kVariants] = {
-            {{256, 256, 18.0, 1.69, 39.0, 2.3},
-             {128, 512, 10.3, 0.70, 26.0, 1.45},
-             {128, 256, 8.3, 0.56, 2.0, 1.03},
-             {64, 256, 7.6, 0.20, 7.6, 0.22}},
-            {{256, 256, 14.0, 1.4, 22.0, 2.3},
-             {128, 512, 9.0, 0.62, 13.0, 1.45},
-             {128, 256, 7.5, 0.50, 3.3, 1.03},
-             {64, 256, 7.6, 0.20, 7.1, 0.22}}};
+            {{256, 256, 12.5, 1.67, 46.4, 2.18},
+             {128, 512, 7.8, 0.66, 25.7, 1.24},
+             {128, 256, 5.1, 0.63, 11.6, 0.70},
+             {64, 512, 4.7, 0.21, 1.9, 0.54}},
+            {{256, 256, 12.7, 1.26, 29.0, 1.54},
+             {128, 512, 7.3, 0.63, 17.2, 0.97},
+             {128, 256, 6.2, 0.50, 8.4, 0.58},
+             {64, 512, 5.0, 0.26, 4.1, 0.42}}};
         const Variant *variants = table[!split_in];
         int best = 0;
         double least = 0.0;
@@ -555,11 +560,18 @@ class Run {
                 pieces += n * (a.p[g].steps0 + a.p[g].steps1);
             }
             pieces /= tiles;
-            const double alone = v.alone + v.alone_piece * pieces;
-            const double full = std::max(alone, v.full + v.full_piece * pieces);
+            const double alone = v.alone + v.alone_piece * pieces, full = v.full + v.full_piece * pieces;
             const double rounds = std::floor(tiles / v.at_once), rest = tiles / v.at_once - rounds;
-            const double time =
-                rounds * full + (rest > 0.0 ? alone + (full - alone) * rest * rest : 0.0);
+            double time;
+            if (k == kTiles64) {
+                time = std::max(alone, v.alone + full * tiles / v.at_once);
+            } else {
+                const double share = k != kTiles128Pair ? rest * rest
+                                     : rest <= 0.5      ? 0.3 * rest
+                                                        : 0.4 + 0.6 * rest;
+                const double more = std::max(0.0, full - alone);
+                time = rounds * (alone + more) + (rest > 0.0 ? alone + more * share : 0.0);
+            }
             if (k == 0 || time < least) {
                 least = time;
                 best = k;
