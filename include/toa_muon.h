@@ -26,8 +26,9 @@
  *   dtype     TOA_F32, TOA_F16 or TOA_BF16 (codes of toa_adam.h); all views of a call share it,
  *             except the momentum, whose type is given apart.
  *   precision products run on the matrix cores with float32 sums.  Their operands carry 22
- *             significant bits (two halves) -- for bfloat16 calls 11 bits in the last two
- *             orthogonalisation steps, whose rounding the steps that follow hardly amplify.
+ *             significant bits (two halves).  In a bfloat16 call that keeps no iterates, those of
+ *             the last two orthogonalisation steps may carry 11, whose rounding the steps that
+ *             follow hardly amplify.
  *   workspace device memory the call may overwrite, 256-byte aligned, as many bytes as the
  *             matching *_workspace function says; calls that may overlap in time (other streams,
  *             other captured graphs) need workspaces of their own.
@@ -77,21 +78,33 @@ TOA_API const char *toa_muon_error_string(int code);
 /* Bytes of workspace for a list; 0 for a list without elements.  TOA_ESIZE through `status`
  * (may be NULL) where a dimension is beyond 2^20. */
 TOA_API size_t toa_muon_orthogonalize_workspace(int dtype, size_t num, const int64_t *rows,
-                                                const int64_t *cols, int steps, int *status);
+                                                const int64_t *cols, int steps, int keep,
+                                                int *status);
 TOA_API size_t toa_muon_backward_workspace(int dtype, size_t num, const int64_t *rows,
-                                           const int64_t *cols, int steps, int *status);
+                                           const int64_t *cols, int steps, int kept, int *status);
 
+/* What the gradient needs of the forward pass -- every iterate and its products -- can be kept
+ * between the two: bytes of that buffer (256-byte aligned) for a list, about 8 bytes for each
+ * element of a matrix and of the square of its shorter side, for each step; small matrices, whose
+ * iterates are made again faster than they are read, need none. */
+TOA_API size_t toa_muon_kept_bytes(int dtype, size_t num, const int64_t *rows, const int64_t *cols,
+                                   int steps, int *status);
+
+/* kept: where the iterates go, or NULL.  keep / kept of the workspace functions says which. */
 TOA_API int toa_muon_orthogonalize_multi(int dtype, size_t num, const int64_t *rows,
                                          const int64_t *cols, const toa_muon_view *in,
                                          const toa_muon_view *out, const toa_muon_series *series,
-                                         void *workspace, size_t workspace_bytes, void *stream);
+                                         void *kept, size_t kept_bytes, void *workspace,
+                                         size_t workspace_bytes, void *stream);
 
-/* grad_in = d<orthogonalize(in), grad_out> / d in; the iterates are computed again from `in`. */
+/* grad_in = d<orthogonalize(in), grad_out> / d in.  kept: what the forward call with the same
+ * `in`, list and series left, which is only read; or NULL: the iterates are computed again. */
 TOA_API int toa_muon_orthogonalize_backward_multi(int dtype, size_t num, const int64_t *rows,
                                                   const int64_t *cols, const toa_muon_view *in,
                                                   const toa_muon_view *grad_out,
                                                   const toa_muon_view *grad_in,
-                                                  const toa_muon_series *series, void *workspace,
+                                                  const toa_muon_series *series, const void *kept,
+                                                  size_t kept_bytes, void *workspace,
                                                   size_t workspace_bytes, void *stream);
 
 /* The optimizer step (workspace as for orthogonalize).

@@ -250,6 +250,48 @@ def test_gradient_steps(steps):
                        eps=0.25)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+def test_kept_iterates_give_the_same_gradient(dtype):
+    """The gradient from kept iterates is that from iterates made again, bit for bit (both take every
+    step by itself with 22-bit operands); the buffer is only read, and serves as often as asked."""
+    shapes = [(90, 400), (20, 30), (300, 130), (90, 400), (65, 65), (0, 5)]
+    for kw in (dict(), dict(steps=1), dict(steps=4, coefficients=(1.5, -0.5, 0.0))):
+        xs = [randn(*s, dtype=dtype, seed=k).cuda() for k, s in enumerate(shapes)]
+        dys = [randn(*s, dtype=dtype, seed=k + 20).cuda() for k, s in enumerate(shapes)]
+        ys, kept = muon_op.orthogonalize_keep_multi(xs, 1 << 30, **kw)
+        assert kept is not None
+        before = kept.clone()
+        want = muon_op.orthogonalize_backward_multi(dys, xs, **kw)
+        for _ in range(2):
+            got = muon_op.orthogonalize_backward_multi(dys, xs, **kw, kept=kept)
+            assert all(map(torch.equal, got, want))
+        assert torch.equal(kept, before)
+        for x, y in zip(xs, ys):
+            if x.numel():
+                exact, allowed = plain.tolerance(plain.orthogonalize, x.double().cpu(), dtype=F32, **kw)
+                plain.assert_close(y, exact, allowed)
+    assert muon_op.orthogonalize_keep_multi(xs, kept.numel() - 1, **kw)[1] is None
+    assert muon_op.orthogonalize_keep_multi(xs[1:2], 1 << 30)[1] is None
+    for bad in (kept[:-256], kept.float(), kept.cpu()):
+        with pytest.raises(RuntimeError, match='not what the forward pass kept'):
+            muon_op.orthogonalize_backward_multi(dys, xs, **kw, kept=bad)
+    with pytest.raises(RuntimeError, match='not what the forward pass kept'):
+        muon_op.orthogonalize_backward_multi(dys[:1], xs[:1], **kw, kept=kept)
+
+
+def test_gradient_with_and_without_keeping(monkeypatch):
+    from torchopt_amd.accelerated_op import muon_op as module
+    x, dy = randn(3, 200, 700, seed=1).cuda(), randn(3, 200, 700, seed=2).cuda()
+    grads = []
+    for limit in (module.KEEP_BYTES, 0):
+        monkeypatch.setattr(module, 'KEEP_BYTES', limit)
+        leaf = x.clone().requires_grad_()
+        y = orthogonalize(leaf)
+        grads += [torch.autograd.grad(y, leaf, dy, retain_graph=True)[0],
+                  torch.autograd.grad(y, leaf, dy)[0]]
+    assert all(torch.equal(g, grads[0]) for g in grads[1:])
+
+
 def test_plain_gradient_is_autograds():
     x, dy = randn(30, 40).double().requires_grad_(), randn(30, 40, seed=1).double()
     want, = torch.autograd.grad(plain.orthogonalize(x), x, dy)

@@ -45,8 +45,8 @@ class Hyper(ctypes.Structure):
 def lib():
     lib = ctypes.CDLL(LIB)
     lib.toa_muon_error_string.restype = ctypes.c_char_p
-    for name in ('orthogonalize', 'backward'):
-        getattr(lib, f'toa_muon_{name}_workspace').restype = ctypes.c_size_t
+    for name in ('orthogonalize_workspace', 'backward_workspace', 'kept_bytes'):
+        getattr(lib, f'toa_muon_{name}').restype = ctypes.c_size_t
     return lib
 
 
@@ -58,17 +58,19 @@ def series(steps=5, a=3.4445, b=-4.775, c=2.0315, eps=1e-7):
     return ctypes.byref(Series(steps, a, b, c, eps))
 
 
-def orth(lib, dtype=F32, rows=(4,), cols=(4,), q=None, data=None, workspace=None, size=0):
+def orth(lib, dtype=F32, rows=(4,), cols=(4,), q=None, data=None, kept=None, kept_size=0,
+         workspace=None, size=0):
     views = (View * max(1, len(rows)))(*[View(data, 1, 1) for _ in rows])
     return lib.toa_muon_orthogonalize_multi(
         dtype, ctypes.c_size_t(len(rows)), sides(*rows), sides(*cols), views, views,
-        q or series(), ctypes.c_void_p(workspace), ctypes.c_size_t(size), None)
+        q or series(), ctypes.c_void_p(kept), ctypes.c_size_t(kept_size),
+        ctypes.c_void_p(workspace), ctypes.c_size_t(size), None)
 
 
 def test_library_exports_every_declared_symbol(lib):
     text = re.sub(r'/\*.*?\*/', '', open(HEADER).read(), flags=re.S)
     names = re.findall(r'TOA_API\s+(?:const\s+char\s*\*|int|size_t)\s*(\w+)\s*\(', text)
-    assert len(names) == 9
+    assert len(names) == 10
     for name in names:
         assert hasattr(lib, name), f'{name} declared in include/toa_muon.h but not exported'
     assert lib.toa_muon_abi_version() == 1
@@ -85,9 +87,14 @@ def test_argument_errors_need_no_device(lib):
     assert orth(lib) == ENULL  # the matrix ...
     assert orth(lib, rows=(100,), cols=(100,), data=256) == ENULL  # ... or the workspace
     need = lib.toa_muon_orthogonalize_workspace(F32, ctypes.c_size_t(1), sides(100), sides(100), 5,
-                                                None)
+                                                0, None)
     assert orth(lib, rows=(100,), cols=(100,), data=256, workspace=256, size=need - 1) == EWORKSPACE
     assert orth(lib, rows=(100,), cols=(100,), data=256, workspace=264, size=need) == EWORKSPACE
+    keep = lib.toa_muon_kept_bytes(F32, ctypes.c_size_t(1), sides(100), sides(100), 5, None)
+    assert keep == 5 * 4 * 128 * 128 * 4  # X, its transpose, S and P of five steps
+    for kept, short in ((256, 1), (264, 0)):
+        assert orth(lib, rows=(100,), cols=(100,), data=256, kept=kept, kept_size=keep - short,
+                    workspace=256, size=need) == EWORKSPACE
     assert orth(lib, rows=((1 << 20) + 1,), cols=(1,)) == ESIZE
     assert orth(lib, rows=(-1,), cols=(4,)) == ESIZE
     inf, nan = float('inf'), float('nan')
@@ -95,7 +102,8 @@ def test_argument_errors_need_no_device(lib):
                 dict(eps=nan), dict(a=100.0), dict(c=1e6)):
         assert orth(lib, q=series(**bad)) == EVALUE, bad
     assert lib.toa_muon_orthogonalize_multi(F32, ctypes.c_size_t(0), None, None, None, None, None,
-                                            None, ctypes.c_size_t(0), None) == ENULL
+                                            None, ctypes.c_size_t(0), None, ctypes.c_size_t(0),
+                                            None) == ENULL
 
 
 def test_step_arguments(lib):
@@ -115,11 +123,12 @@ def test_step_arguments(lib):
 
 
 def test_workspace_sizes(lib):
-    def size(rows, cols, steps=5, which='orthogonalize', dtype=F32):
+    def size(rows, cols, steps=5, which='orthogonalize', dtype=F32, keep=0):
         status = ctypes.c_int(99)
-        n = getattr(lib, f'toa_muon_{which}_workspace')(
-            dtype, ctypes.c_size_t(len(rows)), sides(*rows), sides(*cols), steps,
-            ctypes.byref(status))
+        lists = dtype, ctypes.c_size_t(len(rows)), sides(*rows), sides(*cols), steps
+        if which == 'kept':
+            return lib.toa_muon_kept_bytes(*lists, ctypes.byref(status)), status.value
+        n = getattr(lib, f'toa_muon_{which}_workspace')(*lists, keep, ctypes.byref(status))
         return n, status.value
 
     assert size((), ()) == (0, 0) and size((0,), (7,)) == (0, 0)
@@ -129,6 +138,13 @@ def test_workspace_sizes(lib):
     # one batch holds at most 4 GiB of regions, whatever the list
     assert size((1024,) * 400, (1024,) * 400)[0] < (4 << 30) + (64 << 20)
     assert size((1024,), (1024,), which='backward')[0] > 3 * size((1024,), (1024,))[0]
+    # what is kept is not in the workspace; small matrices keep nothing
+    kept = size((1024,), (1024,), which='kept')[0]
+    whole, rest = (size((1024,), (1024,), which='backward', keep=k)[0] for k in (0, 1))
+    assert whole - rest == kept == 5 * 4 * 4 << 20
+    assert size((32, 1024), (288, 1024), which='kept')[0] == kept
+    assert size((32,), (288,), which='kept') == (0, 0)
+    assert size((1024,), (1024,), keep=1)[0] < size((1024,), (1024,))[0]
     assert size((4,), (4,), steps=0)[1] == EVALUE and size((4,), (4,), dtype=F64)[1] == EDTYPE
     assert size((1 << 21,), (4,))[1] == ESIZE
 

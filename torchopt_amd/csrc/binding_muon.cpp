@@ -82,31 +82,49 @@ Tensor workspaceFor(const char *name, const Tensor &like, size_t bytes, int stat
 
 // ---- orthogonalize and its gradient --------------------------------------------------------
 
-TensorList orthogonalizeMulti(const py::object &inputs_o, int steps, const Coefficients &c,
-                              double eps) {
+// Results, and what the gradient can use of the way to them (or nothing, where that is nothing or more
+// than `keep` bytes).
+std::pair<TensorList, c10::optional<Tensor>> orthogonalizeKeepMulti(const py::object &inputs_o,
+                                                                    int64_t keep, int steps,
+                                                                    const Coefficients &c,
+                                                                    double eps) {
     const char *name = "muonOrthogonalizeMulti";
     const TensorList in = toTensorList(inputs_o, "inputs");
     TensorList out;
-    if (in.empty()) return out;
+    c10::optional<Tensor> kept;
+    if (in.empty()) return {out, kept};
     const int code = gate(name, in);
     const Matrices m(name, in);
     for (const Tensor &t : in) out.push_back(at::empty_like(t));
     const toa_muon_series series = seriesOf(steps, c, eps);
     const OnDeviceOf dev(in[0]);
-    int status;
-    const size_t bytes = toa_muon_orthogonalize_workspace(code, m.rows.size(), m.rows.data(),
-                                                          m.cols.data(), steps, &status);
+    int status = 0;
+    size_t kept_bytes = 0;
+    if (keep > 0) {
+        kept_bytes = toa_muon_kept_bytes(code, m.rows.size(), m.rows.data(), m.cols.data(), steps, &status);
+        if (kept_bytes > (size_t)keep) kept_bytes = 0;
+        if (kept_bytes) kept = workspaceFor(name, in[0], kept_bytes, status);
+    }
+    const size_t bytes = toa_muon_orthogonalize_workspace(
+        code, m.rows.size(), m.rows.data(), m.cols.data(), steps, kept_bytes != 0, &status);
     const Tensor ws = workspaceFor(name, in[0], bytes, status);
     check(toa_muon_orthogonalize_multi(code, m.rows.size(), m.rows.data(), m.cols.data(),
                                        viewsOf(in, m.rows.size()).data(),
-                                       viewsOf(out, m.rows.size()).data(), &series, ws.data_ptr(),
+                                       viewsOf(out, m.rows.size()).data(), &series,
+                                       kept ? kept->data_ptr() : nullptr, kept_bytes, ws.data_ptr(),
                                        bytes, dev.stream()),
           name);
-    return out;
+    return {out, kept};
+}
+
+TensorList orthogonalizeMulti(const py::object &inputs_o, int steps, const Coefficients &c,
+                              double eps) {
+    return orthogonalizeKeepMulti(inputs_o, 0, steps, c, eps).first;
 }
 
 TensorList orthogonalizeBackwardMulti(const py::object &grads_o, const py::object &inputs_o,
-                                      int steps, const Coefficients &c, double eps) {
+                                      int steps, const Coefficients &c, double eps,
+                                      const c10::optional<Tensor> &kept) {
     const char *name = "muonOrthogonalizeBackwardMulti";
     const TensorList in = toTensorList(inputs_o, "inputs");
     TensorList dy = toTensorList(grads_o, "grads"), out;
@@ -125,13 +143,21 @@ TensorList orthogonalizeBackwardMulti(const py::object &grads_o, const py::objec
     const toa_muon_series series = seriesOf(steps, c, eps);
     const OnDeviceOf dev(in[0]);
     int status;
+    size_t kept_bytes = 0;
+    if (kept) {
+        kept_bytes = toa_muon_kept_bytes(code, m.rows.size(), m.rows.data(), m.cols.data(), steps, &status);
+        check(status, name);
+        TORCH_CHECK(kept->device() == in[0].device() && kept->scalar_type() == at::kByte &&
+                        kept->is_contiguous() && kept_bytes && (size_t)kept->numel() == kept_bytes,
+                    name, ": kept is not what the forward pass kept of these inputs");
+    }
     const size_t bytes = toa_muon_backward_workspace(code, m.rows.size(), m.rows.data(),
-                                                     m.cols.data(), steps, &status);
+                                                     m.cols.data(), steps, kept_bytes != 0, &status);
     const Tensor ws = workspaceFor(name, in[0], bytes, status);
     check(toa_muon_orthogonalize_backward_multi(
               code, m.rows.size(), m.rows.data(), m.cols.data(), viewsOf(in, m.rows.size()).data(),
               viewsOf(dy, m.rows.size()).data(), viewsOf(out, m.rows.size()).data(), &series,
-              ws.data_ptr(), bytes, dev.stream()),
+              kept ? kept->data_ptr() : nullptr, kept_bytes, ws.data_ptr(), bytes, dev.stream()),
           name);
     return out;
 }
@@ -253,7 +279,7 @@ void stepMulti(const char *name, const TensorList &out, TensorList grads, const 
     const OnDeviceOf dev(out[0]);
     int status;
     const size_t bytes = toa_muon_orthogonalize_workspace(code, rows.size(), rows.data(),
-                                                          cols.data(), series.steps, &status);
+                                                          cols.data(), series.steps, 0, &status);
     const Tensor ws = workspaceFor(name, out[0], bytes, status);
     check(toa_muon_step_multi(code, kept_code, rows.size(), rows.data(), cols.data(), vo.data(),
                               vg.data(), vm.data(), blocks ? vs.data() : nullptr, &hyper, &series,
@@ -370,9 +396,15 @@ void defineMuonOp(py::module &mod) {
     m.def("orthogonalize_multi", &orthogonalizeMulti,
           "Newton-Schulz orthogonalisation of every matrix of a list (last two dimensions)",
           "inputs"_a, "steps"_a = 5, "coefficients"_a = c, "eps"_a = 1e-7);
+    m.def("orthogonalize_keep_multi", &orthogonalizeKeepMulti,
+          "orthogonalize_multi, and a buffer with the iterates for the gradient, or None where it "
+          "would hold more than `keep` bytes (or nothing)",
+          "inputs"_a, "keep"_a, "steps"_a = 5, "coefficients"_a = c, "eps"_a = 1e-7);
     m.def("orthogonalize_backward_multi", &orthogonalizeBackwardMulti,
-          "gradient of orthogonalize_multi with respect to its inputs", "grads"_a, "inputs"_a,
-          "steps"_a = 5, "coefficients"_a = c, "eps"_a = 1e-7);
+          "gradient of orthogonalize_multi with respect to its inputs, from what "
+          "orthogonalize_keep_multi kept of the same inputs if that is given",
+          "grads"_a, "inputs"_a, "steps"_a = 5, "coefficients"_a = c, "eps"_a = 1e-7,
+          "kept"_a = py::none());
     m.def("forward_multi_", &forwardMulti,
           "momentum and orthogonalisation in place; mutates and returns (updates, mu, scales)",
           "updates"_a, "mu"_a, "scales"_a, "momentum"_a, py::kw_only(), "nesterov"_a = true,

@@ -80,6 +80,7 @@ struct MatNorm {
 struct Group {         // matrices of one shape
     int64_t base;      // bytes from the workspace to the first one's region
     int64_t stride;    // bytes from one region to the next
+    int64_t kept_base, kept_stride;  // the same in the buffer of kept iterates
     int s, w, mat0;
     int tile0, tiles, all;  // workgroups of this launch: first, per matrix, of all its matrices
 };
@@ -87,6 +88,19 @@ struct Group {         // matrices of one shape
 struct Shapes {
     int n;
     Group g[kMaxGroups];
+};
+
+// Where a matrix's buffers lie: at an offset into its region of the workspace or, with this bit set, of
+// the buffer that keeps the iterates between the forward pass and the gradient.
+constexpr int64_t kKept = (int64_t)1 << 62;
+
+struct Region {
+    char *own, *kept;
+    __device__ Region(char *ws, char *kept_, const Group &g, int mat)
+        : own(ws + g.base + mat * g.stride), kept(kept_ + g.kept_base + mat * g.kept_stride) {}
+    __device__ char *operator+(int64_t offset) const {
+        return offset & kKept ? kept + (offset & ~kKept) : own + offset;
+    }
 };
 
 // The caller's tensors come as addresses in records: without this they would be read and written
@@ -525,7 +539,7 @@ struct PackArgs {
     Shapes sh;
     const MatRec *recs;
     const MatNorm *norms;
-    char *ws;
+    char *ws, *kept;
     int64_t off[kMaxGroups], off_t[kMaxGroups];  // of the operand and of its transpose
     StepArgs step;
     int split;
@@ -587,7 +601,7 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     int t = blockIdx.x, mat;
     const int gi = findGroup(a.sh, t, mat);
     const Group &g = a.sh.g[gi];
-    char *region = a.ws + g.base + mat * g.stride;
+    const Region region(a.ws, a.kept, g, mat);
     mat += g.mat0;
     const MatRec &r = a.recs[mat];
     const int across = (int)(padded(g.w) / 64);
@@ -653,7 +667,7 @@ struct Product {             // one matrix's operands, as byte offsets into its 
 };
 
 struct GemmArgs {
-    char *ws;
+    char *ws, *kept;
     const MatRec *recs;
     const Factor *factors;
     int stages, stage, symmetric, mode, split_out;
@@ -760,7 +774,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64, KS > 1 ? 2 : 1) void gemm_kernel(G
     Product p = a.p[gi];
     // (read now, all at once: what only the stores need would be waited for there, one by one)
     asm volatile("" : "+s"(p.d), "+s"(p.dt), "+s"(p.e), "+s"(p.ldd), "+s"(p.lddt), "+s"(p.rows), "+s"(p.cols));
-    char *region = a.ws + a.sh.g[gi].base + mat * a.sh.g[gi].stride;
+    const Region region(a.ws, a.kept, a.sh.g[gi], mat);
     mat += a.sh.g[gi].mat0;
     int ti, tj;
     tileOf(t, (p.rows + BM - 1) / BM, (p.cols + BN - 1) / BN, a.symmetric, ti, tj);
@@ -781,10 +795,10 @@ __global__ __launch_bounds__(WM *WN *KS * 64, KS > 1 ? 2 : 1) void gemm_kernel(G
 
     // Blocks of rows beyond the matrix repeat its last one; what comes of them is not stored.
     const int last_a = (p.rows - 1) / kRows - i0 / kRows, last_b = (p.cols - 1) / kRows - j0 / kRows;
-    const char *const a0 = region + p.a0 + (int64_t)i0 * p.lda;
-    const char *const b0 = region + p.b0 + (int64_t)j0 * p.ldb;
-    const char *const a1 = region + p.a1 + (int64_t)i0 * p.lda;
-    const char *const b1 = region + p.b1 + (int64_t)j0 * p.ldb;
+    const char *const a0 = (region + p.a0) + (int64_t)i0 * p.lda;
+    const char *const b0 = (region + p.b0) + (int64_t)j0 * p.ldb;
+    const char *const a1 = (region + p.a1) + (int64_t)i0 * p.lda;
+    const char *const b1 = (region + p.b1) + (int64_t)j0 * p.ldb;
     // piece number k of this wave is number part + KS k of the tile
     const int steps0 = p.steps0, all = p.steps0 + p.steps1;
     const int steps = (all - part + KS - 1) / KS;
@@ -1141,7 +1155,7 @@ __global__ __launch_bounds__(WM *WN *KS * 64, KS > 1 ? 2 : 1) void gemm_kernel(G
             for (int q = 0; q < 8; ++q) x[q] = turned ? box[(c + q) * 36 + line] : box[line * 36 + c + q];
             const int valid = turned ? p.rows - row : p.cols - column;
             if (a.mode == kToFloat) {
-                store8((float *)(region + p.d + (int64_t)row * p.ldd) + column, valid, x);
+                store8((float *)((region + p.d) + (int64_t)row * p.ldd) + column, valid, x);
                 continue;
             }
             T *o = (T *)r.out + row * r.out_rs + column * r.out_cs;
@@ -1703,7 +1717,7 @@ struct TailArgs {
     Shapes sh;
     const MatRec *recs;
     const MatNorm *norms;
-    char *ws;
+    char *ws, *kept;
     double *parts;                              // <Y_0, X_0 * 2^e>
     int64_t y[kMaxGroups], x[kMaxGroups];       // float rows of Y_0; operand rows of X_0
     int64_t per[kMaxGroups];                    // dot: cells of 32 x 32 per workgroup
@@ -1715,7 +1729,7 @@ __global__ __launch_bounds__(256) void dot_kernel(TailArgs a) {
     int part = blockIdx.x, mat;
     const int gi = findGroup(a.sh, part, mat);
     const Group &g = a.sh.g[gi];
-    char *region = a.ws + g.base + mat * g.stride;
+    const Region region(a.ws, a.kept, g, mat);
     mat += g.mat0;
     const int64_t wp = padded(g.w), ld = rowBytes(wp, true);
     const int across = (int)(wp / 32);
@@ -1744,7 +1758,7 @@ template <typename T> __global__ __launch_bounds__(256) void tail_kernel(TailArg
     int t = blockIdx.x, mat;
     const int gi = findGroup(a.sh, t, mat);
     const Group &g = a.sh.g[gi];
-    char *region = a.ws + g.base + mat * g.stride;
+    const Region region(a.ws, a.kept, g, mat);
     mat += g.mat0;
     const MatRec &r = a.recs[mat];
     const MatNorm n = a.norms[mat];

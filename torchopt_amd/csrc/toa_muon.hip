@@ -23,40 +23,48 @@ constexpr int64_t kMaxDim = (int64_t)1 << 20;
 
 int64_t align256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
-// Where one matrix's buffers lie in its region.
+// What a plan is for.  Keep: the forward pass leaves its iterates in a buffer of the caller's, and the
+// gradient (kGradientKept) finds them there.
+enum Purpose { kForward, kForwardKeep, kGradient, kGradientKept };
+
+// Where one matrix's buffers lie: offsets into its region, or into the kept iterates.
 struct Layout {
     int64_t x[kMaxSteps + 1], xt[kMaxSteps + 1], s[kMaxSteps], p[kMaxSteps];  // (gradient: step by step)
-    int64_t t, y[2], yt[2], m, n, yf, bytes;
+    int64_t t, y[2], yt[2], m, n, yf, bytes, kept_bytes;
 };
 
-Layout layoutOf(int s, int w, int steps, bool backward) {
-    Layout l;
-    int64_t at = 0;
-    auto take = [&](int64_t rows, int64_t cols) {
+Layout layoutOf(int s, int w, int steps, Purpose purpose) {
+    Layout l{};
+    auto take = [&](int64_t &at, int64_t rows, int64_t cols) {
         const int64_t here = at;
         at += align256((rows + kRows - 1) / kRows * kRows * rowBytes(padded(cols), true));
         return here;
     };
-    if (backward) {
+    int64_t at = 0;
+    if (purpose != kForward) {
         // every iterate is kept: the way back needs them in reverse
+        const int64_t where = purpose == kGradient ? 0 : kKept;
         for (int k = 0; k < steps; ++k) {
-            l.x[k] = take(s, w);
-            l.xt[k] = take(w, s);
-            l.s[k] = take(s, s);
-            l.p[k] = take(s, s);
+            l.x[k] = take(at, s, w) | where;
+            l.xt[k] = take(at, w, s) | where;
+            l.s[k] = take(at, s, s) | where;
+            l.p[k] = take(at, s, s) | where;
         }
-        for (int k = 0; k < 2; ++k) {
-            l.y[k] = take(s, w);
-            l.yt[k] = take(w, s);
+        if (where) std::swap(at, l.kept_bytes);
+        if (purpose != kForwardKeep) {
+            for (int k = 0; k < 2; ++k) {
+                l.y[k] = take(at, s, w);
+                l.yt[k] = take(at, w, s);
+            }
+            l.m = take(at, s, s);
+            l.n = take(at, s, s);
+            l.yf = take(at, s, w);
         }
-        l.m = take(s, s);
-        l.n = take(s, s);
-        l.yf = take(s, w);
     } else {
-        const int64_t x0 = take(s, w), x0t = take(w, s);
-        const int64_t x1 = steps > 1 ? take(s, w) : 0, x1t = steps > 1 ? take(w, s) : 0;
-        const int64_t ss = take(s, s), pp = take(s, s);
-        l.t = take(s, s);
+        const int64_t x0 = take(at, s, w), x0t = take(at, w, s);
+        const int64_t x1 = steps > 1 ? take(at, s, w) : 0, x1t = steps > 1 ? take(at, w, s) : 0;
+        const int64_t ss = take(at, s, s), pp = take(at, s, s);
+        l.t = take(at, s, s);
         for (int k = 0; k <= steps; ++k) {
             l.x[k] = k & 1 ? x1 : x0;
             l.xt[k] = k & 1 ? x1t : x0t;
@@ -74,7 +82,7 @@ struct Batch {
     std::vector<size_t> mats;  // indices into the caller's list, shape by shape
     struct Shape {
         int s, w, mat0, count;
-        int64_t base;
+        int64_t base, kept_base;
         Layout lay;
     };
     std::vector<Shape> shapes;
@@ -120,9 +128,12 @@ int smallVariant(int64_t s, int64_t w) {
     return 0;
 }
 
-int plan(size_t num, const int64_t *rows, const int64_t *cols, int steps, bool backward,
-         std::vector<Batch> &batches, std::vector<SmallBatch> &smalls, int64_t &bytes) {
-    bytes = 0;
+// `bytes`: of the workspace; `kept`: of the kept iterates, which lie in the order of the sorted list and
+// so do not depend on how it falls into batches.
+int plan(size_t num, const int64_t *rows, const int64_t *cols, int steps, Purpose purpose,
+         std::vector<Batch> &batches, std::vector<SmallBatch> &smalls, int64_t &bytes, int64_t &kept_bytes) {
+    const bool backward = purpose == kGradient || purpose == kGradientKept;
+    bytes = kept_bytes = 0;
     std::vector<size_t> order;
     order.reserve(num);
     for (size_t i = 0; i < num; ++i) {
@@ -157,7 +168,7 @@ int plan(size_t num, const int64_t *rows, const int64_t *cols, int steps, bool b
     for (size_t k = 0; k < order.size(); ++k) {
         const auto shape = key(order[k]);
         const bool same = k && shape == key(order[k - 1]);
-        if (!same) lay = layoutOf((int)shape.first, (int)shape.second, steps, backward);
+        if (!same) lay = layoutOf((int)shape.first, (int)shape.second, steps, purpose);
         Batch *b = batches.empty() ? nullptr : &batches.back();
         if (!b || b->bytes + lay.bytes > kBatchBytes || (int)b->mats.size() == kBatchMats ||
             (!same && (int)b->shapes.size() == kMaxGroups)) {
@@ -166,10 +177,11 @@ int plan(size_t num, const int64_t *rows, const int64_t *cols, int steps, bool b
         }
         if (b->shapes.empty() || !same)
             b->shapes.push_back({(int)shape.first, (int)shape.second, (int)b->mats.size(), 0,
-                                 b->bytes, lay});
+                                 b->bytes, kept_bytes, lay});
         b->shapes.back().count++;
         b->mats.push_back(order[k]);
         b->bytes += lay.bytes;
+        kept_bytes += lay.kept_bytes;
     }
     for (const Batch &b : batches)
         bytes = std::max(bytes, headOf((int64_t)b.mats.size(), stagesOf(steps, backward)).regions + b.bytes);
@@ -270,7 +282,7 @@ struct Call {
     float *const *scales;
     const toa_muon_hyper *hyper;
     toa_muon_series series;
-    char *ws;
+    char *ws, *kept;  // kept: or null
     hipStream_t stream;
 };
 
@@ -350,7 +362,7 @@ class Run {
   public:
     Run(const Call &c, const Batch &b, const Series &series)
         : c_(c), b_(b), steps_(c.series.steps), back_(c.what == kBackward),
-          stages_(stagesOf(steps_, back_)), head_(headOf((int64_t)b.mats.size(), stages_)),
+          keep_(c.kept != nullptr), stages_(stagesOf(steps_, back_)), head_(headOf((int64_t)b.mats.size(), stages_)),
           f_{series} {
         f_.q.paired = pairedSteps();
     }
@@ -359,11 +371,15 @@ class Run {
         TRY(fillRecords(c_, b_.mats, (MatRec *)(c_.ws + head_.recs)));
         TRY(sums());
         TRY(factors());
-        TRY(pack(back_ ? 0 : -1));
-        int from = 0;  // which of the two buffers holds X
-        for (int k = 0; k < f_.q.paired; k += 2, from ^= 1) TRY(forwardPair(k, from));
-        for (int k = f_.q.paired; k < steps_; ++k, from ^= 1) TRY(forwardStep(k, back_ ? k : from));
+        if (!back_ || !keep_) {
+            TRY(pack(false));
+            int from = 0;  // which of the two buffers holds X
+            for (int k = 0; k < f_.q.paired; k += 2, from ^= 1) TRY(forwardPair(k, from));
+            for (int k = f_.q.paired; k < steps_; ++k, from ^= 1)
+                TRY(forwardStep(k, back_ || keep_ ? k : from));
+        }
         if (!back_) return 0;
+        TRY(pack(true));
         for (int k = steps_ - 1; k >= 0; --k) TRY(backwardStep(k));
         return tail();
     }
@@ -371,7 +387,7 @@ class Run {
   private:
     // whether step k's operands carry 22 bits (see the header)
     bool split(int k) const {
-        return back_ || c_.dtype != TOA_BF16 || k < f_.q.paired || k < steps_ - 2;
+        return back_ || keep_ || c_.dtype != TOA_BF16 || k < f_.q.paired || k < steps_ - 2;
     }
 
     // Steps taken by twos: where that is less work for the batch (see muon_kernels.hpp).
@@ -382,7 +398,7 @@ class Run {
             one += n * (6.0 * s.w + 2.0 * s.s);
             two += n * (3.0 * s.w + 5.0 * s.s);
         }
-        return !back_ && two < 0.95 * one ? steps_ / 2 * 2 : 0;
+        return !back_ && !keep_ && two < 0.95 * one ? steps_ / 2 * 2 : 0;
     }
 
     const MatRec *recs() const { return (const MatRec *)(c_.ws + head_.recs); }
@@ -394,7 +410,8 @@ class Run {
         for (int k = 0; k < sh.n; ++k) {
             const auto &s = b_.shapes[k];
             const int64_t tiles = tilesOf(s, k);
-            sh.g[k] = {head_.regions + s.base, s.lay.bytes, s.s, s.w, s.mat0,
+            sh.g[k] = {head_.regions + s.base, s.lay.bytes, s.kept_base, s.lay.kept_bytes,
+                       s.s, s.w, s.mat0,
                        (int)at, (int)tiles, (int)(tiles * s.count)};
             at += tiles * s.count;
             if (at > std::numeric_limits<int>::max()) return at;
@@ -441,32 +458,28 @@ class Run {
         return launch(factors_kernel, (int64_t)b_.mats.size(), 256, c_.stream, f_);
     }
 
-    int pack(int y) {
+    // The cotangent, or the matrix itself, as operands.
+    int pack(bool cotangent) {
         PackArgs a{};
         a.recs = recs();
         a.norms = (const MatNorm *)(c_.ws + head_.norms);
         a.ws = c_.ws;
+        a.kept = c_.kept;
         a.split = split(0);
         a.step = stepOf(c_);
         const int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int k) {
-            a.off[k] = s.lay.x[0];
-            a.off_t[k] = s.lay.xt[0];
+            a.off[k] = cotangent ? s.lay.y[0] : s.lay.x[0];
+            a.off_t[k] = cotangent ? s.lay.yt[0] : s.lay.xt[0];
             return padded(s.s) / 64 * (padded(s.w) / 64);
         });
         return withType(c_.dtype, [&](auto t) {
             using T = decltype(t);
-            if (c_.what == kStep)
-                return launch(c_.momentum_dtype == TOA_I8      ? pack_kernel<T, kPackMI8>
-                              : c_.momentum_dtype == c_.dtype ? pack_kernel<T, kPackM>
-                                                               : pack_kernel<T, kPackMF32>,
-                              grid, 256, c_.stream, a);
-            TRY(launch(pack_kernel<T, kPackG>, grid, 256, c_.stream, a));
-            if (y < 0) return 0;
-            for (int k = 0; k < a.sh.n; ++k) {
-                a.off[k] = b_.shapes[k].lay.y[y];
-                a.off_t[k] = b_.shapes[k].lay.yt[y];
-            }
-            return launch(pack_kernel<T, kPackAux>, grid, 256, c_.stream, a);
+            return launch(cotangent                          ? pack_kernel<T, kPackAux>
+                          : c_.what != kStep               ? pack_kernel<T, kPackG>
+                          : c_.momentum_dtype == TOA_I8    ? pack_kernel<T, kPackMI8>
+                          : c_.momentum_dtype == c_.dtype ? pack_kernel<T, kPackM>
+                                                           : pack_kernel<T, kPackMF32>,
+                          grid, 256, c_.stream, a);
         });
     }
 
@@ -476,6 +489,7 @@ class Run {
     int product(int stage, int k, bool split_out, bool symmetric, int mode, F operands) {
         GemmArgs a{};
         a.ws = c_.ws;
+        a.kept = c_.kept;
         a.recs = recs();
         a.factors = (const Factor *)(c_.ws + head_.factors);
         a.stages = stages_;
@@ -635,7 +649,7 @@ class Run {
             p.d = l.p[k];
         }));
         if (back_ && k + 1 == steps_) return 0;  // the result itself is not needed
-        return advance(stage + 2, k, k + 1, from, back_ ? k + 1 : from ^ 1,
+        return advance(stage + 2, k, k + 1, from, back_ || keep_ ? k + 1 : from ^ 1,
                        [&](const Layout &l) { return l.p[k]; });
     }
 
@@ -705,6 +719,7 @@ class Run {
         a.recs = recs();
         a.norms = (const MatNorm *)(c_.ws + head_.norms);
         a.ws = c_.ws;
+        a.kept = c_.kept;
         a.parts = (double *)(c_.ws + head_.parts);
         int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int k) {
             a.y[k] = s.lay.yf;
@@ -728,13 +743,13 @@ class Run {
     const Call &c_;
     const Batch &b_;
     const int steps_;
-    const bool back_;
+    const bool back_, keep_;
     const int stages_;
     const Head head_;
     FactorArgs f_;
 };
 
-int run(const Call &call, size_t num, const void *workspace, size_t workspace_bytes) {
+int run(const Call &call, size_t num, size_t workspace_bytes, size_t kept_bytes = 0) {
     if (call.dtype != TOA_F32 && call.dtype != TOA_F16 && call.dtype != TOA_BF16) return TOA_EDTYPE;
     Series series{};
     TRY(boundsOf(call.series, series));
@@ -742,9 +757,10 @@ int run(const Call &call, size_t num, const void *workspace, size_t workspace_by
     if (!call.rows || !call.cols) return TOA_ENULL;
     std::vector<Batch> batches;
     std::vector<SmallBatch> smalls;
-    int64_t bytes;
-    TRY(plan(num, call.rows, call.cols, call.series.steps, call.what == kBackward, batches, smalls,
-             bytes));
+    int64_t bytes, kept;
+    const Purpose purpose = call.what == kBackward ? (call.kept ? kGradientKept : kGradient)
+                                                   : (call.kept ? kForwardKeep : kForward);
+    TRY(plan(num, call.rows, call.cols, call.series.steps, purpose, batches, smalls, bytes, kept));
     if (batches.empty() && smalls.empty()) return 0;
     if (!call.g || !call.out || (call.what != kOrthogonalize && !call.aux)) return TOA_ENULL;
     for (size_t i = 0; i < num; ++i)
@@ -752,8 +768,9 @@ int run(const Call &call, size_t num, const void *workspace, size_t workspace_by
             (!call.g[i].data || !call.out[i].data || (call.aux && !call.aux[i].data) ||
              (call.momentum_dtype == TOA_I8 && (!call.scales || !call.scales[i]))))
             return TOA_ENULL;
-    if (bytes && !workspace) return TOA_ENULL;
-    if (workspace_bytes < (size_t)bytes || ((uintptr_t)workspace & 255)) return TOA_EWORKSPACE;
+    if (bytes && !call.ws) return TOA_ENULL;
+    if (workspace_bytes < (size_t)bytes || ((uintptr_t)call.ws & 255)) return TOA_EWORKSPACE;
+    if (call.kept && (kept_bytes < (size_t)kept || ((uintptr_t)call.kept & 255))) return TOA_EWORKSPACE;
     // (every launch of every batch is checked against the grid's limits before the first goes out)
     for (const Batch &b : batches)
         for (const auto &s : b.shapes)
@@ -765,22 +782,24 @@ int run(const Call &call, size_t num, const void *workspace, size_t workspace_by
     return 0;
 }
 
-size_t workspaceOf(int dtype, size_t num, const int64_t *rows, const int64_t *cols, int steps,
-                   bool backward, int *status) {
+// Of the workspace, or (`kept`) of the kept iterates.
+size_t bytesOf(int dtype, size_t num, const int64_t *rows, const int64_t *cols, int steps,
+               Purpose purpose, bool kept, int *status) {
     int rc = 0;
-    int64_t bytes = 0;
+    int64_t bytes[2] = {};
     try {
         std::vector<Batch> batches;
         std::vector<SmallBatch> smalls;
         rc = dtype != TOA_F32 && dtype != TOA_F16 && dtype != TOA_BF16 ? TOA_EDTYPE
              : steps < 1 || steps > kMaxSteps                        ? TOA_EVALUE
-             : num && (!rows || !cols)                               ? TOA_ENULL
-                                       : plan(num, rows, cols, steps, backward, batches, smalls, bytes);
+             : num && (!rows || !cols)
+                 ? TOA_ENULL
+                 : plan(num, rows, cols, steps, purpose, batches, smalls, bytes[0], bytes[1]);
     } catch (...) {
         rc = (int)hipErrorOutOfMemory;
     }
     if (status) *status = rc;
-    return rc ? 0 : (size_t)bytes;
+    return rc ? 0 : (size_t)bytes[kept];
 }
 
 // Launches over lists of flat arrays, 64 to a launch.
@@ -844,24 +863,29 @@ const char *toa_muon_error_string(int code) {
 }
 
 size_t toa_muon_orthogonalize_workspace(int dtype, size_t num, const int64_t *rows,
-                                        const int64_t *cols, int steps, int *status) {
-    return workspaceOf(dtype, num, rows, cols, steps, false, status);
+                                        const int64_t *cols, int steps, int keep, int *status) {
+    return bytesOf(dtype, num, rows, cols, steps, keep ? kForwardKeep : kForward, false, status);
 }
 
 size_t toa_muon_backward_workspace(int dtype, size_t num, const int64_t *rows, const int64_t *cols,
-                                   int steps, int *status) {
-    return workspaceOf(dtype, num, rows, cols, steps, true, status);
+                                   int steps, int kept, int *status) {
+    return bytesOf(dtype, num, rows, cols, steps, kept ? kGradientKept : kGradient, false, status);
+}
+
+size_t toa_muon_kept_bytes(int dtype, size_t num, const int64_t *rows, const int64_t *cols, int steps,
+                           int *status) {
+    return bytesOf(dtype, num, rows, cols, steps, kForwardKeep, true, status);
 }
 
 int toa_muon_orthogonalize_multi(int dtype, size_t num, const int64_t *rows, const int64_t *cols,
                                  const toa_muon_view *in, const toa_muon_view *out,
-                                 const toa_muon_series *series, void *workspace,
-                                 size_t workspace_bytes, void *stream) {
+                                 const toa_muon_series *series, void *kept, size_t kept_bytes,
+                                 void *workspace, size_t workspace_bytes, void *stream) {
     return guarded([&]() -> int {
         TRY(checkSeries(series));
         const Call c{kOrthogonalize, dtype, dtype, rows, cols, in, nullptr, out, nullptr, nullptr,
-                     *series, (char *)workspace, (hipStream_t)stream};
-        return run(c, num, workspace, workspace_bytes);
+                     *series, (char *)workspace, (char *)kept, (hipStream_t)stream};
+        return run(c, num, workspace_bytes, kept_bytes);
     });
 }
 
@@ -869,13 +893,15 @@ int toa_muon_orthogonalize_backward_multi(int dtype, size_t num, const int64_t *
                                           const int64_t *cols, const toa_muon_view *in,
                                           const toa_muon_view *grad_out,
                                           const toa_muon_view *grad_in,
-                                          const toa_muon_series *series, void *workspace,
+                                          const toa_muon_series *series, const void *kept,
+                                          size_t kept_bytes, void *workspace,
                                           size_t workspace_bytes, void *stream) {
     return guarded([&]() -> int {
         TRY(checkSeries(series));
         const Call c{kBackward, dtype, dtype, rows, cols, in, grad_out, grad_in, nullptr, nullptr,
-                     *series, (char *)workspace, (hipStream_t)stream};
-        return run(c, num, workspace, workspace_bytes);
+                     *series, (char *)workspace, (char *)const_cast<void *>(kept),
+                     (hipStream_t)stream};
+        return run(c, num, workspace_bytes, kept_bytes);
     });
 }
 
@@ -894,8 +920,8 @@ int toa_muon_step_multi(int dtype, int momentum_dtype, size_t num, const int64_t
             (hyper->apply && !(std::isfinite(hyper->lr) && std::isfinite(hyper->weight_decay))))
             return TOA_EVALUE;
         const Call c{kStep, dtype, momentum_dtype, rows, cols, grads, momentum, out, scales, hyper,
-                     *series, (char *)workspace, (hipStream_t)stream};
-        return run(c, num, workspace, workspace_bytes);
+                     *series, (char *)workspace, nullptr, (hipStream_t)stream};
+        return run(c, num, workspace_bytes);
     });
 }
 
