@@ -753,8 +753,10 @@ def run_gpu(cfg_id, steps, warmup, operator_preheat=None, state='init'):
             step()
         torch.cuda.synchronize()
         extra['preheat_operator_launches_on_the_timed_arrays'] = op_launches
-        extra['load_order_kept_for_this_call_site'] = lib.toa_adam_tuned_load_order(
-            code, pu, pm, pv, total)
+        # an order of the staged program (0-3), or the plain schedule (4), which has none
+        kept = lib.toa_adam_tuned_load_order(code, pu, pm, pv, total)
+        extra['load_order_kept_for_this_call_site'] = kept if kept < 4 else -1
+        extra['plain_schedule_kept_for_this_call_site'] = kept == 4
     elif op_launches and cfg.get('fused_step'):
         for _ in range(op_launches):
             step()
