@@ -15,8 +15,9 @@ using namespace toa_muon;
 namespace {
 
 // A batch's regions stay below this (one matrix alone may be larger).  Large batches fill whole
-// rounds of tiles: 96 matrices of 1024^2 take 7.3 ms in one batch, 8.1 in three, 8.9 in eight of a
-// size that stays in the 256 MB of last-level cache.
+// rounds of tiles: 96 matrices of 1024^2 take 7.1 ms in one batch and 7.9 in three, GPT-2-medium's 144
+// matrices (bfloat16 step) 13.2 ms in two batches, 14.2 in 1 GiB and 17.4 in 256 MiB, which stay in the
+// last-level cache.  (In one of 8 GiB they take 13.9: pairs of steps then serve the square ones too.)
 constexpr int64_t kBatchBytes = (int64_t)4 << 30;
 constexpr int kBatchMats = 4096;
 constexpr int64_t kMaxDim = (int64_t)1 << 20;
@@ -426,7 +427,9 @@ class Run {
         a.step = stepOf(c_);
         const int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int k) {
             const int64_t n = (int64_t)s.s * s.w;
-            int64_t per = std::max<int64_t>(8192, (n + kMaxParts - 1) / kMaxParts);
+            // (at least eight elements a thread: more in a row, with few of them at work, cost a
+            // list of odd small matrices 10 us)
+            int64_t per = std::max<int64_t>(2048, (n + kMaxParts - 1) / kMaxParts);
             per = (per + 2047) / 2048 * 2048;
             a.per[k] = per;
             f_.nparts[k] = (int)((n + per - 1) / per);
@@ -724,7 +727,7 @@ class Run {
         int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int k) {
             a.y[k] = s.lay.yf;
             a.x[k] = s.lay.x[0];
-            int64_t parts = std::min<int64_t>(kMaxParts, ((int64_t)s.s * s.w + 8191) / 8192);
+            int64_t parts = std::min<int64_t>(kMaxParts, ((int64_t)s.s * s.w + 2047) / 2048);
             const int64_t cells = (s.s + 31) / 32 * (padded(s.w) / 32);
             a.per[k] = (cells + parts - 1) / parts;
             a.nparts[k] = (int)((cells + a.per[k] - 1) / a.per[k]);
