@@ -65,8 +65,8 @@ typedef struct {
     int64_t row_stride, col_stride; /* in elements */
 } toa_muon_view;
 
-/* 1 <= steps <= 32; coefficients finite, and such that no iterate can grow beyond 2^20 from a
- * start of norm 1 (TOA_EVALUE otherwise); eps >= 0. */
+/* 1 <= steps <= 32; coefficients finite, and such that no iterate but the last can grow beyond 64
+ * from a start of norm 1 (TOA_EVALUE otherwise); eps >= 0. */
 typedef struct {
     int steps;
     double a, b, c, eps;
@@ -75,20 +75,21 @@ typedef struct {
 TOA_API int toa_muon_abi_version(void);
 TOA_API const char *toa_muon_error_string(int code);
 
-/* Bytes of workspace for a list; 0 for a list without elements.  TOA_ESIZE through `status`
- * (may be NULL) where a dimension is beyond 2^20. */
+/* Bytes of workspace for a list; 0 for a list without elements.  What is refused comes through
+ * `status` (may be NULL): TOA_ESIZE where a dimension is beyond 2^20. */
 TOA_API size_t toa_muon_orthogonalize_workspace(int dtype, size_t num, const int64_t *rows,
-                                                const int64_t *cols, int steps, int keep,
-                                                int *status);
+                                                const int64_t *cols, const toa_muon_series *series,
+                                                int keep, int *status);
 TOA_API size_t toa_muon_backward_workspace(int dtype, size_t num, const int64_t *rows,
-                                           const int64_t *cols, int steps, int kept, int *status);
+                                           const int64_t *cols, const toa_muon_series *series,
+                                           int kept, int *status);
 
 /* What the gradient needs of the forward pass -- every iterate and its products -- can be kept
  * between the two: bytes of that buffer (256-byte aligned) for a list, about 8 bytes for each
  * element of a matrix and of the square of its shorter side, for each step; small matrices, whose
- * iterates are made again faster than they are read, need none. */
+ * iterates are made again faster than they are read, need none in a short series. */
 TOA_API size_t toa_muon_kept_bytes(int dtype, size_t num, const int64_t *rows, const int64_t *cols,
-                                   int steps, int *status);
+                                   const toa_muon_series *series, int *status);
 
 /* kept: where the iterates go, or NULL.  keep / kept of the workspace functions says which. */
 TOA_API int toa_muon_orthogonalize_multi(int dtype, size_t num, const int64_t *rows,

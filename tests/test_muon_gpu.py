@@ -250,12 +250,31 @@ def test_gradient_steps(steps):
                        eps=0.25)
 
 
+@pytest.mark.parametrize('steps,coefficients', [
+    (8, plain.COEFFICIENTS), (12, plain.COEFFICIENTS), (20, plain.COEFFICIENTS), (32, (1.5, -0.5, 0.0)),
+    (16, (2.0, -1.5, 0.5)), (3, (5.0, -6.0, 2.0))])
+@pytest.mark.parametrize('m,n', [(5, 9), (20, 50), (70, 300)])
+def test_gradient_of_long_series(m, n, steps, coefficients):
+    """The slopes' product runs far ahead of what a cotangent really grows by."""
+    for rank in (None, 3):
+        x = randn(m, n, seed=1) if rank is None else low_rank(m, n, rank) + 0.05 * randn(m, n, seed=4)
+        check_gradient(x, randn(m, n, seed=2), F32, f'rank {rank}', steps=steps,
+                       coefficients=coefficients)
+    # a cotangent of zeros, and one of a NaN, among others
+    x = [randn(m, n, seed=k).cuda() for k in range(3)]
+    dy = [torch.zeros_like(x[0]), torch.full_like(x[1], float('nan')), randn(m, n, seed=7).cuda()]
+    kw = dict(steps=steps, coefficients=coefficients)
+    dx = muon_op.orthogonalize_backward_multi(dy, x, **kw)
+    assert not dx[0].any() and dx[1].isnan().all()
+    assert torch.equal(dx[2], muon_op.orthogonalize_backward_multi(dy[2:], x[2:], **kw)[0])
+
+
 @pytest.mark.parametrize('dtype', TYPES)
 def test_kept_iterates_give_the_same_gradient(dtype):
     """The gradient from kept iterates is that from iterates made again, bit for bit (both take every
     step by itself with 22-bit operands); the buffer is only read, and serves as often as asked."""
     shapes = [(90, 400), (20, 30), (300, 130), (90, 400), (65, 65), (0, 5)]
-    for kw in (dict(), dict(steps=1), dict(steps=4, coefficients=(1.5, -0.5, 0.0))):
+    for kw in (dict(steps=9), dict(steps=1), dict(steps=4, coefficients=(1.5, -0.5, 0.0)), dict()):
         xs = [randn(*s, dtype=dtype, seed=k).cuda() for k, s in enumerate(shapes)]
         dys = [randn(*s, dtype=dtype, seed=k + 20).cuda() for k, s in enumerate(shapes)]
         ys, kept = muon_op.orthogonalize_keep_multi(xs, 1 << 30, **kw)
@@ -551,6 +570,7 @@ def test_refusals():
         lambda: orthogonalize(x, steps=33), lambda: orthogonalize(x, eps=-1.0),
         lambda: orthogonalize(x, eps=float('nan')),
         lambda: orthogonalize(x, coefficients=(50.0, 1.0, 1.0)),
+        lambda: orthogonalize(x, steps=3, coefficients=(6.0, -9.0, 4.0)),  # may reach 68
         lambda: orthogonalize(x, coefficients=(float('nan'), 1.0, 1.0)),
         lambda: muon_op.orthogonalize_multi([x, x.half()]),
         lambda: muon_op.orthogonalize_multi([x, x.cpu()]),

@@ -86,11 +86,11 @@ def test_argument_errors_need_no_device(lib):
     assert orth(lib, dtype=F64) == EDTYPE and orth(lib, dtype=I8) == EDTYPE
     assert orth(lib) == ENULL  # the matrix ...
     assert orth(lib, rows=(100,), cols=(100,), data=256) == ENULL  # ... or the workspace
-    need = lib.toa_muon_orthogonalize_workspace(F32, ctypes.c_size_t(1), sides(100), sides(100), 5,
-                                                0, None)
+    need = lib.toa_muon_orthogonalize_workspace(F32, ctypes.c_size_t(1), sides(100), sides(100),
+                                                series(), 0, None)
     assert orth(lib, rows=(100,), cols=(100,), data=256, workspace=256, size=need - 1) == EWORKSPACE
     assert orth(lib, rows=(100,), cols=(100,), data=256, workspace=264, size=need) == EWORKSPACE
-    keep = lib.toa_muon_kept_bytes(F32, ctypes.c_size_t(1), sides(100), sides(100), 5, None)
+    keep = lib.toa_muon_kept_bytes(F32, ctypes.c_size_t(1), sides(100), sides(100), series(), None)
     assert keep == 5 * 4 * 128 * 128 * 4  # X, its transpose, S and P of five steps
     for kept, short in ((256, 1), (264, 0)):
         assert orth(lib, rows=(100,), cols=(100,), data=256, kept=kept, kept_size=keep - short,
@@ -101,6 +101,15 @@ def test_argument_errors_need_no_device(lib):
     for bad in (dict(steps=0), dict(steps=33), dict(a=nan), dict(b=inf), dict(eps=-1.0),
                 dict(eps=nan), dict(a=100.0), dict(c=1e6)):
         assert orth(lib, q=series(**bad)) == EVALUE, bad
+        status = ctypes.c_int(0)
+        lists = F32, ctypes.c_size_t(1), sides(100), sides(100), series(**bad)
+        for size in (lambda: lib.toa_muon_orthogonalize_workspace(*lists, 0, ctypes.byref(status)),
+                     lambda: lib.toa_muon_kept_bytes(*lists, ctypes.byref(status))):
+            status.value = 0
+            assert size() == 0 and status.value == EVALUE, bad
+    # the last iterate may grow, as it is not multiplied again
+    assert orth(lib, rows=(0,), cols=(0,), q=series(steps=1, a=100.0)) == 0
+    assert orth(lib, rows=(0,), cols=(0,), q=series(steps=2, a=100.0)) == EVALUE
     assert lib.toa_muon_orthogonalize_multi(F32, ctypes.c_size_t(0), None, None, None, None, None,
                                             None, ctypes.c_size_t(0), None, ctypes.c_size_t(0),
                                             None) == ENULL
@@ -125,7 +134,7 @@ def test_step_arguments(lib):
 def test_workspace_sizes(lib):
     def size(rows, cols, steps=5, which='orthogonalize', dtype=F32, keep=0):
         status = ctypes.c_int(99)
-        lists = dtype, ctypes.c_size_t(len(rows)), sides(*rows), sides(*cols), steps
+        lists = dtype, ctypes.c_size_t(len(rows)), sides(*rows), sides(*cols), series(steps)
         if which == 'kept':
             return lib.toa_muon_kept_bytes(*lists, ctypes.byref(status)), status.value
         n = getattr(lib, f'toa_muon_{which}_workspace')(*lists, keep, ctypes.byref(status))
@@ -144,6 +153,8 @@ def test_workspace_sizes(lib):
     assert whole - rest == kept == 5 * 4 * 4 << 20
     assert size((32, 1024), (288, 1024), which='kept')[0] == kept
     assert size((32,), (288,), which='kept') == (0, 0)
+    # (in a long series the way back measures its norms, which the small form does not)
+    assert size((32,), (288,), which='kept', steps=8)[0] > 0
     assert size((1024,), (1024,), keep=1)[0] < size((1024,), (1024,))[0]
     assert size((4,), (4,), steps=0)[1] == EVALUE and size((4,), (4,), dtype=F64)[1] == EDTYPE
     assert size((1 << 21,), (4,))[1] == ESIZE

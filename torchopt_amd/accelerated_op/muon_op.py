@@ -107,8 +107,8 @@ def orthogonalize(
     Args:
         matrices: GPU tensors of float32, float16 or bfloat16, any strides.
         steps: how often the polynomial is applied, 1 to 32.
-        coefficients: ``(a, b, c)``.  Coefficients under which the iterates could grow beyond
-            2^20 are refused.
+        coefficients: ``(a, b, c)``.  Coefficients under which an iterate but the last could grow
+            beyond 64 are refused.
         eps: added to the Frobenius norm.
 
     Returns:

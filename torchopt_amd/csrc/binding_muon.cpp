@@ -101,12 +101,12 @@ std::pair<TensorList, c10::optional<Tensor>> orthogonalizeKeepMulti(const py::ob
     int status = 0;
     size_t kept_bytes = 0;
     if (keep > 0) {
-        kept_bytes = toa_muon_kept_bytes(code, m.rows.size(), m.rows.data(), m.cols.data(), steps, &status);
+        kept_bytes = toa_muon_kept_bytes(code, m.rows.size(), m.rows.data(), m.cols.data(), &series, &status);
         if (kept_bytes > (size_t)keep) kept_bytes = 0;
         if (kept_bytes) kept = workspaceFor(name, in[0], kept_bytes, status);
     }
     const size_t bytes = toa_muon_orthogonalize_workspace(
-        code, m.rows.size(), m.rows.data(), m.cols.data(), steps, kept_bytes != 0, &status);
+        code, m.rows.size(), m.rows.data(), m.cols.data(), &series, kept_bytes != 0, &status);
     const Tensor ws = workspaceFor(name, in[0], bytes, status);
     check(toa_muon_orthogonalize_multi(code, m.rows.size(), m.rows.data(), m.cols.data(),
                                        viewsOf(in, m.rows.size()).data(),
@@ -145,14 +145,14 @@ TensorList orthogonalizeBackwardMulti(const py::object &grads_o, const py::objec
     int status;
     size_t kept_bytes = 0;
     if (kept) {
-        kept_bytes = toa_muon_kept_bytes(code, m.rows.size(), m.rows.data(), m.cols.data(), steps, &status);
+        kept_bytes = toa_muon_kept_bytes(code, m.rows.size(), m.rows.data(), m.cols.data(), &series, &status);
         check(status, name);
         TORCH_CHECK(kept->device() == in[0].device() && kept->scalar_type() == at::kByte &&
                         kept->is_contiguous() && kept_bytes && (size_t)kept->numel() == kept_bytes,
                     name, ": kept is not what the forward pass kept of these inputs");
     }
     const size_t bytes = toa_muon_backward_workspace(code, m.rows.size(), m.rows.data(),
-                                                     m.cols.data(), steps, kept_bytes != 0, &status);
+                                                     m.cols.data(), &series, kept_bytes != 0, &status);
     const Tensor ws = workspaceFor(name, in[0], bytes, status);
     check(toa_muon_orthogonalize_backward_multi(
               code, m.rows.size(), m.rows.data(), m.cols.data(), viewsOf(in, m.rows.size()).data(),
@@ -279,7 +279,7 @@ void stepMulti(const char *name, const TensorList &out, TensorList grads, const 
     const OnDeviceOf dev(out[0]);
     int status;
     const size_t bytes = toa_muon_orthogonalize_workspace(code, rows.size(), rows.data(),
-                                                          cols.data(), series.steps, 0, &status);
+                                                          cols.data(), &series, 0, &status);
     const Tensor ws = workspaceFor(name, out[0], bytes, status);
     check(toa_muon_step_multi(code, kept_code, rows.size(), rows.data(), cols.data(), vo.data(),
                               vg.data(), vm.data(), blocks ? vs.data() : nullptr, &hyper, &series,

@@ -75,6 +75,8 @@ struct MatNorm {
     double y_scale;    // 2^e for the cotangent
     double size;       // |G|_F
     double plus;       // |G|_F + eps
+    double y_size;     // |Y|_F of the cotangent that was measured last,
+    int y_step, y_exp; // of which iterate it is, and the power of two it is stored with
 };
 
 struct Group {         // matrices of one shape
@@ -383,6 +385,7 @@ struct FactorArgs {
     Factor *factors;                // [matrix][stages]
     int stages;
     int nparts[kMaxGroups], mat_end[kMaxGroups], ngroups;
+    int measured;                   // parts_y are of this iterate's cotangent as it is stored, or -1
 };
 
 // The power of two that takes a bound to at most 2^14.
@@ -414,10 +417,13 @@ struct SeriesTable {
 struct Bounds {
     const Series &q;
     const SeriesTable &table;
-    const double start, ysize;
+    const double start;
+    double ysize;       // of the cotangent of X_ystep, which is stored times 2^yexp
+    int ystep, yexp_;
     __device__ Bounds(const Series &q_, const SeriesTable &table_, double size, double ysize_)
         : q(q_), table(table_), start(startOf(size, q_.eps)),
-          ysize(ysize_ == ysize_ && ysize_ < 1e300 ? ysize_ : 1.0) {}
+          ysize(ysize_ == ysize_ && ysize_ < 1e300 ? ysize_ : 1.0), ystep(q_.steps),
+          yexp_(expOf(ysize)) {}
     __device__ double x(int i) const {  // of X_i
         double grown = start;
         for (int j = 0; j < i; ++j) grown *= table.r[j];
@@ -425,14 +431,15 @@ struct Bounds {
     }
     __device__ double y(int i) const {  // of the cotangent of X_i
         double v = ysize;
-        for (int j = q.steps - 1; j >= i; --j) v *= table.d[j];
+        for (int j = ystep - 1; j >= i; --j) v *= table.d[j];
         return v;
     }
+    __device__ int yexp(int i) const { return i == ystep ? yexp_ : expOf(y(i)); }
 };
 
 __device__ inline MatNorm normOf(const Bounds &b, double size) {
     const double plus = size + b.q.eps;
-    return {ldexp(1.0 / plus, expOf(b.x(0))), ldexp(1.0, expOf(b.y(b.q.steps))), size, plus};
+    return {ldexp(1.0 / plus, expOf(b.x(0))), ldexp(1.0, b.yexp_), size, plus, b.ysize, b.ystep, b.yexp_};
 }
 
 // Factors of a step: 4 of its own, so 8 of a pair's; in the gradient 3 more, behind all of those.
@@ -471,7 +478,7 @@ __device__ inline void stepFactors(const Bounds &b, int t, Factor *f, Factor *ba
     f[2] = {ldexpf(1.f, ex1 - ep - ex), 0.f, 1.f, 0.f};
     if (!back) return;
     const double y1 = b.y(t + 1);
-    const int ey1 = expOf(y1), ey = t ? expOf(b.y(t)) : 0;
+    const int ey1 = b.yexp(t + 1), ey = t ? b.yexp(t) : 0;
     // (where N X is nothing beside P Y, N needs no more range than to be added to it)
     const int em = expOf(2.0 * x * y1);
     const int en = min(expOf((ab + 2.0 * ac * x2) * 2.0 * x * y1), ep + ey1 - ex + 24);
@@ -489,13 +496,30 @@ __global__ __launch_bounds__(256) void factors_kernel(FactorArgs a) {
     int k = 0;
     while (k + 1 < a.ngroups && mat >= a.mat_end[k]) ++k;
     const int np = a.nparts[k];
-    const double size = sqrt(blockSum(t < np ? a.parts[(int64_t)mat * kMaxParts + t] : 0.0, lds));
     const double ysize =
         a.parts_y ? sqrt(blockSum(t < np ? a.parts_y[(int64_t)mat * kMaxParts + t] : 0.0, lds)) : 0.0;
+    Factor *f = a.factors + (int64_t)mat * a.stages + kStepFactors * t;
+    if (a.measured >= 0) {
+        // on the way back: bounds of the cotangents from this one on follow its norm
+        MatNorm n = a.norms[mat];
+        Bounds b(a.q, table, n.size, n.y_size);
+        b.ystep = n.y_step;
+        b.yexp_ = n.y_exp;
+        const double bound = b.y(a.measured);
+        b.yexp_ = b.yexp(a.measured);
+        b.ystep = a.measured;
+        const double now = ldexp(ysize, -b.yexp_);
+        b.ysize = now > 0.0 && now < bound ? now : bound;  // (nothing, or NaN: as before)
+        __syncthreads();  // (everybody has read the norms)
+        if (t == 0) a.norms[mat] = normOf(b, n.size);
+        if (t < a.measured)
+            stepFactors(b, t, f, a.factors + (int64_t)mat * a.stages + kStepFactors * a.q.steps + 3 * t);
+        return;
+    }
+    const double size = sqrt(blockSum(t < np ? a.parts[(int64_t)mat * kMaxParts + t] : 0.0, lds));
     const Bounds b(a.q, table, size, ysize);
     if (t == 0) a.norms[mat] = normOf(b, size);
     if (t >= a.q.steps) return;
-    Factor *f = a.factors + (int64_t)mat * a.stages + kStepFactors * t;
     if (t >= a.q.paired)
         stepFactors(b, t, f,
                     a.parts_y ? a.factors + (int64_t)mat * a.stages + kStepFactors * a.q.steps + 3 * t
@@ -1729,13 +1753,13 @@ struct TailArgs {
     const MatRec *recs;
     const MatNorm *norms;
     char *ws, *kept;
-    double *parts;                              // <Y_0, X_0 * 2^e>
-    int64_t y[kMaxGroups], x[kMaxGroups];       // float rows of Y_0; operand rows of X_0
+    double *parts;                              // <Y_0, X_0 * 2^e>, or <X, X>
+    int64_t y[kMaxGroups], x[kMaxGroups];       // float rows of Y_0; X_0 or another operand
     int64_t per[kMaxGroups];                    // dot: cells of 32 x 32 per workgroup
     int nparts[kMaxGroups];
 };
 
-__global__ __launch_bounds__(256) void dot_kernel(TailArgs a) {
+template <bool SQUARE> __global__ __launch_bounds__(256) void dot_kernel(TailArgs a) {
     __shared__ double lds[4];
     int part = blockIdx.x, mat;
     const int gi = findGroup(a.sh, part, mat);
@@ -1755,9 +1779,9 @@ __global__ __launch_bounds__(256) void dot_kernel(TailArgs a) {
         if (i >= g.s || j >= g.w) continue;
         float x[8], y[8];
         loadOperand(chunkOf(region + a.x[gi], ld, i, j, true), x);
-        load8((const float *)(region + a.y[gi]) + i * wp + j, g.w - j, y);
+        if (!SQUARE) load8((const float *)(region + a.y[gi]) + i * wp + j, g.w - j, y);
 #pragma unroll
-        for (int k = 0; k < 8; ++k) sum += (double)x[k] * (double)y[k];
+        for (int k = 0; k < 8; ++k) sum += (double)x[k] * (double)(SQUARE ? x[k] : y[k]);
     }
     sum = blockSum(sum, lds);
     if (threadIdx.x == 0) a.parts[(int64_t)mat * kMaxParts + part] = sum;

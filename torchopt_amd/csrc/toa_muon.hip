@@ -122,6 +122,11 @@ struct SmallBatch {
     int64_t bytes() const { return records() + (int64_t)mats.size() * stride; }
 };
 
+// The way back bounds each cotangent by the one before.  Bounds that run ahead of the truth cost the
+// operands their low bits, so where a bound may have grown by more than this the norm is measured anew
+// (the default coefficients: 392 at their five steps, so never there).
+constexpr double kMaxGrowth = 512.0;
+
 // Rows / 32 of the variant that takes an s x w matrix, or 0.
 int smallVariant(int64_t s, int64_t w) {
     for (int rb = 1; rb <= 2; ++rb)
@@ -131,9 +136,14 @@ int smallVariant(int64_t s, int64_t w) {
 
 // `bytes`: of the workspace; `kept`: of the kept iterates, which lie in the order of the sorted list and
 // so do not depend on how it falls into batches.
-int plan(size_t num, const int64_t *rows, const int64_t *cols, int steps, Purpose purpose,
+int plan(size_t num, const int64_t *rows, const int64_t *cols, const Series &series, Purpose purpose,
          std::vector<Batch> &batches, std::vector<SmallBatch> &smalls, int64_t &bytes, int64_t &kept_bytes) {
     const bool backward = purpose == kGradient || purpose == kGradientKept;
+    const int steps = series.steps;
+    // (small_kernel measures nothing on its way back)
+    double growth = 1.0;
+    for (int k = 1; k < steps; ++k) growth *= series.d[k];
+    const bool small = purpose == kForward || growth <= kMaxGrowth;
     bytes = kept_bytes = 0;
     std::vector<size_t> order;
     order.reserve(num);
@@ -141,7 +151,7 @@ int plan(size_t num, const int64_t *rows, const int64_t *cols, int steps, Purpos
         if (rows[i] < 0 || cols[i] < 0 || rows[i] > kMaxDim || cols[i] > kMaxDim) return TOA_ESIZE;
         if (!rows[i] || !cols[i]) continue;
         const int64_t s = std::min(rows[i], cols[i]), w = std::max(rows[i], cols[i]);
-        const int rb = smallVariant(s, w);
+        const int rb = small ? smallVariant(s, w) : 0;
         if (!rb) {
             order.push_back(i);
             continue;
@@ -225,7 +235,9 @@ int checkSeries(const toa_muon_series *q) {
     return 0;
 }
 
-// Bounds of the iterates from a start of norm 1 (with a hundredth of slack for rounding).
+// Bounds of the iterates from a start of norm 1 (with a hundredth of slack for rounding).  An iterate that
+// may stay far below its bound loses its low bits (beyond 2^18 columns even at 64), so series that may
+// grow further before their last step are refused.
 int boundsOf(const toa_muon_series &q, Series &f) {
     f.a = (float)q.a;
     f.b = (float)q.b;
@@ -239,7 +251,7 @@ int boundsOf(const toa_muon_series &q, Series &f) {
         f.r[k] = std::max(1.01 * largest(q.a, q.b, q.c, 0, f.x[k]), 1e-3);
         f.d[k] = std::max(1.01 * largest(q.a, 3.0 * q.b, 5.0 * q.c, 0, f.x[k]), 1e-3);
         x = std::max(largest(q.a, q.b, q.c, 1, f.x[k]), 1e-6);
-        if (!(x <= 1048576.0)) return TOA_EVALUE;
+        if (k + 1 < q.steps && !(x <= 64.0)) return TOA_EVALUE;
     }
     // completing the square takes c h^2 away from what (X X^T + h I)^2 brings in: a bit of a or so
     // at most
@@ -381,8 +393,16 @@ class Run {
         }
         if (!back_) return 0;
         TRY(pack(true));
-        for (int k = steps_ - 1; k >= 0; --k) TRY(backwardStep(k));
-        return tail();
+        double growth = 1.0;
+        for (int k = steps_ - 1; k >= 0; --k) {
+            if (k && k + 1 < steps_ && growth * f_.q.d[k] > kMaxGrowth) {
+                TRY(measure(k + 1));
+                growth = 1.0;
+            }
+            growth *= f_.q.d[k];
+            TRY(backwardStep(k));
+        }
+        return dots<false>(0);
     }
 
   private:
@@ -458,6 +478,7 @@ class Run {
         f_.norms = (MatNorm *)(c_.ws + head_.norms);
         f_.factors = (Factor *)(c_.ws + head_.factors);
         f_.stages = stages_;
+        f_.measured = -1;
         return launch(factors_kernel, (int64_t)b_.mats.size(), 256, c_.stream, f_);
     }
 
@@ -717,24 +738,42 @@ class Run {
                        });
     }
 
-    int tail() {
+    // Bounds of the cotangents from that of X_k on by its norm.
+    int measure(int k) {
+        TRY(dots<true>(k));
+        f_.measured = k;
+        return launch(factors_kernel, (int64_t)b_.mats.size(), 256, c_.stream, f_);
+    }
+
+    // <Y_0, X_0>, or the squares of the cotangent of X_k.
+    template <bool SQUARE> int dots(int k) {
+        TailArgs a = tailArgs();
+        a.parts = (double *)(c_.ws + (SQUARE ? head_.parts_y : head_.parts));
+        const int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int g) {
+            a.y[g] = s.lay.yf;
+            a.x[g] = SQUARE ? s.lay.y[(steps_ - k) & 1] : s.lay.x[0];
+            const int64_t parts = std::min<int64_t>(kMaxParts, ((int64_t)s.s * s.w + 2047) / 2048);
+            const int64_t cells = (s.s + 31) / 32 * (padded(s.w) / 32);
+            a.per[g] = (cells + parts - 1) / parts;
+            a.nparts[g] = (int)((cells + a.per[g] - 1) / a.per[g]);
+            f_.nparts[g] = a.nparts[g];
+            return (int64_t)a.nparts[g];
+        });
+        TRY(launch(dot_kernel<SQUARE>, grid, 256, c_.stream, a));
+        return SQUARE ? 0 : tail(a);
+    }
+
+    TailArgs tailArgs() const {
         TailArgs a{};
         a.recs = recs();
         a.norms = (const MatNorm *)(c_.ws + head_.norms);
         a.ws = c_.ws;
         a.kept = c_.kept;
-        a.parts = (double *)(c_.ws + head_.parts);
-        int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int k) {
-            a.y[k] = s.lay.yf;
-            a.x[k] = s.lay.x[0];
-            int64_t parts = std::min<int64_t>(kMaxParts, ((int64_t)s.s * s.w + 2047) / 2048);
-            const int64_t cells = (s.s + 31) / 32 * (padded(s.w) / 32);
-            a.per[k] = (cells + parts - 1) / parts;
-            a.nparts[k] = (int)((cells + a.per[k] - 1) / a.per[k]);
-            return (int64_t)a.nparts[k];
-        });
-        TRY(launch(dot_kernel, grid, 256, c_.stream, a));
-        grid = shapes(a.sh, [&](const Batch::Shape &s, int) {
+        return a;
+    }
+
+    int tail(TailArgs &a) {
+        const int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int) {
             return padded(s.s) / 64 * (padded(s.w) / 64);
         });
         return withType(c_.dtype, [&](auto t) {
@@ -763,7 +802,7 @@ int run(const Call &call, size_t num, size_t workspace_bytes, size_t kept_bytes 
     int64_t bytes, kept;
     const Purpose purpose = call.what == kBackward ? (call.kept ? kGradientKept : kGradient)
                                                    : (call.kept ? kForwardKeep : kForward);
-    TRY(plan(num, call.rows, call.cols, call.series.steps, purpose, batches, smalls, bytes, kept));
+    TRY(plan(num, call.rows, call.cols, series, purpose, batches, smalls, bytes, kept));
     if (batches.empty() && smalls.empty()) return 0;
     if (!call.g || !call.out || (call.what != kOrthogonalize && !call.aux)) return TOA_ENULL;
     for (size_t i = 0; i < num; ++i)
@@ -785,22 +824,29 @@ int run(const Call &call, size_t num, size_t workspace_bytes, size_t kept_bytes 
     return 0;
 }
 
-// Of the workspace, or (`kept`) of the kept iterates.
-size_t bytesOf(int dtype, size_t num, const int64_t *rows, const int64_t *cols, int steps,
-               Purpose purpose, bool kept, int *status) {
-    int rc = 0;
-    int64_t bytes[2] = {};
+// Nothing thrown in here may cross the C boundary.
+template <typename F> int guarded(F fn) {
     try {
+        return fn();
+    } catch (...) {
+        return (int)hipErrorOutOfMemory;
+    }
+}
+
+// Of the workspace, or (`kept`) of the kept iterates.
+size_t bytesOf(int dtype, size_t num, const int64_t *rows, const int64_t *cols,
+               const toa_muon_series *q, Purpose purpose, bool kept, int *status) {
+    int64_t bytes[2] = {};
+    const int rc = guarded([&]() -> int {
+        if (dtype != TOA_F32 && dtype != TOA_F16 && dtype != TOA_BF16) return TOA_EDTYPE;
+        TRY(checkSeries(q));
+        Series series{};
+        TRY(boundsOf(*q, series));
+        if (num && (!rows || !cols)) return TOA_ENULL;
         std::vector<Batch> batches;
         std::vector<SmallBatch> smalls;
-        rc = dtype != TOA_F32 && dtype != TOA_F16 && dtype != TOA_BF16 ? TOA_EDTYPE
-             : steps < 1 || steps > kMaxSteps                        ? TOA_EVALUE
-             : num && (!rows || !cols)
-                 ? TOA_ENULL
-                 : plan(num, rows, cols, steps, purpose, batches, smalls, bytes[0], bytes[1]);
-    } catch (...) {
-        rc = (int)hipErrorOutOfMemory;
-    }
+        return plan(num, rows, cols, series, purpose, batches, smalls, bytes[0], bytes[1]);
+    });
     if (status) *status = rc;
     return rc ? 0 : (size_t)bytes[kept];
 }
@@ -837,15 +883,6 @@ int blocks(size_t num, const void *const *in, void *const *out, const float *con
     return 0;
 }
 
-// Nothing thrown in here may cross the C boundary.
-template <typename F> int guarded(F fn) {
-    try {
-        return fn();
-    } catch (...) {
-        return (int)hipErrorOutOfMemory;
-    }
-}
-
 }  // namespace
 
 extern "C" {
@@ -866,18 +903,19 @@ const char *toa_muon_error_string(int code) {
 }
 
 size_t toa_muon_orthogonalize_workspace(int dtype, size_t num, const int64_t *rows,
-                                        const int64_t *cols, int steps, int keep, int *status) {
-    return bytesOf(dtype, num, rows, cols, steps, keep ? kForwardKeep : kForward, false, status);
+                                        const int64_t *cols, const toa_muon_series *series, int keep,
+                                        int *status) {
+    return bytesOf(dtype, num, rows, cols, series, keep ? kForwardKeep : kForward, false, status);
 }
 
 size_t toa_muon_backward_workspace(int dtype, size_t num, const int64_t *rows, const int64_t *cols,
-                                   int steps, int kept, int *status) {
-    return bytesOf(dtype, num, rows, cols, steps, kept ? kGradientKept : kGradient, false, status);
+                                   const toa_muon_series *series, int kept, int *status) {
+    return bytesOf(dtype, num, rows, cols, series, kept ? kGradientKept : kGradient, false, status);
 }
 
-size_t toa_muon_kept_bytes(int dtype, size_t num, const int64_t *rows, const int64_t *cols, int steps,
-                           int *status) {
-    return bytesOf(dtype, num, rows, cols, steps, kForwardKeep, true, status);
+size_t toa_muon_kept_bytes(int dtype, size_t num, const int64_t *rows, const int64_t *cols,
+                           const toa_muon_series *series, int *status) {
+    return bytesOf(dtype, num, rows, cols, series, kForwardKeep, true, status);
 }
 
 int toa_muon_orthogonalize_multi(int dtype, size_t num, const int64_t *rows, const int64_t *cols,
