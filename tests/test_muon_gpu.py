@@ -566,7 +566,8 @@ def test_refusals():
     wide = torch.ones(3, 8, device='cuda')
     refused = [
         lambda: orthogonalize(v), lambda: orthogonalize(d), lambda: orthogonalize([x, v]),
-        lambda: orthogonalize(x.to(torch.int32)), lambda: orthogonalize(x, steps=0),
+        lambda: orthogonalize(x.to(torch.int32)), lambda: orthogonalize(torch._neg_view(x)),
+        lambda: orthogonalize(x, steps=2.5), lambda: orthogonalize(x, steps=0),
         lambda: orthogonalize(x, steps=33), lambda: orthogonalize(x, eps=-1.0),
         lambda: orthogonalize(x, eps=float('nan')),
         lambda: orthogonalize(x, coefficients=(50.0, 1.0, 1.0)),

@@ -261,6 +261,37 @@ def test_compiled():
     assert torch.equal(leaf.grad, other.grad)
 
 
+def test_registered_operators_pass_opcheck():
+    x, dy = randn(2, 20, 30, seed=1), randn(2, 20, 30, seed=2)
+    p, g, m = (randn(20, 30, seed=k) for k in (3, 4, 5))
+    q, s = torchopt_amd.quantize_blocks(m)
+    series, ops = (3, list(plain.COEFFICIENTS), 1e-7), torch.ops.torchopt_amd
+    torch.library.opcheck(ops.orthogonalize_multi.default, ([x, x[0]], *series))
+    torch.library.opcheck(ops.orthogonalize_multi.default, ([x.clone().requires_grad_()], *series))
+    torch.library.opcheck(ops.orthogonalize_backward_multi.default, ([dy], [x], *series))
+    torch.library.opcheck(ops.muon_forward_multi_.default, ([g.clone()], [q.clone()], [s.clone()], 0.9,
+                                                            True, *series, None))
+    torch.library.opcheck(ops.muon_fused_step_multi_.default, (
+        [p.clone()], [g], [m.clone()], [], 0.9, 0.1, True, 0.0, False, *series, 'none'))
+
+
+@pytest.mark.parametrize('kind', [None, torch.int8])
+def test_compiled_transform(kind):
+    t = scale_by_muon(momentum_dtype=kind)
+    gs = [randn(20, 30, seed=1), randn(40, 300, seed=2)]
+    state, other = t.init(gs), t.init(gs)
+
+    def step(gs, state):
+        return t.update(gs, state)
+
+    mine = torch.compile(step, fullgraph=True, backend='aot_eager')
+    for _ in range(2):
+        out, state = mine([g.clone() for g in gs], state)
+        want, other = t.update([g.clone() for g in gs], other)
+        assert all(map(torch.equal, out, want))
+        assert all(map(torch.equal, state.momentum, other.momentum))
+
+
 def test_a_run_of_them_together():
     """A small network: matrices by FusedMuon with 8-bit blocks, the rest by FusedAdam, in
     bfloat16, saved and restored half way; the restored run repeats the first bit for bit."""

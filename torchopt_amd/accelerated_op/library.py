@@ -205,8 +205,30 @@ def _muon_fused_step_multi_(params: List[Tensor], updates: List[Tensor], mu: Lis
 
 
 class dispatch:  # noqa: N801 - used as a namespace
-    """The functions of `torchopt_amd._C.adam_op`, routed through the registered operators while
-    `torch.compile` is tracing and called directly otherwise."""
+    """The functions of `torchopt_amd._C.adam_op` (and two of `muon_op`), routed through the
+    registered operators while `torch.compile` is tracing and called directly otherwise."""
+
+    @staticmethod
+    def muon_forward_multi_(updates, mu, scales, momentum, *, nesterov, steps, coefficients, eps,
+                            adjust_lr_fn):
+        if torch.compiler.is_compiling():
+            torch.ops.torchopt_amd.muon_forward_multi_(updates, mu, scales or [], momentum, nesterov,
+                                                       steps, list(coefficients), eps, adjust_lr_fn)
+        else:
+            muon_op.forward_multi_(updates, mu, scales, momentum, nesterov=nesterov, steps=steps,
+                                   coefficients=coefficients, eps=eps, adjust_lr_fn=adjust_lr_fn)
+
+    @staticmethod
+    def muon_fused_step_multi_(params, updates, mu, scales, momentum, lr, *, nesterov,
+                               weight_decay, maximize, steps, coefficients, eps, adjust_lr_fn):
+        if torch.compiler.is_compiling():
+            torch.ops.torchopt_amd.muon_fused_step_multi_(
+                params, updates, mu, scales or [], momentum, lr, nesterov, weight_decay, maximize,
+                steps, list(coefficients), eps, adjust_lr_fn)
+        else:
+            muon_op.fused_step_multi_(params, updates, mu, scales, momentum, lr, nesterov=nesterov,
+                                      weight_decay=weight_decay, maximize=maximize, steps=steps,
+                                      coefficients=coefficients, eps=eps, adjust_lr_fn=adjust_lr_fn)
 
     @staticmethod
     def forward_(updates, mu, nu, b1, b2, eps, eps_root, count):

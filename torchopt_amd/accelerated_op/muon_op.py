@@ -23,6 +23,7 @@ differentiable a second time.
 
 from __future__ import annotations
 
+import operator
 from typing import Any, Sequence
 
 import torch
@@ -121,7 +122,7 @@ def orthogonalize(
     for t in tensors:
         if not isinstance(t, torch.Tensor):
             raise TypeError(f'orthogonalize: expected tensors, got {type(t).__name__}')
-    series = (int(steps), tuple(float(c) for c in coefficients), float(eps))
+    series = (operator.index(steps), tuple(float(c) for c in coefficients), float(eps))
     out: list[torch.Tensor | None] = [None] * len(tensors)
     grad = torch.is_grad_enabled()
     for ks in _by_kind(tensors) if tensors else []:
@@ -137,7 +138,7 @@ def orthogonalize(
             out[k] = y
     if single:
         return out[0]
-    return out if isinstance(matrices, list) else type(matrices)(out)
+    return out if isinstance(matrices, list) else tuple(out)
 
 
 def quantize_blocks(tensors: torch.Tensor | Sequence[torch.Tensor]):

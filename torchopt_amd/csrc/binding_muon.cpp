@@ -29,6 +29,8 @@ toa_muon_series seriesOf(int steps, const Coefficients &c, double eps) {
 int gate(const char *name, const TensorList &l) {
     for (const Tensor &t : l) {
         if (!t.is_cuda()) throw std::runtime_error("Not implemented");
+        TORCH_CHECK(!t.is_neg(), name, ": expected tensors that are what their memory holds; use "
+                                       "resolve_neg() on views with the negative bit");
         TORCH_CHECK(t.device() == l[0].device(), name, ": expected all tensors on ", l[0].device(),
                     ", got one on ", t.device());
         TORCH_CHECK(t.scalar_type() == l[0].scalar_type(), name, ": expected scalar type ",

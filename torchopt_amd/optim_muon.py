@@ -26,7 +26,8 @@ from typing import Any, Callable, Iterable, Sequence
 
 import torch
 
-from torchopt_amd.accelerated_op.muon_op import (COEFFICIENTS, dequantize_blocks, muon_op,
+from torchopt_amd.accelerated_op.library import dispatch
+from torchopt_amd.accelerated_op.muon_op import (COEFFICIENTS, dequantize_blocks,
                                                  quantize_blocks)
 from torchopt_amd.transform.scale_by_muon import (ScaleByMuonState, check_muon, require_matrix,
                                                   zero_momentum)
@@ -171,7 +172,7 @@ class FusedMuon:
                 scales = None
                 if state.scales[ks[0]] is not None:
                     scales = [state.scales[k] for k in ks]
-                muon_op.fused_step_multi_(
+                dispatch.muon_fused_step_multi_(
                     [group[k] for k in ks], [group[k].grad for k in ks],
                     [state.momentum[k] for k in ks], scales, self.momentum, lr,
                     nesterov=self.nesterov, weight_decay=self.weight_decay,

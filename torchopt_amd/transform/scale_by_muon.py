@@ -23,7 +23,8 @@ from typing import Any, NamedTuple
 import torch
 
 from torchopt_amd import _tree
-from torchopt_amd.accelerated_op.muon_op import COEFFICIENTS, muon_op, orthogonalize
+from torchopt_amd.accelerated_op.library import dispatch
+from torchopt_amd.accelerated_op.muon_op import COEFFICIENTS, orthogonalize
 from torchopt_amd.base import GradientTransformation
 
 
@@ -148,9 +149,9 @@ def scale_by_muon(
                 scales = None
                 if s_leaves[ks[0]] is not None:
                     scales = [s_leaves[k] for k in ks]
-                muon_op.forward_multi_([new_g[k] for k in ks], [m_leaves[k] for k in ks], scales,
-                                       momentum, nesterov=nesterov, adjust_lr_fn=adjust_lr_fn,
-                                       **series)
+                dispatch.muon_forward_multi_(
+                    [new_g[k] for k in ks], [m_leaves[k] for k in ks], scales, momentum,
+                    nesterov=nesterov, adjust_lr_fn=adjust_lr_fn, **series)
         elif live:
             if any(m_leaves[k].dtype == torch.int8 for k in live):
                 raise ValueError('scale_by_muon: a momentum in 8-bit blocks is updated in place '
