@@ -145,10 +145,25 @@ struct FillArgs {
     MatRec r[kFill];
 };
 // Records travel in the launch's own arguments: no host buffer has to outlive the call, and a
-// captured graph holds them by value.
+// captured graph holds them by value.  Few of them come with the first pass over the matrices, which
+// leaves them in the workspace for the others, and that batch's factors are made by the pass that
+// makes its operands: two launches less, 5 us of 195 for one 1024^2 matrix.
+constexpr int kFew = 24;
 __global__ void fill_kernel(FillArgs a, MatRec *dst, int n) {
     const int i = threadIdx.x;
     if (i < n) dst[i] = a.r[i];
+}
+
+// A copy in scalar registers.
+__device__ inline MatRec uniform(const MatRec *p) {
+    MatRec r;
+    constexpr int kWords = sizeof(MatRec) / 4;
+    int words[kWords];
+    __builtin_memcpy(words, p, sizeof(MatRec));
+#pragma unroll
+    for (int i = 0; i < kWords; ++i) words[i] = __builtin_amdgcn_readfirstlane(words[i]);
+    __builtin_memcpy(&r, words, sizeof(MatRec));
+    return r;
 }
 
 // ---- the momentum and the norms --------------------------------------------------------------
@@ -176,6 +191,8 @@ struct SumArgs {
     double *parts;     // [matrix][kMaxParts]
     StepArgs step;
     int64_t per[kMaxGroups];  // elements per workgroup, a multiple of 2048
+    int few;                  // so many records are here, and `recs` is where they go
+    MatRec r[kFew];
 };
 
 template <typename T> __device__ inline void load8(const T *p, int valid, float (&v)[8]) {
@@ -354,7 +371,10 @@ __global__ __launch_bounds__(256) void sum_kernel(SumArgs a) {
     int part = blockIdx.x, mat;
     const int gi = findGroup(a.sh, part, mat);
     mat += a.sh.g[gi].mat0;
-    const MatRec &r = a.recs[mat];
+    if (a.few && blockIdx.x == 0)
+        for (int i = threadIdx.x; i < a.few * (int)(sizeof(MatRec) / 4); i += 256)
+            ((int *)const_cast<MatRec *>(a.recs))[i] = ((const int *)a.r)[i];
+    const MatRec r = uniform(a.few ? a.r + mat : a.recs + mat);
     const int64_t n = (int64_t)r.s * r.w, from = part * a.per[gi];
     const int64_t to = from + a.per[gi] < n ? from + a.per[gi] : n;
     const double sum = blockSum(sumPass<T, KIND>(r, a.step, from, to), lds);
@@ -487,45 +507,60 @@ __device__ inline void stepFactors(const Bounds &b, int t, Factor *f, Factor *ba
     back[2] = {ldexpf(1.f, ey - en - ex), 0.f, ldexpf(1.f, (en + ex) - (ep + ey1)), 0.f};
 }
 
-// One workgroup per matrix: norm, then a thread per step for the factors of its stages.
+// By a whole workgroup: a matrix's norms and, if it is the one to `write`, those and the factors of all
+// stages into the workspace, a thread for each step.
+__device__ inline MatNorm makeFactors(const FactorArgs &a, int mat, int np, bool write,
+                                      SeriesTable &table, double *lds) {
+    const int t = threadIdx.x;
+    table.load(a.q);
+    const double ysize =
+        a.parts_y ? sqrt(blockSum(t < np ? a.parts_y[(int64_t)mat * kMaxParts + t] : 0.0, lds)) : 0.0;
+    const double size = sqrt(blockSum(t < np ? a.parts[(int64_t)mat * kMaxParts + t] : 0.0, lds));
+    const Bounds b(a.q, table, size, ysize);
+    const MatNorm norm = normOf(b, size);
+    if (!write) return norm;
+    if (t == 0) a.norms[mat] = norm;
+    Factor *f = a.factors + (int64_t)mat * a.stages + kStepFactors * t;
+    if (t < a.q.steps) {
+        if (t >= a.q.paired)
+            stepFactors(b, t, f,
+                        a.parts_y ? a.factors + (int64_t)mat * a.stages + kStepFactors * a.q.steps + 3 * t
+                                  : nullptr);
+        else if (t % 2 == 0)
+            pairFactors(b, t, f);
+    }
+    return norm;
+}
+
+// One workgroup per matrix.
 __global__ __launch_bounds__(256) void factors_kernel(FactorArgs a) {
     __shared__ double lds[4];
     __shared__ SeriesTable table;
     const int mat = blockIdx.x, t = threadIdx.x;
-    table.load(a.q);
     int k = 0;
     while (k + 1 < a.ngroups && mat >= a.mat_end[k]) ++k;
     const int np = a.nparts[k];
-    const double ysize =
-        a.parts_y ? sqrt(blockSum(t < np ? a.parts_y[(int64_t)mat * kMaxParts + t] : 0.0, lds)) : 0.0;
-    Factor *f = a.factors + (int64_t)mat * a.stages + kStepFactors * t;
-    if (a.measured >= 0) {
-        // on the way back: bounds of the cotangents from this one on follow its norm
-        MatNorm n = a.norms[mat];
-        Bounds b(a.q, table, n.size, n.y_size);
-        b.ystep = n.y_step;
-        b.yexp_ = n.y_exp;
-        const double bound = b.y(a.measured);
-        b.yexp_ = b.yexp(a.measured);
-        b.ystep = a.measured;
-        const double now = ldexp(ysize, -b.yexp_);
-        b.ysize = now > 0.0 && now < bound ? now : bound;  // (nothing, or NaN: as before)
-        __syncthreads();  // (everybody has read the norms)
-        if (t == 0) a.norms[mat] = normOf(b, n.size);
-        if (t < a.measured)
-            stepFactors(b, t, f, a.factors + (int64_t)mat * a.stages + kStepFactors * a.q.steps + 3 * t);
+    if (a.measured < 0) {
+        makeFactors(a, mat, np, true, table, lds);
         return;
     }
-    const double size = sqrt(blockSum(t < np ? a.parts[(int64_t)mat * kMaxParts + t] : 0.0, lds));
-    const Bounds b(a.q, table, size, ysize);
-    if (t == 0) a.norms[mat] = normOf(b, size);
-    if (t >= a.q.steps) return;
-    if (t >= a.q.paired)
-        stepFactors(b, t, f,
-                    a.parts_y ? a.factors + (int64_t)mat * a.stages + kStepFactors * a.q.steps + 3 * t
-                              : nullptr);
-    else if (t % 2 == 0)
-        pairFactors(b, t, f);
+    // on the way back: bounds of the cotangents from this one on follow its norm
+    table.load(a.q);
+    const double stored = sqrt(blockSum(t < np ? a.parts_y[(int64_t)mat * kMaxParts + t] : 0.0, lds));
+    const MatNorm n = a.norms[mat];
+    Bounds b(a.q, table, n.size, n.y_size);
+    b.ystep = n.y_step;
+    b.yexp_ = n.y_exp;
+    const double bound = b.y(a.measured);
+    b.yexp_ = b.yexp(a.measured);
+    b.ystep = a.measured;
+    const double now = ldexp(stored, -b.yexp_);
+    b.ysize = now > 0.0 && now < bound ? now : bound;  // (nothing, or NaN: as before)
+    __syncthreads();  // (everybody has read the norms)
+    if (t == 0) a.norms[mat] = normOf(b, n.size);
+    if (t < a.measured)
+        stepFactors(b, t, a.factors + (int64_t)mat * a.stages + kStepFactors * t,
+                    a.factors + (int64_t)mat * a.stages + kStepFactors * a.q.steps + 3 * t);
 }
 
 // ---- operands ----------------------------------------------------------------------------------
@@ -572,6 +607,7 @@ struct PackArgs {
     int64_t off[kMaxGroups], off_t[kMaxGroups];  // of the operand and of its transpose
     StepArgs step;
     int split;
+    FactorArgs f;  // FEW: what is to be made of the sums on the way
 };
 
 // An element of G, of the step's U, or of the cotangent, `at` elements behind the first.
@@ -625,9 +661,11 @@ __device__ inline void elements8(const MatRec &r, const StepArgs &a, int64_t at,
 // elements that are neighbours in memory are eight columns of one of the two and go there at once;
 // the other is made through LDS.  HBM-bound: 4 bytes (bfloat16 and its momentum) in, 8 out, GPT-2-medium's
 // 302 million elements in 676 us = 5.4 TB/s.
-template <typename T, int KIND>
+template <typename T, int KIND, bool FEW>
 __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     __shared__ float tile[64][65];  // [operand row or column][the other]
+    __shared__ SeriesTable table;
+    __shared__ double lds[4];
     int t = blockIdx.x, mat;
     const int gi = findGroup(a.sh, t, mat);
     const Group &g = a.sh.g[gi];
@@ -636,7 +674,9 @@ __global__ __launch_bounds__(256) void pack_kernel(PackArgs a) {
     const MatRec &r = a.recs[mat];
     const int across = (int)(padded(g.w) / 64);
     const int i0 = t / across * 64, j0 = t % across * 64;
-    const double scale = KIND == kPackAux ? a.norms[mat].y_scale : a.norms[mat].x_scale;
+    const MatNorm norm =
+        FEW ? makeFactors(a.f, mat, a.f.nparts[gi], t == 0, table, lds) : a.norms[mat];
+    const double scale = KIND == kPackAux ? norm.y_scale : norm.x_scale;
     const int64_t rs = KIND == kPackAux ? r.aux_rs : r.g_rs, cs = KIND == kPackAux ? r.aux_cs : r.g_cs;
     // "lines" run along the smaller stride: rows of the operand, or (turned) its columns
     const bool by_rows = cs <= rs;
@@ -1378,18 +1418,6 @@ __device__ inline void gather(f32x16 (&share)[RB * (RB + 1) / 2], float *shares,
         if (r != k) writeElement<RB>(m, col, row, v);
     }
     __syncthreads();
-}
-
-// A copy in scalar registers.
-__device__ inline MatRec uniform(const MatRec *p) {
-    MatRec r;
-    constexpr int kWords = sizeof(MatRec) / 4;
-    int words[kWords];
-    __builtin_memcpy(words, p, sizeof(MatRec));
-#pragma unroll
-    for (int i = 0; i < kWords; ++i) words[i] = __builtin_amdgcn_readfirstlane(words[i]);
-    __builtin_memcpy(&r, words, sizeof(MatRec));
-    return r;
 }
 
 constexpr int smallColumnBlocks(int rb) { return rb == 1 ? 27 : 7; }

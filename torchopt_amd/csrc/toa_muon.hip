@@ -375,24 +375,24 @@ class Run {
   public:
     Run(const Call &c, const Batch &b, const Series &series)
         : c_(c), b_(b), steps_(c.series.steps), back_(c.what == kBackward),
-          keep_(c.kept != nullptr), stages_(stagesOf(steps_, back_)), head_(headOf((int64_t)b.mats.size(), stages_)),
+          keep_(c.kept != nullptr), few_(b.mats.size() <= kFew), stages_(stagesOf(steps_, back_)), head_(headOf((int64_t)b.mats.size(), stages_)),
           f_{series} {
         f_.q.paired = pairedSteps();
     }
 
     int go() {
-        TRY(fillRecords(c_, b_.mats, (MatRec *)(c_.ws + head_.recs)));
+        if (!few_) TRY(fillRecords(c_, b_.mats, (MatRec *)(c_.ws + head_.recs)));
         TRY(sums());
         TRY(factors());
         if (!back_ || !keep_) {
-            TRY(pack(false));
+            TRY(pack(false, few_));
             int from = 0;  // which of the two buffers holds X
             for (int k = 0; k < f_.q.paired; k += 2, from ^= 1) TRY(forwardPair(k, from));
             for (int k = f_.q.paired; k < steps_; ++k, from ^= 1)
                 TRY(forwardStep(k, back_ || keep_ ? k : from));
         }
         if (!back_) return 0;
-        TRY(pack(true));
+        TRY(pack(true, few_ && keep_));
         double growth = 1.0;
         for (int k = steps_ - 1; k >= 0; --k) {
             if (k && k + 1 < steps_ && growth * f_.q.d[k] > kMaxGrowth) {
@@ -445,6 +445,10 @@ class Run {
         a.recs = recs();
         a.parts = (double *)(c_.ws + head_.parts);
         a.step = stepOf(c_);
+        if (few_) {
+            a.few = (int)b_.mats.size();
+            for (int k = 0; k < a.few; ++k) a.r[k] = recordOf(c_, b_.mats[k]);
+        }
         const int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int k) {
             const int64_t n = (int64_t)s.s * s.w;
             // (at least eight elements a thread: more in a row, with few of them at work, cost a
@@ -479,12 +483,17 @@ class Run {
         f_.factors = (Factor *)(c_.ws + head_.factors);
         f_.stages = stages_;
         f_.measured = -1;
-        return launch(factors_kernel, (int64_t)b_.mats.size(), 256, c_.stream, f_);
+        return few_ ? 0 : launch(factors_kernel, (int64_t)b_.mats.size(), 256, c_.stream, f_);
     }
 
     // The cotangent, or the matrix itself, as operands.
-    int pack(bool cotangent) {
+    int pack(bool cotangent, bool with_factors) {
+        return with_factors ? pack<true>(cotangent) : pack<false>(cotangent);
+    }
+
+    template <bool FEW> int pack(bool cotangent) {
         PackArgs a{};
+        a.f = f_;
         a.recs = recs();
         a.norms = (const MatNorm *)(c_.ws + head_.norms);
         a.ws = c_.ws;
@@ -498,11 +507,11 @@ class Run {
         });
         return withType(c_.dtype, [&](auto t) {
             using T = decltype(t);
-            return launch(cotangent                          ? pack_kernel<T, kPackAux>
-                          : c_.what != kStep               ? pack_kernel<T, kPackG>
-                          : c_.momentum_dtype == TOA_I8    ? pack_kernel<T, kPackMI8>
-                          : c_.momentum_dtype == c_.dtype ? pack_kernel<T, kPackM>
-                                                           : pack_kernel<T, kPackMF32>,
+            return launch(cotangent                          ? pack_kernel<T, kPackAux, FEW>
+                          : c_.what != kStep               ? pack_kernel<T, kPackG, FEW>
+                          : c_.momentum_dtype == TOA_I8    ? pack_kernel<T, kPackMI8, FEW>
+                          : c_.momentum_dtype == c_.dtype ? pack_kernel<T, kPackM, FEW>
+                                                           : pack_kernel<T, kPackMF32, FEW>,
                           grid, 256, c_.stream, a);
         });
     }
@@ -785,7 +794,7 @@ class Run {
     const Call &c_;
     const Batch &b_;
     const int steps_;
-    const bool back_, keep_;
+    const bool back_, keep_, few_;
     const int stages_;
     const Head head_;
     FactorArgs f_;
