@@ -298,6 +298,50 @@ def test_kept_iterates_give_the_same_gradient(dtype):
         muon_op.orthogonalize_backward_multi(dys[:1], xs[:1], **kw, kept=kept)
 
 
+@pytest.mark.parametrize('each', [1, 2])
+def test_gradients_of_many_shapes(each):
+    """More shapes than one launch takes, in few matrices and in more than come with a launch's
+    arguments; kept and made again."""
+    shapes = [(40 + 9 * k, 230 + 13 * k) for k in range(20)]
+    xs = [randn(each, *s, seed=k).cuda() for k, s in enumerate(shapes)]
+    dys = [randn(each, *s, seed=k + 50).cuda() for k, s in enumerate(shapes)]
+    _, kept = muon_op.orthogonalize_keep_multi(xs, 1 << 30)
+    got = muon_op.orthogonalize_backward_multi(dys, xs, kept=kept)
+    assert all(map(torch.equal, got, muon_op.orthogonalize_backward_multi(dys, xs)))
+    for k in (0, 7, 15, 16, 19):
+        exact, allowed = plain.tolerance(plain.gradient, xs[k][-1].double().cpu(),
+                                         dys[k][-1].double().cpu(), dtype=F32)
+        plain.assert_close(got[k][-1], exact, allowed, str(shapes[k]), spread=True)
+
+
+@pytest.mark.parametrize('m,n', [(20, 40), (90, 300)])
+@pytest.mark.parametrize('of_x,of_dy', [(1e-10, 1e-20), (1e20, 1e25), (1e-20, 1e-25), (1.0, 1e30),
+                                        (1.0, 1e-30)])
+def test_gradient_magnitudes(m, n, of_x, of_dy):
+    check_gradient(randn(m, n, seed=1, scale=of_x), randn(m, n, seed=2, scale=of_dy), F32, eps=0.0)
+
+
+def test_a_matrix_beyond_32_bits():
+    """1100 x 2^20 in float16: its operand has 4.8 GB.  (Reference on the GPU in 64 bits; both
+    steps of two are half-step roundings of float16 apart.)"""
+    m, n = 1100, 1 << 20
+    gen = torch.Generator(device='cuda').manual_seed(1)
+    x = torch.randn(m, n, generator=gen, device='cuda', dtype=torch.float16)
+    y = orthogonalize(x, steps=2)
+    w = x.double()
+    w /= w.square().sum().sqrt() + 1e-7
+    a, b, c = plain.COEFFICIENTS
+    for _ in range(2):
+        s = w @ w.t()
+        w = (b * s + c * (s @ s) + a * torch.eye(m, device='cuda', dtype=torch.float64)) @ w
+    # rows of the operands at both ends and in the middle, whole columns too
+    half = torch.finfo(torch.float16)
+    for at in (slice(0, 40), slice(540, 560), slice(1060, 1100)):
+        diff = (y[at].double() - w[at]).abs() - half.eps / 2 * w[at].abs() - half.smallest_normal * half.eps / 2
+        # 22-bit operands: two steps of few 2^-22 each
+        assert float(diff.max()) <= 2.0 ** -18 * float(w[at].abs().max())
+
+
 def test_gradient_with_and_without_keeping(monkeypatch):
     from torchopt_amd.accelerated_op import muon_op as module
     x, dy = randn(3, 200, 700, seed=1).cuda(), randn(3, 200, 700, seed=2).cuda()
