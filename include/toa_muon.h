@@ -86,8 +86,8 @@ TOA_API size_t toa_muon_backward_workspace(int dtype, size_t num, const int64_t 
 
 /* What the gradient needs of the forward pass -- every iterate and its products -- can be kept
  * between the two: bytes of that buffer (256-byte aligned) for a list, about 8 bytes for each
- * element of a matrix and of the square of its shorter side, for each step; small matrices, whose
- * iterates are made again faster than they are read, need none in a short series. */
+ * element of a matrix and of the square of its shorter side, for each step; lists of small
+ * matrices, whose iterates are made again faster than they are read, need none in a short series. */
 TOA_API size_t toa_muon_kept_bytes(int dtype, size_t num, const int64_t *rows, const int64_t *cols,
                                    const toa_muon_series *series, int *status);
 

@@ -213,6 +213,23 @@ def test_larger_batches(count, m, n):
             plain.assert_close(y[k], exact, allowed, f'{dtype} {k}', spread=True)
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+def test_small_ones_beside_larger_ones(dtype):
+    """Few go through the larger ones' launches, many through their own."""
+    for few in (3, 60):
+        sizes = [(20, 30), (7, 129), (64, 100)] * (few // 3) + [(90, 400), (130, 65)]
+        xs = [randn(*s, dtype=dtype, seed=k) for k, s in enumerate(sizes)]
+        dys = [randn(*s, dtype=dtype, seed=k + 200) for k, s in enumerate(sizes)]
+        leaves = [x.cuda().requires_grad_() for x in xs]
+        ys = orthogonalize(leaves)
+        grads = torch.autograd.grad(ys, leaves, [d.cuda() for d in dys])
+        for k in sorted({0, 1, 2, len(xs) - 3, len(xs) - 2, len(xs) - 1}):
+            exact, allowed = plain.tolerance(plain.orthogonalize, xs[k].double(), dtype=dtype)
+            plain.assert_close(ys[k], exact, allowed, f'{few} {sizes[k]}')
+            exact, allowed = plain.tolerance(plain.gradient, xs[k].double(), dys[k].double(), dtype=dtype)
+            plain.assert_close(grads[k], exact, allowed, f'gradient {few} {sizes[k]}')
+
+
 def test_the_same_call_gives_the_same_bits():
     x, dy = randn(4, 200, 700, seed=1).cuda(), randn(4, 200, 700, seed=2).cuda()
     s, ds = randn(9, 32, 288, seed=3).cuda(), randn(9, 32, 288, seed=4).cuda()

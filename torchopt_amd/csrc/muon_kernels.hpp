@@ -194,6 +194,7 @@ struct SumArgs {
     int few;                  // so many records are here, and `recs` is where they go
     MatRec r[kFew];
 };
+static_assert(sizeof(SumArgs) <= 4096, "a launch's arguments");
 
 template <typename T> __device__ inline void load8(const T *p, int valid, float (&v)[8]) {
     if (valid >= 8 && ((uintptr_t)p & 15) == 0) {
@@ -609,6 +610,7 @@ struct PackArgs {
     int split;
     FactorArgs f;  // FEW: what is to be made of the sums on the way
 };
+static_assert(sizeof(PackArgs) <= 4096, "a launch's arguments");
 
 // An element of G, of the step's U, or of the cotangent, `at` elements behind the first.
 template <typename T, int KIND>
@@ -744,6 +746,7 @@ struct GemmArgs {
     Shapes sh;
     Product p[kMaxGroups];
 };
+static_assert(sizeof(GemmArgs) <= 4096, "a launch's arguments");
 
 __device__ inline f32x16 mfma(half8 a, half8 b, f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);

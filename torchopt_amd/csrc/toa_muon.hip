@@ -127,6 +127,9 @@ struct SmallBatch {
 // (the default coefficients: 392 at their five steps, so never there).
 constexpr double kMaxGrowth = 512.0;
 
+// Tiles of 64 x 64 that small matrices may add to the launches of larger ones (which hold 512 at once).
+constexpr int64_t kFewTiles = 128;
+
 // Rows / 32 of the variant that takes an s x w matrix, or 0.
 int smallVariant(int64_t s, int64_t w) {
     for (int rb = 1; rb <= 2; ++rb)
@@ -145,18 +148,39 @@ int plan(size_t num, const int64_t *rows, const int64_t *cols, const Series &ser
     for (int k = 1; k < steps; ++k) growth *= series.d[k];
     const bool small = purpose == kForward || growth <= kMaxGrowth;
     bytes = kept_bytes = 0;
-    std::vector<size_t> order;
+    auto key = [&](size_t i) {
+        return std::make_pair(std::min(rows[i], cols[i]), std::max(rows[i], cols[i]));
+    };
+    std::vector<size_t> order, few;  // through the tiles; small ones
     order.reserve(num);
+    int64_t few_tiles = 0;
     for (size_t i = 0; i < num; ++i) {
         if (rows[i] < 0 || cols[i] < 0 || rows[i] > kMaxDim || cols[i] > kMaxDim) return TOA_ESIZE;
         if (!rows[i] || !cols[i]) continue;
-        const int64_t s = std::min(rows[i], cols[i]), w = std::max(rows[i], cols[i]);
-        const int rb = small ? smallVariant(s, w) : 0;
-        if (!rb) {
+        const auto shape = key(i);
+        if (small && smallVariant(shape.first, shape.second)) {
+            few.push_back(i);
+            few_tiles += (shape.first + 63) / 64 * ((shape.second + 63) / 64);
+        } else {
             order.push_back(i);
-            continue;
         }
-        const int64_t kept = backward ? align256(steps * smallKept(rb, (int)w)) : 0;
+    }
+    // A few small ones beside larger ones go with them: their tiles find room in launches that are made
+    // anyway, which costs next to nothing, and a launch of their own 20 to 50 us.
+    if (!order.empty() && few_tiles <= kFewTiles) {
+        std::vector<std::pair<int64_t, int64_t>> shapes;
+        for (const auto *list : {&order, &few})
+            for (size_t i : *list) shapes.push_back(key(i));
+        std::sort(shapes.begin(), shapes.end());
+        if (std::unique(shapes.begin(), shapes.end()) - shapes.begin() <= kMaxGroups) {
+            order.insert(order.end(), few.begin(), few.end());
+            few.clear();
+        }
+    }
+    for (size_t i : few) {
+        const auto shape = key(i);
+        const int rb = smallVariant(shape.first, shape.second);
+        const int64_t kept = backward ? align256(steps * smallKept(rb, (int)shape.second)) : 0;
         auto it = std::find_if(smalls.rbegin(), smalls.rend(),
                                [&](const SmallBatch &b) { return b.rb == rb; });
         SmallBatch *b = it == smalls.rend() ? nullptr : &*it;
@@ -168,9 +192,6 @@ int plan(size_t num, const int64_t *rows, const int64_t *cols, const Series &ser
         b->stride = std::max(b->stride, kept);
     }
     for (const SmallBatch &b : smalls) bytes = std::max(bytes, b.bytes());
-    auto key = [&](size_t i) {
-        return std::make_pair(std::min(rows[i], cols[i]), std::max(rows[i], cols[i]));
-    };
     // (long rows first: their tiles take longest and should not be what a launch ends with)
     std::stable_sort(order.begin(), order.end(), [&](size_t i, size_t j) {
         return std::make_pair(key(i).second, key(i).first) > std::make_pair(key(j).second, key(j).first);
