@@ -2,14 +2,15 @@
 orthogonalisation, weight decay and the addition to the parameters -- on the operators of
 `torchopt_amd._C.muon_op`, one call per device and dtype for any number of parameters.
 
-The reference has no counterpart.  Constructor arguments are those of ``torch.optim.Muon``, and so
-is the step:
+The reference has no counterpart.  Constructor arguments are those of ``torch.optim.Muon``.  The step:
 
     ``M <- momentum * M + g``,   ``U = g + momentum * M`` (``nesterov``; else ``U = M``),
     ``P <- (1 - lr * weight_decay) * P - lr * r * orthogonalize(U)``
 
-with ``r`` after `adjust_lr_fn` (see `scale_by_muon`).  Differences:
+with ``r`` after `adjust_lr_fn` (see `scale_by_muon`).  Beside ``torch.optim.Muon``:
 
+  * the momentum is the plain sum, not the mean of the gradients, which is ``1 - momentum`` times it;
+    the normalisation takes the factor out again (but for `eps`);
   * parameters of more than two dimensions are taken too, as the matrix of their first dimension
     times all the others (a convolution's kernel); vectors and scalars are refused;
   * `momentum_dtype=torch.int8` keeps the momentum in 8-bit blocks: a quarter of float32's
