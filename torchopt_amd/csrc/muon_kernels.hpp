@@ -11,8 +11,8 @@
 // tile of up to two products with a common sum, plus a multiple of the unit matrix, stored in both
 // orientations (X and X^T; for the symmetric ones the mirror image).  No stage reads a third
 // matrix; measured, the read of one at a tile's end cost as much as 15 % of its products.
-// (Where c is zero or tiny beside b: S = X X^T, P = c S S + b S + a I, N = c (M S + S M) + b M, with
-// that third matrix.)
+// (Where c is zero, or c h^2 large beside a: S = X X^T, P = c S S + b S + a I,
+// N = c (M S + S M) + b M, with that third matrix.)
 //
 // Two steps at once, where X is wide: the S of the next step is P S P, so X itself is needed once:
 //     S = X X^T,  P = c S S + b S + a I,  T = P S,  S' = T P + h I,  P' = c S' S' + (a - b h / 2) I,
@@ -26,7 +26,7 @@
 // dropped, lo lo, is 2^-22 of it).  Halves have few exponents, so every matrix is stored times a
 // power of two that takes its bound to 2^13..2^14: |X_k| <= max of the polynomial on the previous
 // interval (from the start's norm, 1 or less), and products of such bounds for the others.  An
-// element is at most the spectral norm, so nothing overflows, and what lies 2^-24 below the bound
+// element is at most the spectral norm, so nothing overflows, and what lies 2^-15 below the bound
 // still has all its bits.  ("half" operands keep hi alone: 11 bits.)
 //
 // Layout.  An operand lies the way the matrix instructions read it: by blocks of 32 rows, and in
