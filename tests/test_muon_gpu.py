@@ -48,8 +48,21 @@ def test_orthogonalize_sizes(m, n, dtype):
     check_forward(randn(m, n, dtype=dtype, seed=m * n), dtype, f'{m} x {n}')
 
 
+@pytest.mark.parametrize('dtype', TYPES)
+@pytest.mark.parametrize('m,n', [(1, 5000), (7, 3000), (32, 900), (33, 700), (63, 300), (64, 1111), (2000, 40)])
+def test_thin_matrices(m, n, dtype):
+    """Too wide for one workgroup, up to 64 rows: what lies between X's own products is one launch."""
+    x = randn(3, m, n, dtype=dtype, seed=m + n)
+    for kw in (dict(), dict(steps=4), dict(steps=3, coefficients=(1.5, -0.5, 0.0)),
+               dict(steps=2, coefficients=(0.5, 1.0, 0.01))):
+        y = orthogonalize(x.cuda(), **kw)
+        for k in range(3):
+            exact, allowed = plain.tolerance(plain.orthogonalize, x[k].double(), dtype=dtype, **kw)
+            plain.assert_close(y[k], exact, allowed, str(kw), spread=m > 1)
+
+
 @pytest.mark.parametrize('steps', [1, 2, 3, 4, 6, 9])
-@pytest.mark.parametrize('m,n', [(20, 50), (90, 400), (130, 140)])
+@pytest.mark.parametrize('m,n', [(20, 50), (90, 400), (130, 140), (50, 700)])
 def test_numbers_of_steps(m, n, steps):
     """(90 x 400 takes its steps in pairs and an odd one last.)"""
     for dtype in (F32, BF16):

@@ -1256,6 +1256,100 @@ __global__ __launch_bounds__(WM *WN *KS * 64, KS > 1 ? 2 : 1) void gemm_kernel(G
     }
 }
 
+// ---- thin matrices -----------------------------------------------------------------------------
+//
+// Two steps at once are five products of s x s matrices between one of X with itself and one with X.
+// With up to 64 rows each of the five is a single tile, so one workgroup makes all of them for a
+// matrix, from S to Q, in LDS: four waves, a 32 x 32 block each.  Bound by the way through five
+// products in a row: 14 us where five launches take 29 (one 32 x 2048 float32 matrix: 114 -> 83 us, 24
+// of 60 x 1500: 140 -> 107).
+
+constexpr int kThin = 64;
+
+struct SquareArgs {
+    char *ws;
+    const Factor *factors;
+    int stages, stage;
+    Shapes sh;
+    int64_t off[kMaxGroups];  // of S, and then of Q
+};
+
+__global__ __launch_bounds__(256) void square_kernel(SquareArgs a) {
+    constexpr int kBlock32 = kRows * kThin * 4;  // bytes of 32 rows: two pieces
+    __shared__ __attribute__((aligned(16))) char lds[3][2 * kBlock32];
+    int part = blockIdx.x, mat;
+    const int gi = findGroup(a.sh, part, mat);
+    const Group &g = a.sh.g[gi];
+    char *const global_s = Region(a.ws, a.ws, g, mat) + a.off[gi];
+    mat += g.mat0;
+    const int s = g.s;
+    const Factor *const f = a.factors + (int64_t)mat * a.stages + a.stage;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int p = wave >> 1, q = wave & 1;
+    // (16 bytes are a chunk of one row; rows beyond the matrix hold anything)
+    for (int i = threadIdx.x; i < 2 * kBlock32 / 16; i += 256) {
+        const int row = i / (kBlock32 / 16) * kRows + i % kRows;
+        half8 v = {};
+        if (row < s) v = *global<half8>(global_s + i * 16);
+        *(half8 *)(lds[0] + i * 16) = v;
+    }
+    __syncthreads();
+    // D = f.acc A B^T + f.add E + f.diag I, all of them symmetric: the result is written as its transpose
+    const int mine = q * kBlock32 + p * (kRows * kPiece) + (lane & 31) * 16 + (lane >> 5) * 8;
+    auto product = [&](const char *A, const char *B, const char *E, char *D, const Factor f) {
+        f32x16 sum;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) sum[i] = 0.f;
+#pragma unroll
+        for (int piece = 0; piece < 2; ++piece) {
+            half8 x[4], y[4];  // two of hi, two of lo
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+                const int at = piece * kRows * kPiece + c * 1024 + lane * 16;
+                x[c] = *(const half8 *)(A + p * kBlock32 + at);
+                y[c] = *(const half8 *)(B + q * kBlock32 + at);
+            }
+            beforeMatrix();
+#pragma unroll
+            for (int c = 0; c < 2; ++c) {
+                sum = mfma(x[2 + c], y[c], sum);
+                sum = mfma(x[c], y[2 + c], sum);
+                sum = mfma(x[c], y[c], sum);
+            }
+            afterMatrix();
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            half4 hi, lo, eh = {}, el = {};
+            if (f.add != 0.f) {
+                eh = *(const half4 *)(E + mine + u * 512);
+                el = *(const half4 *)(E + mine + u * 512 + 2048);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int row = p * 32 + u * 8 + (lane >> 5) * 4 + i, col = q * 32 + (lane & 31);
+                float v = sum[4 * u + i] * f.acc;
+                if (f.add != 0.f) v += f.add * ((float)eh[i] + (float)el[i]);
+                if (row == col) v += f.diag;
+                if (row >= s || col >= s) v = 0.f;
+                hi[i] = (_Float16)v;
+                lo[i] = (_Float16)(v - (float)hi[i]);
+            }
+            *(half4 *)(D + mine + u * 512) = hi;
+            *(half4 *)(D + mine + u * 512 + 2048) = lo;
+        }
+        __syncthreads();
+    };
+    char *const S = lds[0], *const P = lds[1], *const T = lds[2];
+    product(S, S, S, P, f[1]);
+    product(P, S, S, T, f[2]);
+    product(T, P, S, S, f[3]);
+    product(S, S, S, T, f[4]);
+    product(T, P, S, S, f[5]);
+    for (int i = threadIdx.x; i < (s + kRows - 1) / kRows * (kBlock32 / 16); i += 256)
+        *global<half8>(global_s + i * 16) = *(const half8 *)(S + i * 16);
+}
+
 // ---- small matrices ----------------------------------------------------------------------------
 //
 // Up to 32 rows and 864 columns, or 64 and 224: one workgroup takes a matrix through everything, and

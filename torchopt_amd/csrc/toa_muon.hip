@@ -711,6 +711,10 @@ class Run {
     int forwardPair(int k, int from) {
         const int stage = kStepFactors * k;
         TRY(gram(stage, k, from));
+        if (thin()) {
+            TRY(squares(stage, k));
+            return advance(stage + 6, k, k + 2, from, from ^ 1, [&](const Layout &l) { return l.s[k]; });
+        }
         TRY(symmetric(stage + 1, k, [&](Product &p, const Layout &l) {
             p.a0 = p.b0 = p.e = l.s[k];
             p.d = l.p[k];
@@ -736,6 +740,25 @@ class Run {
             p.d = l.s[k];
         }));
         return advance(stage + 6, k, k + 2, from, from ^ 1, [&](const Layout &l) { return l.s[k]; });
+    }
+
+    // Everything between the products with X of two steps at once, in one launch.
+    bool thin() const {
+        return std::all_of(b_.shapes.begin(), b_.shapes.end(),
+                           [](const Batch::Shape &s) { return s.s <= kThin; });
+    }
+
+    int squares(int stage, int k) {
+        SquareArgs a{};
+        a.ws = c_.ws;
+        a.factors = (const Factor *)(c_.ws + head_.factors);
+        a.stages = stages_;
+        a.stage = stage;
+        const int64_t grid = shapes(a.sh, [&](const Batch::Shape &s, int g) {
+            a.off[g] = s.lay.s[k];
+            return (int64_t)1;
+        });
+        return launch(square_kernel, grid, 256, c_.stream, a);
     }
 
     int backwardStep(int k) {
