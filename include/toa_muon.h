@@ -27,8 +27,8 @@
  *             except the momentum, whose type is given apart.
  *   precision products run on the matrix cores with float32 sums.  Their operands carry 22
  *             significant bits (two halves).  In a bfloat16 call that keeps no iterates, those of
- *             the last two orthogonalisation steps may carry 11, whose rounding the steps that
- *             follow hardly amplify.
+ *             the last orthogonalisation step may carry 11, where the coefficients keep what that
+ *             adds within half a step of bfloat16 (the default ones do not).
  *   workspace device memory the call may overwrite, 256-byte aligned, as many bytes as the
  *             matching *_workspace function says; calls that may overlap in time (other streams,
  *             other captured graphs) need workspaces of their own.

@@ -1,0 +1,101 @@
+"""16-bit results of the orthogonalisation are the 64-bit form's, rounded once to their type.
+
+For a result `z + e` that is rounded to the type, with `z` exact: each element ends no farther from
+`z` than `|round(z) - z| + 2 |e|` (either both round to the same value, or `z` lies within `|e|` of a
+border, and then `|round(z) - z|` is half a step less `|e|` at least).  So the whole deviation is at most
+that of the rounded exact result and twice the norm of `e`, for which `plain.tolerance` gives what
+operands of 22 bits and float32 sums may commit."""
+
+from __future__ import annotations
+
+import pytest
+import torch
+
+import muon_plain as plain
+from torchopt_amd import orthogonalize
+from torchopt_amd._C import muon_op
+
+pytestmark = pytest.mark.gpu
+
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+# one workgroup; thin; tiles with steps one by one and by twos
+SIZES = [(24, 60), (60, 200), (40, 1000), (128, 128), (200, 256), (260, 100), (100, 900), (512, 512)]
+
+
+def randn(*shape, seed=0):
+    return torch.randn(*shape, generator=torch.Generator().manual_seed(seed))
+
+
+def low_rank(m, n, rank):
+    return randn(m, rank, seed=rank) @ randn(rank, n, seed=rank + 1)
+
+
+def special(m, n):
+    spread = torch.ones(m, n)
+    spread[0, 0] = 1e4
+    k = min(m, n)
+    u, v = torch.linalg.qr(randn(m, k, seed=1))[0], torch.linalg.qr(randn(n, k, seed=2))[0]
+    yield from ((f'rank {r}', low_rank(m, n, r)) for r in (1, 2, 3, 8))
+    yield from [('identity', torch.eye(m, n)), ('ones', torch.ones(m, n)), ('one element', spread),
+                ('decaying', u @ torch.diag(torch.arange(1.0, k + 1) ** -1.5) @ v.t()),
+                ('full rank', randn(m, n, seed=3))]
+
+
+def rounded_once(y, exact, allowed, what):
+    rounding = float((exact.to(y.dtype).double() - exact).norm())
+    off = float((y.double().cpu() - exact).norm())
+    assert off <= rounding + 2.0 * allowed, \
+        f'{what}: off by {off:.4g}; rounding alone {rounding:.4g}, arithmetic {allowed:.3g}'
+
+
+@pytest.mark.parametrize('dtype', [F16, BF16])
+@pytest.mark.parametrize('m,n', SIZES)
+def test_special_matrices_are_rounded_once(m, n, dtype):
+    """The default coefficients, whose last steps magnify what is rounded before them: few large
+    singular values among many small ones show it most."""
+    for what, x in special(m, n):
+        x = x.to(dtype)
+        for steps in (5, 2, 1):
+            exact, allowed = plain.tolerance(plain.orthogonalize, x.double(), dtype=F32, steps=steps)
+            rounded_once(orthogonalize(x.cuda(), steps=steps), exact, allowed, f'{what}, {steps} steps')
+
+
+@pytest.mark.parametrize('coefficients,steps', [((5.0, -10.0, 6.0), 2), ((3.0, -3.0, -0.1), 3),
+                                                ((0.5, 1.0, 0.01), 3)])
+def test_other_coefficients_are_rounded_once(coefficients, steps):
+    kw = dict(steps=steps, coefficients=coefficients)
+    for m, n in ((128, 128), (100, 900)):
+        for rank in (1, 3, 8):
+            x = low_rank(m, n, rank).to(BF16)
+            exact, allowed = plain.tolerance(plain.orthogonalize, x.double(), dtype=F32, **kw)
+            rounded_once(orthogonalize(x.cuda(), **kw), exact, allowed, f'{m} x {n}, rank {rank}')
+
+
+@pytest.mark.parametrize('coefficients,steps', [((1.875, -1.25, 0.375), 5), ((1.875, -1.25, 0.375), 1),
+                                                ((1.5, -0.5, 0.0), 6), ((2.0, -1.5, 0.5), 4),
+                                                ((-1.5, 0.5, 0.0), 3)])
+def test_gentle_coefficients_stay_near_one_rounding(coefficients, steps):
+    """Series that converge may read the last step's operands in 11 bits, an eighth of bfloat16's
+    rounding, where that stays below half a step.  Here they magnify it at most four times -- at singular
+    value t by (|p'| + dP/dS |S + h I| + max |P|) / |P|, which is 3.1 at most for the quintics and 2.3 for
+    the cubics -- which is half a rounding beside the result's own, independent of it, so sqrt(1.25) = 1.12
+    times the result's alone.  A tenth more for few elements."""
+    kw = dict(steps=steps, coefficients=coefficients)
+    for m, n in ((128, 128), (100, 260), (512, 300), (3, 2000)):
+        for rank in (1, 2, 3, 8, None):
+            x = (low_rank(m, n, rank) if rank else randn(m, n, seed=5)).to(BF16)
+            exact = plain.orthogonalize(x.double(), **kw)
+            rounding = float((exact.to(BF16).double() - exact).norm())
+            off = float((orthogonalize(x.cuda(), **kw).double().cpu() - exact).norm())
+            assert off <= 1.23 * rounding, f'{m} x {n}, rank {rank}: {off / rounding:.3f}'
+
+
+def test_step_of_low_rank_gradients_is_rounded_once():
+    for m, n in ((128, 128), (260, 100), (512, 512)):
+        gs = [low_rank(m, n, rank).to(BF16) for rank in (1, 3)]
+        mine, kept = [g.cuda() for g in gs], [torch.zeros(m, n, dtype=BF16, device='cuda') for _ in gs]
+        muon_op.forward_multi_(mine, kept, None, 0.0, nesterov=False, adjust_lr_fn='none')
+        for g, y in zip(gs, mine):
+            exact, allowed = plain.tolerance(plain.orthogonalize, g.double(), dtype=F32)
+            rounded_once(y, exact, allowed, f'{m} x {n}')

@@ -115,7 +115,8 @@ def orthogonalize(
     Returns:
         A tensor like `matrices` (a list or tuple of them for a list or tuple), differentiable
         with respect to it.  Results come from products with 22-bit operands and float32 sums;
-        for bfloat16 the operands of the last two steps may carry 11 bits.
+        for bfloat16 the operands of the last step may carry 11 bits, where the coefficients keep
+        what that adds within half a step of the type (the default ones do not).
     """
     single = isinstance(matrices, torch.Tensor)
     tensors = [matrices] if single else list(matrices)

@@ -27,7 +27,8 @@
 // power of two that takes its bound to 2^13..2^14: |X_k| <= max of the polynomial on the previous
 // interval (from the start's norm, 1 or less), and products of such bounds for the others.  An
 // element is at most the spectral norm, so nothing overflows, and what lies 2^-15 below the bound
-// still has all its bits.  ("half" operands keep hi alone: 11 bits.)
+// still has all its bits.  ("half" operands keep hi alone: 11 bits, in the last step of bfloat16 calls
+// whose series magnifies their rounding little.)
 //
 // Layout.  An operand lies the way the matrix instructions read it: by blocks of 32 rows, and in
 // them by pieces of 4 KiB, [32 hi | 32 lo] of 32 columns or 64 halves of 64 columns of each row.  A
@@ -392,6 +393,7 @@ struct Factor {
 struct Series {
     int steps, square;              // square: S carries h
     int paired;                     // so many steps are taken by twos
+    int halves;                     // bfloat16: the last step's operands may carry 11 bits
     float a, b, c;
     double eps, h;
     double x[kMaxSteps + 1];        // bound of |X_k| from a start of norm 1

@@ -248,6 +248,20 @@ double largest(double k0, double k1, double k2, int n0, double top) {
     return best;
 }
 
+// The smallest |a + b q + c q^2| on [0, top].
+double smallest(double a, double b, double c, double top) {
+    auto at = [&](double q) { return a + q * (b + q * c); };
+    double lo = std::min(at(0.0), at(top)), hi = std::max(at(0.0), at(top));
+    if (c != 0.0) {
+        const double q = -b / (2.0 * c);
+        if (q > 0.0 && q < top) {
+            lo = std::min(lo, at(q));
+            hi = std::max(hi, at(q));
+        }
+    }
+    return lo > 0.0 ? lo : hi < 0.0 ? -hi : 0.0;
+}
+
 int checkSeries(const toa_muon_series *q) {
     if (!q) return TOA_ENULL;
     if (q->steps < 1 || q->steps > kMaxSteps || !std::isfinite(q->a) || !std::isfinite(q->b) ||
@@ -278,6 +292,18 @@ int boundsOf(const toa_muon_series &q, Series &f) {
     // at most
     f.h = q.c != 0.0 ? q.b / (2.0 * q.c) : 0.0;
     f.square = q.c != 0.0 && std::fabs(q.c) * f.h * f.h <= 2.0 * std::fabs(q.a);
+    // Operands of 11 bits in the last step, each element off by 2^-12 of itself: that of X moves the
+    // result by the slope, that of S (or S + h I, as it is kept) by what P changes with it, that of P by P
+    // itself, all beside a result of |P X| >= (least |P|) |X|.  Up to 8 times 2^-12 is half a step of
+    // bfloat16.  (The default coefficients reach 21, as c h^2 cancels most of a: with two such steps few
+    // large singular values came out up to 2.6 roundings off.  Those that converge, (1.875, -1.25, 0.375)
+    // or (2, -1.5, 0.5), take 6: five steps of 4 matrices of 4096 x 1024 in 765 us, at 22 bits throughout
+    // 880; of 24 of 1024^2 in 1.68 ms, 1.88.)
+    const double top = f.x[q.steps - 1] * f.x[q.steps - 1];
+    const double kept = f.square ? std::max(std::fabs(f.h), std::fabs(f.h + top)) : top;
+    const double of_s = f.square ? 2.0 * std::fabs(q.c) * kept
+                                 : std::max(std::fabs(q.b), std::fabs(q.b + 2.0 * q.c * top));
+    f.halves = f.d[q.steps - 1] + of_s * kept + f.r[q.steps - 1] <= 8.0 * smallest(q.a, q.b, q.c, top);
     return 0;
 }
 
@@ -427,9 +453,9 @@ class Run {
     }
 
   private:
-    // whether step k's operands carry 22 bits (see the header)
+    // whether step k's operands carry 22 bits (see boundsOf)
     bool split(int k) const {
-        return back_ || keep_ || c_.dtype != TOA_BF16 || k < f_.q.paired || k < steps_ - 2;
+        return back_ || keep_ || c_.dtype != TOA_BF16 || !f_.q.halves || k < f_.q.paired || k < steps_ - 1;
     }
 
     // Steps taken by twos: where that is less work for the batch (see muon_kernels.hpp).
