@@ -25,7 +25,15 @@ toa_muon_series seriesOf(int steps, const Coefficients &c, double eps) {
     return {steps, c[0], c[1], c[2], eps};
 }
 
-// Same device and dtype throughout, and an element type the library serves.
+// Nothing here carries the tangents of forward-mode differentiation on: a result without one would
+// count as a constant.
+void requireNoTangent(const char *name, const TensorList &l) {
+    for (const Tensor &t : l)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t._fw_grad(/*level=*/0).defined(), name,
+                                    ": forward-mode derivatives are not served, got a dual tensor");
+}
+
+// Same device and dtype throughout, no tangents, and an element type the library serves.
 int gate(const char *name, const TensorList &l) {
     for (const Tensor &t : l) {
         if (!t.is_cuda()) throw std::runtime_error("Not implemented");
@@ -36,6 +44,7 @@ int gate(const char *name, const TensorList &l) {
         TORCH_CHECK(t.scalar_type() == l[0].scalar_type(), name, ": expected scalar type ",
                     l[0].scalar_type(), " but found ", t.scalar_type());
     }
+    requireNoTangent(name, l);
     const int code = dtypeCode(l[0], name);
     TORCH_CHECK(code != TOA_F64, "\"", name, "\" not implemented for 'Double'");
     return code;
@@ -231,6 +240,7 @@ void stepMulti(const char *name, const TensorList &out, TensorList grads, const 
     if (out.empty()) return;
     for (const Tensor &t : mu)
         if (!t.is_cuda()) throw std::runtime_error("Not implemented");
+    requireNoTangent(name, mu);
     TensorList all = out;
     all.insert(all.end(), grads.begin(), grads.end());
     const int code = gate(name, all);
@@ -243,6 +253,7 @@ void stepMulti(const char *name, const TensorList &out, TensorList grads, const 
     TORCH_CHECK(blocks != scales_o.is_none(), name,
                 blocks ? ": an 8-bit momentum needs its scales" : ": scales belong to an 8-bit momentum");
     const TensorList scales = blocks ? toTensorList(scales_o, "scales") : TensorList();
+    requireNoTangent(name, scales);
     TORCH_CHECK(!blocks || scales.size() == out.size(), name, ": tensor lists differ in length");
 
     std::vector<int64_t> rows(out.size()), cols(out.size());
@@ -355,6 +366,7 @@ py::object dequantizeMulti(const py::object &out_o, const py::object &codes_o,
                 ": tensor lists differ in length");
     if (out.empty()) return out_o;
     const int code = gate(name, out);
+    requireNoTangent(name, scales);
     std::vector<const int8_t *> src;
     std::vector<const float *> src_scales;
     std::vector<size_t> n;
