@@ -12,7 +12,10 @@ that one learning rate serves both), 1 for ``'none'``.
 
 A leaf of more than two dimensions is the matrix of its first dimension times all the others.
 In place the whole tree is one call per device and dtype, which overwrites updates and momentum.
-Out of place everything is differentiable with respect to updates and momentum.
+Out of place everything is differentiable with respect to updates and momentum.  Both ways a 16-bit
+momentum is the 64-bit sum rounded once, and the look-ahead and the result are held in 32 bits until the
+update is rounded to its type; the series may round differently, as `orthogonalize` takes the other way
+through its steps where a gradient is needed.
 """
 
 from __future__ import annotations
@@ -32,6 +35,7 @@ __all__ = ['ScaleByMuonState', 'scale_by_muon']
 
 ADJUST = (None, 'original', 'match_rms_adamw', 'none')
 BLOCK = 128  # elements that share a scale in an 8-bit momentum
+_HALVES = (torch.float16, torch.bfloat16)
 
 
 class ScaleByMuonState(NamedTuple):
@@ -159,12 +163,17 @@ def scale_by_muon(
             looked = []
             for k in live:
                 g, m = new_g[k], m_leaves[k]
-                new_m[k] = m.mul(momentum).add(g)
-                u = new_m[k].mul(momentum).add(g) if nesterov else new_m[k]
-                looked.append(u.flatten(1))
+                halves = m.dtype in _HALVES and g.dtype == m.dtype
+                if halves:
+                    # (a sum in 16 bits would round twice, and one in 32 with the decay rate as a
+                    # float breaks the ties of short binary fractions)
+                    new_m[k] = m.double().mul(momentum).add(g).to(m.dtype)
+                else:
+                    new_m[k] = m.mul(momentum).add(g)
+                u = new_m[k].float() if halves else new_m[k]
+                looked.append((u.mul(momentum).add(g) if nesterov else u).flatten(1))
             for k, o in zip(live, orthogonalize(looked, **series)):
                 g, r = new_g[k], shape_rate(new_g[k], adjust_lr_fn)
-                # (16-bit updates with a float32 momentum are orthogonalised in float32)
                 new_g[k] = (o if r == 1.0 else o.mul(r)).view(g.shape).to(g.dtype)
         return (_tree.rebuild(new_g, updates, g_spec),
                 ScaleByMuonState(momentum=_tree.rebuild(new_m, state.momentum, m_spec),
