@@ -100,12 +100,14 @@ class FusedMuon:
                                                         scales=tuple(s for _, s in kept))
 
     def state_dict(self) -> tuple:
-        """Per group ``(steps taken, ScaleByMuonState)``, or None before the first step."""
+        """Per group ``(steps taken, ScaleByMuonState)`` with the tensors that steps go on to change, or
+        None before the first step."""
         return tuple(None if s is None else (n, s) for n, s in zip(self._taken, self.state_groups))
 
     def load_state_dict(self, state_dict: Sequence[Any]) -> None:
-        """Takes the state of `state_dict()` back.  A momentum kept in another type (one in 8-bit
-        blocks into an optimizer that keeps float32, or the other way round) is converted."""
+        """Takes a copy of the state of `state_dict()`, which steps then leave as it is.  A momentum
+        kept in another type (one in 8-bit blocks into an optimizer that keeps float32, or the other
+        way round) is converted."""
         if len(state_dict) != len(self.param_groups):
             raise ValueError(f'expected the state of {len(self.param_groups)} groups, got '
                              f'{len(state_dict)}')
@@ -130,12 +132,12 @@ class FusedMuon:
 
     def _kept(self, p: torch.Tensor, m: torch.Tensor, scales: torch.Tensor | None):
         """A momentum and its scales in the type, place and memory layout this optimizer keeps for
-        `p`, from any other."""
+        `p`, from any other, in memory of their own."""
         kind = p.dtype if self.momentum_dtype is None else self.momentum_dtype
         same_layout = m.stride() == torch.empty_like(p, device='meta').stride()
-        m = m.to(p.device)
+        m = m.detach().to(p.device, copy=True)
         if scales is not None:
-            scales = scales.to(p.device)
+            scales = scales.detach().to(p.device, copy=True)
             if kind == torch.int8 and same_layout:
                 return m, scales
             m = dequantize_blocks(m, scales, torch.float32)
