@@ -50,11 +50,11 @@ def check_muon(momentum: float, ns_steps: int, ns_coefficients: tuple, eps: floa
     """Refuses hyper-parameters that the operator does not take."""
     if not 0.0 <= momentum < 1.0:
         raise ValueError(f'Invalid momentum value: {momentum}')
-    if not 1 <= ns_steps <= 32:
-        raise ValueError(f'Invalid ns_steps value: {ns_steps} (1 to 32)')
+    if int(ns_steps) != ns_steps or not 1 <= ns_steps <= 32:
+        raise ValueError(f'Invalid ns_steps value: {ns_steps} (a whole number, 1 to 32)')
     if len(ns_coefficients) != 3 or not all(math.isfinite(c) for c in ns_coefficients):
         raise ValueError(f'Invalid ns_coefficients: {ns_coefficients} (three finite numbers)')
-    if not eps >= 0.0:
+    if not 0.0 <= eps < math.inf:
         raise ValueError(f'Invalid epsilon value: {eps}')
     if adjust_lr_fn not in ADJUST:
         raise ValueError(f'Invalid adjust_lr_fn: {adjust_lr_fn!r}')
