@@ -26,7 +26,8 @@
  *   dtype     TOA_F32, TOA_F16 or TOA_BF16 (codes of toa_adam.h); all views of a call share it,
  *             except the momentum, whose type is given apart.
  *   precision products run on the matrix cores with float32 sums.  Their operands carry 22
- *             significant bits (two halves).  In a bfloat16 call that keeps no iterates, those of
+ *             significant bits (two halves): float32 results are about as far off as those of plain
+ *             float32 products.  In a bfloat16 call that keeps no iterates, those of
  *             the last orthogonalisation step may carry 11, where the coefficients keep what that
  *             adds within half a step of bfloat16 (the default ones do not).
  *   workspace device memory the call may overwrite, 256-byte aligned, as many bytes as the

@@ -23,8 +23,8 @@
 //
 // Operands.  The matrix cores multiply halves; an operand element is kept as hi + lo, two halves
 // that together carry 22 bits, and a product is hi hi + hi lo + lo hi with float32 sums (what is
-// dropped, lo lo, is 2^-22 of it).  Halves have few exponents, so every matrix is stored times a
-// power of two that takes its bound to 2^13..2^14: |X_k| <= max of the polynomial on the previous
+// dropped, lo lo, is 2^-24 of it on average; small_kernel, whose sums are too short to hide that, has
+// it in float32).  Halves have few exponents, so every matrix is stored times a power of two that takes its bound to 2^13..2^14: |X_k| <= max of the polynomial on the previous
 // interval (from the start's norm, 1 or less), and products of such bounds for the others.  An
 // element is at most the spectral norm, so nothing overflows, and what lies 2^-15 below the bound
 // still has all its bits.  ("half" operands keep hi alone: 11 bits, in the last step of bfloat16 calls
@@ -1356,9 +1356,9 @@ __global__ __launch_bounds__(256) void square_kernel(SquareArgs a) {
 //
 // Up to 32 rows and 864 columns, or 64 and 224: one workgroup takes a matrix through everything, and
 // the iterates never leave its LDS.  What a small matrix costs is not arithmetic but the way through
-// nineteen launches: three of 32 x 288 take 22 us here and 125 through the tiles, with their gradient
-// 76 and 389.  Of the 22, 5 are the norm and the factors, 6 the way into LDS, 2 each step, of which the
-// sums over the waves take most.
+// nineteen launches: three float32 ones of 32 x 288 take 24 us here and 125 through the tiles, with their
+// gradient 85 and 389.  Of the 24, 5 are the norm and the factors, 6 the way into LDS, 2.4 each step, of
+// which the sums over the waves take most.
 //
 // Eight waves share the columns by blocks of 32.  A block's result of a matrix instruction has a
 // column in each lane and rows in its registers (layout C); that is just the layout of the right
@@ -1401,10 +1401,12 @@ struct Pair {
     __device__ float value(int i) const { return (float)hi[i >> 3][i & 7] + (float)lo[i >> 3][i & 7]; }
 };
 
-__device__ inline f32x16 multiply(const Pair &a, const Pair &b, f32x16 sum) {
+// ALL: with lo lo, for float32 (see the top).
+template <bool ALL> __device__ inline f32x16 product(const Pair &a, const Pair &b, f32x16 sum) {
     beforeMatrix();
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
+        if (ALL) sum = mfma(a.lo[t], b.lo[t], sum);
         sum = mfma(a.lo[t], b.hi[t], sum);
         sum = mfma(a.hi[t], b.lo[t], sum);
         sum = mfma(a.hi[t], b.hi[t], sum);
@@ -1414,10 +1416,15 @@ __device__ inline f32x16 multiply(const Pair &a, const Pair &b, f32x16 sum) {
 }
 
 // p x into one sum and x p into another, by turns: neither waits for its own last result.
-__device__ inline void multiplyBoth(const Pair &p, const Pair &x, f32x16 &px, f32x16 &xp) {
+template <bool ALL>
+__device__ inline void productBoth(const Pair &p, const Pair &x, f32x16 &px, f32x16 &xp) {
     beforeMatrix();
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
+        if (ALL) {
+            px = mfma(p.lo[t], x.lo[t], px);
+            xp = mfma(x.lo[t], p.lo[t], xp);
+        }
         px = mfma(p.lo[t], x.hi[t], px);
         xp = mfma(x.hi[t], p.lo[t], xp);
         px = mfma(p.hi[t], x.lo[t], px);
@@ -1532,6 +1539,11 @@ __global__ __launch_bounds__(kSmallWaves * 64) void small_kernel(SmallArgs a) {
     __shared__ double sums[kSmallWaves];
     __shared__ SeriesTable table;
 
+    constexpr bool kAll = std::is_same<T, float>::value;
+    auto multiply = [](const Pair &x, const Pair &y, const f32x16 &sum) { return product<kAll>(x, y, sum); };
+    auto multiplyBoth = [](const Pair &p, const Pair &x, f32x16 &px, f32x16 &xp) {
+        productBoth<kAll>(p, x, px, xp);
+    };
     const MatRec r = uniform(a.recs ? a.recs + blockIdx.x : a.r + blockIdx.x);
     const int s = r.s, w = r.w, steps = a.q.steps;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

@@ -401,6 +401,10 @@ template <typename T, int RB> auto smallKernel(const Call &c) {
 int runSmall(const Call &c, const SmallBatch &b, const Series &series) {
     SmallArgs a{};
     a.q = series;
+    // float32: S without h I, whose rounding is a good part of what a sum over few columns is off by
+    // (16 x 16: 1.6e-6 with it, 6e-7 without and with all partial products, plain float32 8e-7; 22 -> 24
+    // us for three of 32 x 288, their gradient 78 -> 85)
+    if (c.dtype == TOA_F32) a.q.square = 0;
     a.step = stepOf(c);
     a.apply = c.hyper && c.hyper->apply;
     a.stride = b.stride;
