@@ -122,3 +122,48 @@ def test_float32_is_as_exact_as_plain_float32(m, n):
     off = float((orthogonalize(x.cuda()).double().cpu() - exact).norm())
     usual = float((plain_float32(x).double() - exact).norm())
     assert off <= 1.53 * usual, f'{m} x {n}: {off / usual:.2f}'
+
+
+@pytest.mark.parametrize('m,n', [(100, 100), (128, 128), (100, 900), (200, 256), (512, 512)])
+def test_gradients_at_rank_one(m, n):
+    """Most of such a gradient is the cotangent times a in every step, and what is off in the multiple of
+    the unit matrix in P is off everywhere.  A step's average errors, relative to a = 3.44: h + S_ii is
+    rounded by 5.2e-8, which c (h + S)^2 makes 7.2e-8; P's diagonal by 5.2e-8; the cotangent by 5.2e-8 and
+    in its sum by 3e-8 (6e-8): 1.1e-7 together; and lo lo, which is dropped, is c / a * 2^-22 / 3 = 4.7e-8 on
+    the diagonal, always to one side.  1.6e-7 a step, if all of it adds up over the steps; 1.5 * 2^-23 are
+    allowed."""
+    x = low_rank(m, n, 1)
+    dy = randn(m, n, seed=5)
+    exact = plain.gradient(x.double(), dy.double())
+    dx, = muon_op.orthogonalize_backward_multi([dy.cuda()], [x.cuda()])
+    off = float((dx.double().cpu() - exact).norm() / exact.norm())
+    assert off <= 5 * 1.5 * 2.0 ** -23, f'{off:.3g}'
+
+
+def plain_float32_gradient(x, dy, steps=5):
+    a, b, c = plain.COEFFICIENTS
+    size = x.square().sum((1, 2), keepdim=True).sqrt()
+    xs, g = [x / (size + 1e-7)], x
+    for _ in range(steps - 1):
+        s = xs[-1] @ xs[-1].mT
+        xs.append(a * xs[-1] + (b * s + c * (s @ s)) @ xs[-1])
+    y = dy
+    for x in reversed(xs):
+        s = x @ x.mT
+        z = y @ x.mT
+        m = z + z.mT
+        ms = m @ s
+        y = a * y + (b * s + c * (s @ s)) @ y + (b * m + c * (ms + ms.mT)) @ x
+    along = (y * g).sum((1, 2), keepdim=True) / (size * (size + 1e-7))
+    return (y - g * along) / (size + 1e-7)
+
+
+@pytest.mark.parametrize('m,n', [(16, 16), (32, 288), (65, 65), (100, 100), (100, 300), (200, 256)])
+def test_float32_gradients_are_as_exact_as_plain_float32(m, n):
+    """As for the results: operands off by 1.53 times what float32's are, sums alike."""
+    x, dy = randn(16, m, n, seed=m + n), randn(16, m, n, seed=m + n + 1)
+    exact = torch.stack([plain.gradient(g, d) for g, d in zip(x.double(), dy.double())])
+    dx, = muon_op.orthogonalize_backward_multi([dy.cuda()], [x.cuda()])
+    off = float((dx.double().cpu() - exact).norm())
+    usual = float((plain_float32_gradient(x, dy).double() - exact).norm())
+    assert off <= 1.53 * usual, f'{m} x {n}: {off / usual:.2f}'

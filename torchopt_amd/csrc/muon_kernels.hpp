@@ -395,7 +395,7 @@ struct Series {
     int paired;                     // so many steps are taken by twos
     int halves;                     // bfloat16: the last step's operands may carry 11 bits
     float a, b, c;
-    double eps, h;
+    double eps, h, unit;            // unit: the multiple of I in P
     double x[kMaxSteps + 1];        // bound of |X_k| from a start of norm 1
     double r[kMaxSteps];            // bound of |p(t) / t| on [0, x_k], which is |P|'s
     double d[kMaxSteps];            // bound of |p'| on [0, x_k]
@@ -475,13 +475,12 @@ __device__ inline void pairFactors(const Bounds &b, int t, Factor *f) {
     const int ex = expOf(x), es = expOf(x2), ep = expOf(r), et = expOf(r * x2), eq = expOf(r * r1);
     const int es1 = expOf(q.square ? fmax(fabs(q.h), fabs(q.h + x1 * x1)) : x1 * x1), ep1 = expOf(r1);
     const int ex2 = t + 2 == q.steps ? 0 : expOf(b.x(t + 2));
-    const double unit = q.square ? (double)q.a - (double)q.b * q.h * 0.5 : (double)q.a;
     f[0] = {ldexpf(1.f, es - 2 * ex), 0.f, 1.f, 0.f};
     f[1] = {ldexpf(q.c, ep - 2 * es), ldexpf(q.b, ep - es), 1.f, ldexpf(q.a, ep)};
     f[2] = {ldexpf(1.f, et - ep - es), 0.f, 1.f, 0.f};
     f[3] = {ldexpf(1.f, es1 - et - ep), 0.f, 1.f, (float)(q.square ? ldexp(q.h, es1) : 0.0)};
     f[4] = {ldexpf(q.c, ep1 - 2 * es1), q.square ? 0.f : ldexpf(q.b, ep1 - es1), 1.f,
-            (float)ldexp(unit, ep1)};
+            (float)ldexp(q.unit, ep1)};
     f[5] = {ldexpf(1.f, eq - ep1 - ep), 0.f, 1.f, 0.f};
     f[6] = {ldexpf(1.f, ex2 - eq - ex), 0.f, 1.f, 0.f};
 }
@@ -495,9 +494,8 @@ __device__ inline void stepFactors(const Bounds &b, int t, Factor *f, Factor *ba
     const bool last = t + 1 == q.steps;
     const int ex1 = last && !back ? 0 : expOf(b.x(t + 1));
     const float add = q.square ? 0.f : q.b;
-    const double unit = q.square ? (double)q.a - (double)q.b * q.h * 0.5 : (double)q.a;
     f[0] = {ldexpf(1.f, es - 2 * ex), 0.f, 1.f, (float)(q.square ? ldexp(q.h, es) : 0.0)};
-    f[1] = {ldexpf(q.c, ep - 2 * es), ldexpf(add, ep - es), 1.f, (float)ldexp(unit, ep)};
+    f[1] = {ldexpf(q.c, ep - 2 * es), ldexpf(add, ep - es), 1.f, (float)ldexp(q.unit, ep)};
     f[2] = {ldexpf(1.f, ex1 - ep - ex), 0.f, 1.f, 0.f};
     if (!back) return;
     const double y1 = b.y(t + 1);

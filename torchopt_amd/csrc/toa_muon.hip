@@ -292,6 +292,22 @@ int boundsOf(const toa_muon_series &q, Series &f) {
     // at most
     f.h = q.c != 0.0 ? q.b / (2.0 * q.c) : 0.0;
     f.square = q.c != 0.0 && std::fabs(q.c) * f.h * f.h <= 2.0 * std::fabs(q.a);
+    // What is off in the multiple of I in P is off everywhere, and in every step: where S is small beside it
+    // (few large singular values) it is most of the error.  So h is a number that an operand holds exactly,
+    // and the multiple of I that P is given takes what the product makes of it -- with c as a float, and
+    // without the square of h's low half -- to a.  (a - b h / 2, with h and b each rounded by itself: 1.3e-6
+    // off in gradients of rank one, now 7e-7; 100 x 100 of full rank 1.1e-6, now 9e-7.)
+    f.unit = q.a;
+    if (f.square) {
+        auto half = [](double v) {
+            int e;
+            const double m = std::frexp(v, &e);
+            return std::ldexp(std::nearbyint(std::ldexp(m, 11)), e - 11);
+        };
+        const double exact = (float)f.h, hi = half(exact), lo = half(exact - hi);
+        f.h = hi + lo;
+        f.unit = q.a - (double)f.c * (f.h * f.h - lo * lo);
+    }
     // Operands of 11 bits in the last step, each element off by 2^-12 of itself: that of X moves the
     // result by the slope, that of S (or S + h I, as it is kept) by what P changes with it, that of P by P
     // itself, all beside a result of |P X| >= (least |P|) |X|.  Up to 8 times 2^-12 is half a step of
@@ -404,7 +420,10 @@ int runSmall(const Call &c, const SmallBatch &b, const Series &series) {
     // float32: S without h I, whose rounding is a good part of what a sum over few columns is off by
     // (16 x 16: 1.6e-6 with it, 6e-7 without and with all partial products, plain float32 8e-7; 22 -> 24
     // us for three of 32 x 288, their gradient 78 -> 85)
-    if (c.dtype == TOA_F32) a.q.square = 0;
+    if (c.dtype == TOA_F32) {
+        a.q.square = 0;
+        a.q.unit = c.series.a;
+    }
     a.step = stepOf(c);
     a.apply = c.hyper && c.hyper->apply;
     a.stride = b.stride;
