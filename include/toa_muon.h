@@ -67,7 +67,7 @@ typedef struct {
 } toa_muon_view;
 
 /* 1 <= steps <= 32; coefficients finite, and such that no iterate but the last can grow beyond 64
- * from a start of norm 1 (TOA_EVALUE otherwise); eps >= 0. */
+ * from a start of norm 1, and the last not beyond 1e30 (TOA_EVALUE otherwise); eps >= 0. */
 typedef struct {
     int steps;
     double a, b, c, eps;

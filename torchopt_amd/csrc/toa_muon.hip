@@ -285,6 +285,8 @@ int boundsOf(const toa_muon_series &q, Series &f) {
         if (k == q.steps) break;
         f.r[k] = std::max(1.01 * largest(q.a, q.b, q.c, 0, f.x[k]), 1e-3);
         f.d[k] = std::max(1.01 * largest(q.a, 3.0 * q.b, 5.0 * q.c, 0, f.x[k]), 1e-3);
+        // (operands are scaled by 2^-110 at most)
+        if (!(std::max(f.r[k], f.d[k]) <= 1e30)) return TOA_EVALUE;
         x = std::max(largest(q.a, q.b, q.c, 1, f.x[k]), 1e-6);
         if (k + 1 < q.steps && !(x <= 64.0)) return TOA_EVALUE;
     }
