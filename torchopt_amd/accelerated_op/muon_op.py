@@ -148,7 +148,8 @@ def quantize_blocks(tensors: torch.Tensor | Sequence[torch.Tensor]):
     Each 128 consecutive elements in memory order (the last ones may be fewer) share one float32
     scale, the largest magnitude among them over 127; the int8 code of an element is its multiple
     of the scale, rounded half to even.  So an element is off by half a scale at most, and a block
-    of zeros stays one.  A block with a NaN or an infinity stands for NaN throughout."""
+    of zeros stays one.  A block with a NaN or an infinity stands for NaN throughout.  Neither this nor
+    `dequantize_blocks` is differentiable."""
     if isinstance(tensors, torch.Tensor):
         codes, scales = muon_op.quantize_multi([tensors])
         return codes[0], scales[0]

@@ -15,9 +15,9 @@ using namespace toa_muon;
 namespace {
 
 // A batch's regions stay below this (one matrix alone may be larger).  Large batches fill whole
-// rounds of tiles: 96 matrices of 1024^2 take 7.1 ms in one batch and 7.9 in three, GPT-2-medium's 144
-// matrices (bfloat16 step) 13.2 ms in two batches, 14.2 in 1 GiB and 17.4 in 256 MiB, which stay in the
-// last-level cache.  (In one of 8 GiB they take 13.9: pairs of steps then serve the square ones too.)
+// rounds of tiles: 96 matrices of 1024^2 take 7.2 ms in one batch and 8.0 in three, GPT-2-medium's 144
+// matrices (bfloat16 step) 16.4 ms in two batches, 17.6 in 1 GiB and 21.4 in 256 MiB, which stay in the
+// last-level cache.  (One of 8 GiB and two of 4 take the same, side by side: 15.9.)
 constexpr int64_t kBatchBytes = (int64_t)4 << 30;
 constexpr int kBatchMats = 4096;
 constexpr int64_t kMaxDim = (int64_t)1 << 20;
@@ -124,13 +124,16 @@ struct SmallBatch {
 
 // The way back bounds each cotangent by the one before.  Bounds that run ahead of the truth cost the
 // operands their low bits, so where a bound may have grown by more than this the norm is measured anew
-// (the default coefficients: 392 at their five steps, so never there).
+// (the default coefficients: 394 at their five steps, so never there).
 constexpr double kMaxGrowth = 512.0;
 
 // Tiles of 64 x 64 that small matrices may add to the launches of larger ones (which hold 512 at once).
 constexpr int64_t kFewTiles = 128;
 
-// Rows / 32 of the variant that takes an s x w matrix, or 0.
+// Rows / 32 of the variant that takes an s x w matrix, or 0: what its LDS holds.  The one for 64 rows spills
+// 55 to 65 registers, and is ahead of the tiles or level with them all the same: one 64 x 64 float32 matrix 52
+// us (77), its gradient 154 (193); one 33 x 224 62 (64) and 189 (200), one 64 x 224 64 (63) and 198 (197); 256
+// of these 94 (124) and 313 (431).
 int smallVariant(int64_t s, int64_t w) {
     for (int rb = 1; rb <= 2; ++rb)
         if (s <= 32 * rb) return w <= 32 * smallColumnBlocks(rb) ? rb : 0;
@@ -646,7 +649,8 @@ class Run {
     // takes between the two: the large tiles as the square of the share filled; the 128 x 128 of which
     // two fit on a compute unit little more than one alone up to one to a unit, and most of a round
     // beyond; the 64 x 64 follow each other without rounds.
-    // Microseconds fitted to 1..48 matrices of 1024^2, 2048^2, 4096^2, 16 x 512^2 and 64 x 256^2, to
+    // Microseconds of whole launches -- so with their start, the change of workgroups and the last to end --
+    // fitted to 1..48 matrices of 1024^2, 2048^2, 4096^2, 16 x 512^2 and 64 x 256^2, to
     // 3..10 % (the 64 x 64 then 8 % up: long lists of different operands miss the L2 more); the variant
     // chosen is 0.3 % from the best of the four on average, 7 % at most.  Large
     // tiles get most out of a full chip (P X of 48 matrices of 1024^2: 324 us in 256 x 256, 379, 400

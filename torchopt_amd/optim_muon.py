@@ -2,7 +2,9 @@
 orthogonalisation, weight decay and the addition to the parameters -- on the operators of
 `torchopt_amd._C.muon_op`, one call per device and dtype for any number of parameters.
 
-The reference has no counterpart.  Constructor arguments are those of ``torch.optim.Muon``.  The step:
+The reference has no counterpart.  Constructor arguments are those of ``torch.optim.Muon``; parameters come as
+tensors (dicts of groups are refused, `add_param_group` takes another list), with the same settings for all
+groups.  The step:
 
     ``M <- momentum * M + g``,   ``U = g + momentum * M`` (``nesterov``; else ``U = M``),
     ``P <- (1 - lr * weight_decay) * P - lr * r * orthogonalize(U)``
@@ -11,6 +13,10 @@ with ``r`` after `adjust_lr_fn` (see `scale_by_muon`).  Beside ``torch.optim.Muo
 
   * the momentum is the plain sum, not the mean of the gradients, which is ``1 - momentum`` times it;
     the normalisation takes the factor out again (but for `eps`);
+  * the series runs on operands of 22 significant bits with float32 sums, not in bfloat16, whatever the
+    parameters' type;
+  * `ns_steps` is at most 32 (there 99), and coefficients under which an iterate could grow beyond 64 are
+    refused by the first step;
   * parameters of more than two dimensions are taken too, as the matrix of their first dimension
     times all the others (a convolution's kernel); vectors and scalars are refused;
   * `momentum_dtype=torch.int8` keeps the momentum in 8-bit blocks: a quarter of float32's
